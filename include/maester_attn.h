@@ -190,6 +190,29 @@ int ma_ce_rows(void* logits, int64_t pitch, const int64_t* targets, int64_t rows
 int ma_ce_loss_reduce(const float* nll, int64_t n, const float* scale, float* loss, void* stream);
 int ma_transpose(const void* src, void* dst, int64_t rows, int64_t cols, int src_dtype, int dst_dtype, void* stream);
 
+/* ---- log-probabilities of given tokens -----------------------------------------------------------------
+ * The per-token form of the loss above, for objectives that weigh tokens themselves (policy, preference,
+ * distillation) and for scoring.  No counterpart in the reference, whose loss is the scalar alone.
+ * logits: [rows, vocab] of dtype, `pitch` elements between rows, any alignment; targets: int64 [rows].
+ * y_j = x_j / temperature, with softcap > 0 first x = softcap * tanh(x / softcap).  All outputs fp32:
+ *   logp[row] = y_target - log sum exp y, entropy[row] = -sum p log p, both 0 for a row that does not
+ *   count (target == ignore_index or outside [0, vocab)); stats[row] = {max of temperature * y,
+ *   log sum exp(y - max y)}, [rows, 2], for the backward (may be NULL).
+ *   top_ids int64 / top_logp fp32 [rows, top_k]: the top_k largest logits, best first, equal ones by
+ *   ascending index (a NaN logit ranks with -inf), for every row; NULL with top_k = 0.
+ * Logits of -inf have probability 0.  A row with a NaN or +inf, or with nothing but -inf, has NaN
+ * outputs.  ma_token_logprobs_bwd: dlogits (rows `dpitch` apart, may alias logits) =
+ *   dlogp * d logp + dentropy * d entropy, zeros for a row that does not count; either of dlogp /
+ *   dentropy (fp32 [rows]) may be NULL (= 0); stats and entropy as the forward wrote them. */
+#define MA_LOGPROBS_MAX_TOP 64
+#define MA_LOGPROBS_MAX_VOCAB ((1 << 30) - 1)
+int ma_token_logprobs_fwd(const void* logits, int64_t pitch, const int64_t* targets, int64_t rows, int64_t vocab,
+                          int64_t ignore_index, float softcap, float temperature, int top_k, float* logp, float* entropy,
+                          float* stats, int64_t* top_ids, float* top_logp, int dtype, void* stream);
+int ma_token_logprobs_bwd(const void* logits, int64_t pitch, const int64_t* targets, int64_t rows, int64_t vocab,
+                          int64_t ignore_index, float softcap, float temperature, const float* stats, const float* entropy,
+                          const float* dlogp, const float* dentropy, void* dlogits, int64_t dpitch, int dtype, void* stream);
+
 /* ---- fused QK-RMSNorm + RoPE prologue ------------------------------------------------------------
  * Replaces query_norm/key_norm (model.py:135-172, 366-368) followed by apply_rotary_emb
  * (model.py:97-106, 371-372) with the table gather by position_ids (model.py:744-747):

@@ -222,6 +222,54 @@ int ma_ce_loss_reduce(const float* nll, int64_t n, const float* scale, float* lo
     return launch_ce_loss_reduce(nll, n, scale, loss, (hipStream_t)stream);
 }
 
+static int check_logprobs(const char* who, const void* logits, int64_t pitch, const int64_t* targets, int64_t rows, int64_t vocab,
+                          float softcap, float temperature, int dtype) {
+    MA_TRY(check_dtype(who, dtype));
+    if (!logits || !targets) return fail(MA_ERR_BAD_ARG, "%s: logits / targets is NULL", who);
+    if (rows <= 0) return fail(MA_ERR_BAD_ARG, "%s: rows=%lld must be positive", who, (long long)rows);
+    // one workgroup of 512 threads a row: a launch has fewer than 2^32 threads
+    if (rows >= ((int64_t)1 << 23)) return fail(MA_ERR_UNSUPPORTED, "%s: rows=%lld is 2^23 or more", who, (long long)rows);
+    if (vocab <= 0 || vocab > MA_LOGPROBS_MAX_VOCAB) return fail(MA_ERR_BAD_ARG, "%s: vocab=%lld out of range", who, (long long)vocab);
+    if (pitch < vocab) return fail(MA_ERR_BAD_ARG, "%s: pitch=%lld is below vocab=%lld", who, (long long)pitch, (long long)vocab);
+    if (!(softcap >= 0.f) || softcap > 1e30f) return fail(MA_ERR_BAD_ARG, "%s: softcap must be >= 0 (0 = none) and finite", who);
+    if (!(temperature > 1e-6f) || temperature > 1e6f) return fail(MA_ERR_BAD_ARG, "%s: temperature must be in (1e-6, 1e6]", who);
+    if (((uintptr_t)logits & (dtype == MA_DTYPE_BF16 ? 1 : 3)) != 0)
+        return fail(MA_ERR_BAD_ARG, "%s: logits not aligned to its element size", who);
+    return MA_OK;
+}
+
+int ma_token_logprobs_fwd(const void* logits, int64_t pitch, const int64_t* targets, int64_t rows, int64_t vocab,
+                          int64_t ignore_index, float softcap, float temperature, int top_k, float* logp, float* entropy,
+                          float* stats, int64_t* top_ids, float* top_logp, int dtype, void* stream) {
+    const char* who = "ma_token_logprobs_fwd";
+    MA_TRY(check_logprobs(who, logits, pitch, targets, rows, vocab, softcap, temperature, dtype));
+    if (top_k < 0 || top_k > MA_LOGPROBS_MAX_TOP || top_k > vocab)
+        return fail(MA_ERR_BAD_ARG, "%s: top_k=%d must be in 0 .. %d and at most vocab=%lld", who, top_k, MA_LOGPROBS_MAX_TOP, (long long)vocab);
+    if (!logp || !entropy) return fail(MA_ERR_BAD_ARG, "%s: logp / entropy is NULL", who);
+    if (((uintptr_t)stats & 7) != 0) return fail(MA_ERR_BAD_ARG, "%s: stats not 8-byte aligned", who);
+    if (top_k > 0 && (!top_ids || !top_logp)) return fail(MA_ERR_BAD_ARG, "%s: top_ids / top_logp is NULL with top_k=%d", who, top_k);
+    TokenLogprobsArgs a = {logits, pitch, targets, rows, vocab, ignore_index, softcap, temperature, top_k, logp, entropy, stats,
+                           top_ids, top_logp, nullptr, nullptr, nullptr, 0};
+    return launch_token_logprobs_fwd(a, dtype, (hipStream_t)stream);
+}
+
+int ma_token_logprobs_bwd(const void* logits, int64_t pitch, const int64_t* targets, int64_t rows, int64_t vocab,
+                          int64_t ignore_index, float softcap, float temperature, const float* stats, const float* entropy,
+                          const float* dlogp, const float* dentropy, void* dlogits, int64_t dpitch, int dtype, void* stream) {
+    const char* who = "ma_token_logprobs_bwd";
+    MA_TRY(check_logprobs(who, logits, pitch, targets, rows, vocab, softcap, temperature, dtype));
+    if (!stats || !entropy || !dlogits) return fail(MA_ERR_BAD_ARG, "%s: stats / entropy / dlogits is NULL", who);
+    if (dpitch < vocab) return fail(MA_ERR_BAD_ARG, "%s: dpitch=%lld is below vocab=%lld", who, (long long)dpitch, (long long)vocab);
+    if (((uintptr_t)dlogits & (dtype == MA_DTYPE_BF16 ? 1 : 3)) != 0)
+        return fail(MA_ERR_BAD_ARG, "%s: dlogits not aligned to its element size", who);
+    // workgroups of 256 threads: a launch has fewer than 2^32 threads
+    if (rows * token_logprobs_bwd_chunks(vocab) >= ((int64_t)1 << 24))
+        return fail(MA_ERR_UNSUPPORTED, "%s: rows=%lld of vocab=%lld exceed the grid limit", who, (long long)rows, (long long)vocab);
+    TokenLogprobsArgs a = {logits, pitch, targets, rows, vocab, ignore_index, softcap, temperature, 0, nullptr, (float*)entropy,
+                           (float*)stats, nullptr, nullptr, dlogp, dentropy, dlogits, dpitch};
+    return launch_token_logprobs_bwd(a, dtype, (hipStream_t)stream);
+}
+
 int ma_packed_ids_build(const int32_t* starts, const int32_t* lengths, const int32_t* counts, int B, int max_docs, int S,
                         int64_t* position_ids, int64_t* document_ids, void* stream) {
     const char* who = "ma_packed_ids_build";

@@ -59,6 +59,24 @@ int launch_transpose(const void* src, void* dst, int64_t rows, int64_t cols, int
 int launch_ce_valid_count(const int64_t* targets, int64_t n, int64_t ignore_index, int vocab, float* stats, hipStream_t stream);
 int launch_ce_loss_reduce(const float* nll, int64_t n, const float* scale, float* loss, hipStream_t stream);
 
+struct TokenLogprobsArgs {
+    const void* logits;
+    int64_t pitch;
+    const int64_t* targets;
+    int64_t rows, vocab, ignore_index;
+    float softcap, temperature;
+    int top_k;
+    float *logp, *entropy, *stats;        // outputs of the forward, entropy and stats inputs of the backward
+    int64_t* top_ids;
+    float* top_logp;
+    const float *dlogp, *dentropy;
+    void* dlogits;
+    int64_t dpitch;
+};
+int token_logprobs_bwd_chunks(int64_t vocab);
+int launch_token_logprobs_fwd(const TokenLogprobsArgs& a, int dtype, hipStream_t st);
+int launch_token_logprobs_bwd(const TokenLogprobsArgs& a, int dtype, hipStream_t st);
+
 struct AttnArgs {
     ma_tensor4 q, k, v, o, dout, dq, dk, dv;
     float* lse;

@@ -1,0 +1,60 @@
+"""Argument checks of the log-probability entry points, before any launch (no GPU), and the oracle's own pins."""
+import numpy as np
+import pytest
+import torch
+import torch.nn.functional as F
+
+from maester_amd import _lib, token_logprobs
+from oracle import token_logprobs as O
+
+P = 0x1000
+NAN = float("nan")
+
+
+def _fwd(logits=P, pitch=100, targets=P, rows=4, vocab=100, cap=0.0, temp=1.0, k=0, logp=P, ent=P, ids=P, top=P, dtype=1):
+    return _lib.lib().ma_token_logprobs_fwd(logits, pitch, targets, rows, vocab, -100, cap, temp, k, logp, ent, None, ids, top, dtype, None)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(logits=None), -1, "NULL"), (dict(targets=None), -1, "NULL"), (dict(logp=None), -1, "logp"), (dict(rows=0), -1, "rows"),
+    (dict(rows=1 << 23), -2, "rows"), (dict(vocab=0), -1, "vocab"), (dict(vocab=1 << 30, pitch=1 << 31), -1, "vocab"),
+    (dict(pitch=99), -1, "pitch"), (dict(cap=-1.0), -1, "softcap"), (dict(cap=NAN), -1, "softcap"), (dict(temp=0.0), -1, "temperature"),
+    (dict(temp=NAN), -1, "temperature"), (dict(k=65), -1, "top_k"), (dict(k=-1), -1, "top_k"), (dict(k=6, vocab=5), -1, "top_k"),
+    (dict(k=2, ids=None), -1, "top_ids"), (dict(dtype=7), -1, "dtype"), (dict(logits=P + 1), -1, "aligned")])
+def test_forward_refusals(kw, code, text):
+    assert _fwd(**kw) == code and text in _lib.lib().ma_last_error().decode()
+
+
+def _bwd(logits=P, pitch=100, rows=4, vocab=100, stats=P, ent=P, dx=P, dpitch=100, dtype=0):
+    return _lib.lib().ma_token_logprobs_bwd(logits, pitch, P, rows, vocab, -100, 0.0, 1.0, stats, ent, P, P, dx, dpitch, dtype, None)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(logits=None), -1, "NULL"), (dict(stats=None), -1, "stats"), (dict(dx=None), -1, "dlogits"), (dict(dpitch=99), -1, "dpitch"),
+    (dict(dx=P + 2), -1, "aligned"), (dict(rows=1 << 20, vocab=262208, pitch=262208, dpitch=262208), -2, "grid")])
+def test_backward_refusals(kw, code, text):
+    assert _bwd(**kw) == code and text in _lib.lib().ma_last_error().decode()
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(RuntimeError):
+        token_logprobs(torch.zeros(2, 5), torch.zeros(2, dtype=torch.long))
+    with pytest.raises(ValueError):
+        token_logprobs(torch.zeros(2, 5), torch.zeros(3, dtype=torch.long))
+
+
+@pytest.mark.parametrize("softcap,temperature", [(None, 1.0), (4.0, 0.6)])
+def test_oracle_against_torch(softcap, temperature):
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(7, 31, generator=g, dtype=torch.float64).requires_grad_()
+    t = torch.randint(0, 31, (7,), generator=g)
+    t[2] = -100
+    a, b = torch.randn(7, generator=g, dtype=torch.float64), torch.randn(7, generator=g, dtype=torch.float64)
+    y = (softcap * torch.tanh(x / softcap) if softcap else x) / temperature
+    logp = -F.cross_entropy(y, t, ignore_index=-100, reduction="none")
+    entropy = torch.distributions.Categorical(logits=y).entropy() * (t != -100)
+    dx, = torch.autograd.grad((logp * a).sum() + (entropy * b).sum(), x)
+    out = O.rows(x.detach().numpy(), t.numpy(), 5, softcap=softcap, temperature=temperature, dlogp=a.numpy(), dentropy=b.numpy())
+    assert np.allclose(out["logp"], logp.detach().numpy(), atol=1e-12) and np.allclose(out["entropy"], entropy.detach().numpy(), atol=1e-12)
+    assert np.allclose(out["dx"], dx.numpy(), atol=1e-12)
+    assert np.array_equal(out["top_ids"], torch.sort(x.detach(), dim=1, descending=True, stable=True).indices[:, :5].numpy())
