@@ -200,15 +200,19 @@ int ma_transpose(const void* src, void* dst, int64_t rows, int64_t cols, int src
  *   log sum exp(y - max y)}, [rows, 2], for the backward (may be NULL).
  *   top_ids int64 / top_logp fp32 [rows, top_k]: the top_k largest logits, best first, equal ones by
  *   ascending index (a NaN logit ranks with -inf), for every row; NULL with top_k = 0.
+ *   workspace: at least ma_token_logprobs_workspace_bytes(...) bytes (0 with many rows: then it may be
+ *   NULL), 16-byte aligned, where the parts that few rows are cut into leave their results.
  * Logits of -inf have probability 0.  A row with a NaN or +inf, or with nothing but -inf, has NaN
  * outputs.  ma_token_logprobs_bwd: dlogits (rows `dpitch` apart, may alias logits) =
  *   dlogp * d logp + dentropy * d entropy, zeros for a row that does not count; either of dlogp /
  *   dentropy (fp32 [rows]) may be NULL (= 0); stats and entropy as the forward wrote them. */
 #define MA_LOGPROBS_MAX_TOP 64
 #define MA_LOGPROBS_MAX_VOCAB ((1 << 30) - 1)
+size_t ma_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_k);
 int ma_token_logprobs_fwd(const void* logits, int64_t pitch, const int64_t* targets, int64_t rows, int64_t vocab,
                           int64_t ignore_index, float softcap, float temperature, int top_k, float* logp, float* entropy,
-                          float* stats, int64_t* top_ids, float* top_logp, int dtype, void* stream);
+                          float* stats, int64_t* top_ids, float* top_logp, void* workspace, size_t workspace_bytes, int dtype,
+                          void* stream);
 int ma_token_logprobs_bwd(const void* logits, int64_t pitch, const int64_t* targets, int64_t rows, int64_t vocab,
                           int64_t ignore_index, float softcap, float temperature, const float* stats, const float* entropy,
                           const float* dlogp, const float* dentropy, void* dlogits, int64_t dpitch, int dtype, void* stream);

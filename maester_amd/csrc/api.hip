@@ -238,9 +238,15 @@ static int check_logprobs(const char* who, const void* logits, int64_t pitch, co
     return MA_OK;
 }
 
+size_t ma_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_k) {
+    if (rows <= 0 || vocab <= 0 || top_k < 0) return 0;
+    return token_logprobs_workspace_bytes(rows, vocab, top_k);
+}
+
 int ma_token_logprobs_fwd(const void* logits, int64_t pitch, const int64_t* targets, int64_t rows, int64_t vocab,
                           int64_t ignore_index, float softcap, float temperature, int top_k, float* logp, float* entropy,
-                          float* stats, int64_t* top_ids, float* top_logp, int dtype, void* stream) {
+                          float* stats, int64_t* top_ids, float* top_logp, void* workspace, size_t workspace_bytes, int dtype,
+                          void* stream) {
     const char* who = "ma_token_logprobs_fwd";
     MA_TRY(check_logprobs(who, logits, pitch, targets, rows, vocab, softcap, temperature, dtype));
     if (top_k < 0 || top_k > MA_LOGPROBS_MAX_TOP || top_k > vocab)
@@ -248,8 +254,11 @@ int ma_token_logprobs_fwd(const void* logits, int64_t pitch, const int64_t* targ
     if (!logp || !entropy) return fail(MA_ERR_BAD_ARG, "%s: logp / entropy is NULL", who);
     if (((uintptr_t)stats & 7) != 0) return fail(MA_ERR_BAD_ARG, "%s: stats not 8-byte aligned", who);
     if (top_k > 0 && (!top_ids || !top_logp)) return fail(MA_ERR_BAD_ARG, "%s: top_ids / top_logp is NULL with top_k=%d", who, top_k);
+    const size_t need = token_logprobs_workspace_bytes(rows, vocab, top_k);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0))
+        return fail(MA_ERR_BAD_ARG, "%s: workspace of %zu bytes, need %zu, 16-byte aligned", who, workspace ? workspace_bytes : (size_t)0, need);
     TokenLogprobsArgs a = {logits, pitch, targets, rows, vocab, ignore_index, softcap, temperature, top_k, logp, entropy, stats,
-                           top_ids, top_logp, nullptr, nullptr, nullptr, 0};
+                           top_ids, top_logp, nullptr, nullptr, nullptr, 0, workspace};
     return launch_token_logprobs_fwd(a, dtype, (hipStream_t)stream);
 }
 
@@ -266,7 +275,7 @@ int ma_token_logprobs_bwd(const void* logits, int64_t pitch, const int64_t* targ
     if (rows * token_logprobs_bwd_chunks(vocab) >= ((int64_t)1 << 24))
         return fail(MA_ERR_UNSUPPORTED, "%s: rows=%lld of vocab=%lld exceed the grid limit", who, (long long)rows, (long long)vocab);
     TokenLogprobsArgs a = {logits, pitch, targets, rows, vocab, ignore_index, softcap, temperature, 0, nullptr, (float*)entropy,
-                           (float*)stats, nullptr, nullptr, dlogp, dentropy, dlogits, dpitch};
+                           (float*)stats, nullptr, nullptr, dlogp, dentropy, dlogits, dpitch, nullptr};
     return launch_token_logprobs_bwd(a, dtype, (hipStream_t)stream);
 }
 

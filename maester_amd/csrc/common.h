@@ -72,7 +72,9 @@ struct TokenLogprobsArgs {
     const float *dlogp, *dentropy;
     void* dlogits;
     int64_t dpitch;
+    void* ws;
 };
+size_t token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_k);
 int token_logprobs_bwd_chunks(int64_t vocab);
 int launch_token_logprobs_fwd(const TokenLogprobsArgs& a, int dtype, hipStream_t st);
 int launch_token_logprobs_bwd(const TokenLogprobsArgs& a, int dtype, hipStream_t st);

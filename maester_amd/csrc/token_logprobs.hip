@@ -14,13 +14,19 @@
 #include "common.h"
 #include "rowio.h"
 
+#define MA_TRY(expr)            \
+    do {                        \
+        int rc__ = (expr);      \
+        if (rc__) return rc__;  \
+    } while (0)
+
 #pragma clang fp reassociate(off)
 
 namespace ma {
 
 namespace {
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 512;       // >= 8 * MA_LOGPROBS_MAX_TOP: the waves' best keys, one a thread
 constexpr int kLpWaves = kLpThreads / 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -139,25 +145,138 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t k) {
     return k;
 }
 
+// 64 keys of a wave, one a lane, into descending order
+__device__ __forceinline__ uint64_t wave_sort_descending(uint64_t k) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int size = 2; size <= 64; size <<= 1) {
+#pragma unroll
+        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+            const uint64_t o = __shfl_xor((unsigned long long)k, stride, 64);
+            const bool larger = ((lane & size) == 0) == ((lane & stride) == 0);   // this lane keeps the larger key
+            k = (o > k) == larger ? o : k;
+        }
+    }
+    return k;
+}
+
+// LDS of the selection: keys (one slot a thread), the number of them that are in use
+struct Selection {
+    uint64_t key[kLpThreads];
+    int count;
+};
+// Number of the n keys in LDS that are larger than `key`: its rank, as keys are unique.
+__device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int n) {
+    int rank = 0;
+    for (int i = 0; i < n; ++i) rank += keys[i] > key ? 1 : 0;
+    return rank;
+}
+// The `want` largest of the workgroup's per-thread keys (0: none), best first, in sel.key; returns how many there are
+// (fewer than `want` if not enough threads have a key).  Every wave sorts its own 64, the waves' best are ranked by
+// counting.  Ends with a barrier.
+__device__ __forceinline__ int best_of_threads(uint64_t key, int want, Selection& sel) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    key = wave_sort_descending(key);
+    if (threadIdx.x == 0) sel.count = 0;
+    __syncthreads();
+    if (lane < want) sel.key[wave * want + lane] = key;
+    if (lane < want && key) atomicAdd(&sel.count, 1);
+    __syncthreads();
+    const int n = kLpWaves * want, have = sel.count < want ? sel.count : want;
+    uint64_t mine = 0;
+    int rank = kLpThreads;
+    if ((int)threadIdx.x < n) {
+        mine = sel.key[threadIdx.x];
+        if (mine) rank = rank_of(mine, sel.key, n);
+    }
+    __syncthreads();
+    if (rank < want) sel.key[rank] = mine;
+    __syncthreads();
+    return have;
+}
+
+// ---- forward --------------------------------------------------------------------------------------------
+// A row is cut into `parts` runs of groups, one workgroup each, so that a few rows fill the chip as well; part 0..parts-1
+// of every row leave their statistics and their best keys in the workspace for token_logprobs_join_kernel (parts == 1:
+// the outputs are written here).
+//
+// The alternatives do not need the row again: while a thread streams its groups it remembers the best group of its own
+// (larger maximum, then lower index).  The k largest elements lie in the k threads whose best is largest, since any
+// other thread's elements are below k distinct ones; those threads' groups, k / 512 of the part, are read once more (from
+// cache) and what is not below the k-th best thread's maximum, a little over k elements, is ranked by counting.  If
+// those threads hold more than 512 such elements the k largest are taken one after another.  Against a pass over the row
+// per alternative: 4096 rows of 262208 bf16 logits with 8 alternatives 4.26 -> 0.42 ms (5.1 TB/s, a large copy moves
+// 4.8), one such row with 20 alternatives, cut into 64 parts, 909 -> 18 us in the two kernels.
+struct Outputs {
+    float *logp, *entropy, *stats;
+    int64_t* top_ids;
+    float* top_logp;
+};
+struct Workspace {
+    Stats* stats;      // [rows, parts]
+    uint64_t* keys;    // [rows, parts, top_k]
+};
+
 template <typename T, bool CAP>
+__device__ __forceinline__ void write_row(const Row<T>& r, int64_t row, int64_t target, bool valid, const Shape& sh, const Stats& t,
+                                          const Outputs& out) {
+    const float log_l = log2f(t.l) * kLn2;
+    const float y = valid ? capped<CAP>(ld1<T>(r.p + target), sh) : 0.f;
+    out.logp[row] = valid ? (y - t.m) * sh.inv_temp - log_l : 0.f;
+    out.entropy[row] = valid ? log_l - t.s / t.l : 0.f;
+    if (out.stats) *(float2*)(out.stats + 2 * row) = make_float2(t.m, log_l);
+}
+template <bool CAP>
+__device__ __forceinline__ void write_alternative(uint64_t key, int64_t at, const Shape& sh, const Stats& t, const Outputs& out) {
+    out.top_ids[at] = (int64_t)(int)~(uint32_t)key;
+    out.top_logp[at] = (capped<CAP>(unordered((uint32_t)(key >> 32)), sh) - t.m) * sh.inv_temp - log2f(t.l) * kLn2;
+}
+
+template <typename T, bool CAP, bool TOP>
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_fwd_kernel(const T* __restrict__ logits, int64_t pitch,
                                                                         const int64_t* __restrict__ targets, int vocab,
-                                                                        int64_t ignore_index, Shape sh, int top_k,
-                                                                        float* __restrict__ logp_out, float* __restrict__ entropy_out,
-                                                                        float* __restrict__ stats_out, int64_t* __restrict__ top_ids,
-                                                                        float* __restrict__ top_logp) {
+                                                                        int64_t ignore_index, Shape sh, int top_k, int parts,
+                                                                        Workspace ws, Outputs out) {
     __shared__ Stats s_box[kLpWaves];
+    __shared__ Selection s_sel;
+    __shared__ uint64_t s_found[kLpThreads];
     __shared__ uint64_t s_key[kLpWaves];
+    __shared__ int s_found_n;
     const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x;
+    const int64_t row = blockIdx.x / parts;
+    const int part = blockIdx.x % parts;
     const Row<T> r(logits + row * pitch, vocab);
     const int64_t target = targets[row];
     const bool valid = target != ignore_index && target >= 0 && target < vocab;
+    // groups [g0, g1) of this part; the last parts of a short row may be empty
+    const int per = (r.groups + parts - 1) / parts;
+    const int g0 = min(part * per, r.groups), g1 = min(g0 + per, r.groups);
 
+    if (!TOP && !valid) {     // nothing of this row is asked for: it is not read
+        if (tid == 0) {
+            if (parts > 1) {
+                ws.stats[blockIdx.x] = {0.f, 1.f, 0.f};
+            } else {
+                out.logp[row] = out.entropy[row] = 0.f;
+                if (out.stats) *(float2*)(out.stats + 2 * row) = make_float2(0.f, 0.f);
+            }
+        }
+        return;
+    }
     Stats t = {-INFINITY, 0.f, 0.f};
-    for (int g = tid; g < r.groups; g += kLpThreads) {
+    float best = -INFINITY;
+    int best_g = g0 + tid;
+    for (int g = g0 + tid; g < g1; g += kLpThreads) {
         float v[8];
         r.load(g, v);
+        if (TOP) {
+            float vm = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+            vm = fmaxf(vm, fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+            if (vm > best) {
+                best = vm;
+                best_g = g;
+            }
+        }
         if (CAP) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = capped<CAP>(v[i], sh);
@@ -165,37 +284,111 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_fwd_kernel(const T*
         fold8(v, sh.inv_temp, t);
     }
     t = workgroup_stats(t, sh.inv_temp, s_box);
-    const float log_l = log2f(t.l) * kLn2;
     if (tid == 0) {
-        const float y = valid ? capped<CAP>(ld1<T>(r.p + target), sh) : 0.f;
-        logp_out[row] = valid ? (y - t.m) * sh.inv_temp - log_l : 0.f;
-        entropy_out[row] = valid ? log_l - t.s / t.l : 0.f;
-        if (stats_out) *(float2*)(stats_out + 2 * row) = make_float2(t.m, log_l);
+        if (parts == 1)
+            write_row<T, CAP>(r, row, target, valid, sh, t, out);
+        else
+            ws.stats[blockIdx.x] = t;
     }
-    // the alternatives, best first: each round takes the largest key below the last round's
-    uint64_t last = ~0ull;
-    for (int k = 0; k < top_k; ++k) {
-        uint64_t best = 0;
-        for (int g = tid; g < r.groups; g += kLpThreads) {
+    if (!TOP) return;
+
+    const int threads = best_of_threads(g0 + tid < g1 ? key_of(best, best_g) : 0, top_k, s_sel);
+    // (maximum, group) of the last of the best threads; with fewer threads than top_k every element of theirs counts
+    const uint64_t bar = threads == top_k ? s_sel.key[threads - 1] : 0;
+    if (tid == 0) s_found_n = 0;
+    __syncthreads();
+    // their groups, each thread's `rounds` of them in a row
+    const int rounds = (g1 - g0 + kLpThreads - 1) / kLpThreads;
+    auto each = [&](auto&& f) {
+        for (int c = tid; c < threads * rounds; c += kLpThreads) {
+            const int owner = ((int)~(uint32_t)s_sel.key[c / rounds] - g0) % kLpThreads;
+            const int g = g0 + owner + (c % rounds) * kLpThreads;
+            if (g >= g1) continue;
             float v[8];
             r.load(g, v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int j = r.first(g) + i;
-                const uint64_t key = key_of(v[i], j);
-                if (j >= 0 && j < vocab && key < last && key > best) best = key;
+                if (j >= 0 && j < vocab && key_of(v[i], g) >= bar) f(key_of(v[i], j));
             }
         }
-        best = wave_max_key(best);
-        __syncthreads();
-        if ((tid & 63) == 0) s_key[tid >> 6] = best;
-        __syncthreads();
-        for (int w = 0; w < kLpWaves; ++w) best = s_key[w] > best ? s_key[w] : best;
-        last = best;
-        if (tid == 0) {
-            top_ids[row * top_k + k] = (int64_t)(int)~(uint32_t)best;
-            top_logp[row * top_k + k] = (capped<CAP>(unordered((uint32_t)(best >> 32)), sh) - t.m) * sh.inv_temp - log_l;
+    };
+    each([&](uint64_t key) {
+        const int n = atomicAdd(&s_found_n, 1);
+        if (n < kLpThreads) s_found[n] = key;
+    });
+    __syncthreads();
+    const int found = s_found_n;
+    if (found <= kLpThreads) {
+        if (tid < found) {
+            const int rank = rank_of(s_found[tid], s_found, found);
+            if (rank < top_k) {
+                if (parts == 1)
+                    write_alternative<CAP>(s_found[tid], row * top_k + rank, sh, t, out);
+                else
+                    ws.keys[(int64_t)blockIdx.x * top_k + rank] = s_found[tid];
+            }
         }
+        if (parts > 1 && tid >= found && tid < top_k) ws.keys[(int64_t)blockIdx.x * top_k + tid] = 0;
+        return;
+    }
+    uint64_t last = ~0ull;
+    for (int k = 0; k < top_k; ++k) {
+        uint64_t top = 0;
+        each([&](uint64_t key) {
+            if (key < last && key > top) top = key;
+        });
+        top = wave_max_key(top);
+        __syncthreads();
+        if ((tid & 63) == 0) s_key[tid >> 6] = top;
+        __syncthreads();
+        for (int w = 0; w < kLpWaves; ++w) top = s_key[w] > top ? s_key[w] : top;
+        last = top;
+        if (tid == 0) {
+            if (parts == 1)
+                write_alternative<CAP>(top, row * top_k + k, sh, t, out);
+            else
+                ws.keys[(int64_t)blockIdx.x * top_k + k] = top;
+        }
+    }
+}
+
+// One workgroup per row of several parts: at most kLpMaxParts statistics and kLpMaxParts * 64 keys, 8 a thread.
+constexpr int kLpMaxParts = 64;
+template <typename T, bool CAP>
+__global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(const T* __restrict__ logits, int64_t pitch,
+                                                                         const int64_t* __restrict__ targets, int vocab,
+                                                                         int64_t ignore_index, Shape sh, int top_k, int parts,
+                                                                         Workspace ws, Outputs out) {
+    __shared__ Stats s_box[kLpWaves];
+    __shared__ Selection s_sel;
+    __shared__ uint64_t s_found[kLpThreads];
+    __shared__ int s_found_n;
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    Stats t = {-INFINITY, 0.f, 0.f};
+    if (tid < parts) t = ws.stats[row * parts + tid];
+    t = workgroup_stats(t, sh.inv_temp, s_box);
+    if (tid == 0) {
+        const int64_t target = targets[row];
+        write_row<T, CAP>(Row<T>(logits + row * pitch, vocab), row, target, target != ignore_index && target >= 0 && target < vocab, sh, t, out);
+    }
+    if (top_k == 0) return;
+    const uint64_t* keys = ws.keys + row * parts * top_k;
+    const int n = parts * top_k;
+    uint64_t best = 0;
+    for (int i = tid; i < n; i += kLpThreads) best = keys[i] > best ? keys[i] : best;
+    const int threads = best_of_threads(best, top_k, s_sel);
+    const uint64_t bar = threads == top_k ? s_sel.key[threads - 1] : 0;
+    if (tid == 0) s_found_n = 0;
+    __syncthreads();
+    // only the best threads have keys at or above the bar, so at most 64 * 8 of them
+    for (int i = tid; i < n; i += kLpThreads)
+        if (keys[i] && keys[i] >= bar) s_found[atomicAdd(&s_found_n, 1)] = keys[i];
+    __syncthreads();
+    if (tid < s_found_n) {
+        const int rank = rank_of(s_found[tid], s_found, s_found_n);
+        if (rank < top_k) write_alternative<CAP>(s_found[tid], row * top_k + rank, sh, t, out);
     }
 }
 
@@ -258,6 +451,19 @@ __global__ __launch_bounds__(kLpBwdThreads) void token_logprobs_bwd_kernel(const
 
 }  // namespace
 
+// Parts that a row is cut into: workgroups for 16 rounds of the chip's 1024 resident ones, but none with fewer than 512
+// groups (a group per thread).
+int token_logprobs_parts(int64_t rows, int64_t vocab) {
+    const int64_t want = (4096 + rows - 1) / rows, most = (vocab / 8 + kLpThreads - 1) / kLpThreads;
+    const int64_t parts = want < most ? want : most;
+    return (int)(parts < 1 ? 1 : parts > kLpMaxParts ? kLpMaxParts : parts);
+}
+static size_t stats_bytes(int64_t rows, int parts) { return ((size_t)rows * parts * sizeof(Stats) + 15) & ~(size_t)15; }
+size_t token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_k) {
+    const int parts = token_logprobs_parts(rows, vocab);
+    return parts == 1 ? 0 : stats_bytes(rows, parts) + (size_t)rows * parts * top_k * sizeof(uint64_t);
+}
+
 // workgroups per row of the gradient kernel, for a row that starts anywhere
 int token_logprobs_bwd_chunks(int64_t vocab) {
     const int per = kLpBwdThreads * kLpBwdGroups;
@@ -270,13 +476,20 @@ Shape shape_of(float softcap, float temperature) {
     return {softcap, softcap > 0.f ? 1.f / softcap : 0.f, 1.f / temperature};
 }
 
-template <typename T>
+template <typename T, bool CAP>
 int fwd(const TokenLogprobsArgs& a, hipStream_t st) {
     const Shape sh = shape_of(a.softcap, a.temperature);
-    const dim3 grid((unsigned)a.rows);
-    auto kernel = a.softcap > 0.f ? token_logprobs_fwd_kernel<T, true> : token_logprobs_fwd_kernel<T, false>;
-    kernel<<<grid, kLpThreads, 0, st>>>((const T*)a.logits, a.pitch, a.targets, (int)a.vocab, a.ignore_index, sh, a.top_k, a.logp,
-                                        a.entropy, a.stats, a.top_ids, a.top_logp);
+    const int parts = token_logprobs_parts(a.rows, a.vocab);
+    const Workspace ws = {(Stats*)a.ws, (uint64_t*)((char*)a.ws + stats_bytes(a.rows, parts))};
+    const Outputs out = {a.logp, a.entropy, a.stats, a.top_ids, a.top_logp};
+    auto kernel = a.top_k ? token_logprobs_fwd_kernel<T, CAP, true> : token_logprobs_fwd_kernel<T, CAP, false>;
+    kernel<<<(unsigned)(a.rows * parts), kLpThreads, 0, st>>>((const T*)a.logits, a.pitch, a.targets, (int)a.vocab, a.ignore_index, sh,
+                                                              a.top_k, parts, ws, out);
+    if (parts > 1) {
+        MA_TRY(check_launch("token_logprobs_fwd_kernel"));
+        token_logprobs_join_kernel<T, CAP><<<(unsigned)a.rows, kLpThreads, 0, st>>>((const T*)a.logits, a.pitch, a.targets, (int)a.vocab,
+                                                                                     a.ignore_index, sh, a.top_k, parts, ws, out);
+    }
     return check_launch("token_logprobs_fwd_kernel");
 }
 template <typename T>
@@ -293,7 +506,8 @@ int bwd(const TokenLogprobsArgs& a, hipStream_t st) {
 }  // namespace
 
 int launch_token_logprobs_fwd(const TokenLogprobsArgs& a, int dtype, hipStream_t st) {
-    return dtype == MA_DTYPE_BF16 ? fwd<uint16_t>(a, st) : fwd<float>(a, st);
+    if (a.softcap > 0.f) return dtype == MA_DTYPE_BF16 ? fwd<uint16_t, true>(a, st) : fwd<float, true>(a, st);
+    return dtype == MA_DTYPE_BF16 ? fwd<uint16_t, false>(a, st) : fwd<float, false>(a, st);
 }
 int launch_token_logprobs_bwd(const TokenLogprobsArgs& a, int dtype, hipStream_t st) {
     return dtype == MA_DTYPE_BF16 ? bwd<uint16_t>(a, st) : bwd<float>(a, st);

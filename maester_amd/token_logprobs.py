@@ -54,11 +54,14 @@ def token_logprobs_forward(logits, targets, top_k=0, ignore_index=-100, softcap=
     top_logp = torch.empty(rows, top_k, dtype=torch.float32, device=dev) if top_k else None
     code = _lib.dtype_code(logits.dtype)
     if rows:
+        L = _lib.lib()
+        ws_bytes = L.ma_token_logprobs_workspace_bytes(rows, vocab, top_k)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         with torch.cuda.device(dev):
-            rc = _lib.lib().ma_token_logprobs_fwd(
+            rc = L.ma_token_logprobs_fwd(
                 _lib.ptr(logits), _row_pitch(logits), _lib.ptr(targets), rows, vocab, int(ignore_index), softcap, temperature,
-                top_k, _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(stats), _lib.ptr(top_ids), _lib.ptr(top_logp), code,
-                _lib.current_stream(dev))
+                top_k, _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(stats), _lib.ptr(top_ids), _lib.ptr(top_logp),
+                _lib.ptr(ws), ws_bytes, code, _lib.current_stream(dev))
         _lib.check(rc)
     return logp, entropy, stats, top_ids, top_logp
 

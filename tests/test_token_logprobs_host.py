@@ -11,8 +11,8 @@ P = 0x1000
 NAN = float("nan")
 
 
-def _fwd(logits=P, pitch=100, targets=P, rows=4, vocab=100, cap=0.0, temp=1.0, k=0, logp=P, ent=P, ids=P, top=P, dtype=1):
-    return _lib.lib().ma_token_logprobs_fwd(logits, pitch, targets, rows, vocab, -100, cap, temp, k, logp, ent, None, ids, top, dtype, None)
+def _fwd(logits=P, pitch=100, targets=P, rows=4, vocab=100, cap=0.0, temp=1.0, k=0, logp=P, ent=P, ids=P, top=P, ws=P, ws_bytes=1 << 20, dtype=1):
+    return _lib.lib().ma_token_logprobs_fwd(logits, pitch, targets, rows, vocab, -100, cap, temp, k, logp, ent, None, ids, top, ws, ws_bytes, dtype, None)
 
 
 @pytest.mark.parametrize("kw,code,text", [
@@ -20,7 +20,8 @@ def _fwd(logits=P, pitch=100, targets=P, rows=4, vocab=100, cap=0.0, temp=1.0, k
     (dict(rows=1 << 23), -2, "rows"), (dict(vocab=0), -1, "vocab"), (dict(vocab=1 << 30, pitch=1 << 31), -1, "vocab"),
     (dict(pitch=99), -1, "pitch"), (dict(cap=-1.0), -1, "softcap"), (dict(cap=NAN), -1, "softcap"), (dict(temp=0.0), -1, "temperature"),
     (dict(temp=NAN), -1, "temperature"), (dict(k=65), -1, "top_k"), (dict(k=-1), -1, "top_k"), (dict(k=6, vocab=5), -1, "top_k"),
-    (dict(k=2, ids=None), -1, "top_ids"), (dict(dtype=7), -1, "dtype"), (dict(logits=P + 1), -1, "aligned")])
+    (dict(k=2, ids=None), -1, "top_ids"), (dict(vocab=50000, pitch=50000, ws=None), -1, "workspace"),
+    (dict(vocab=50000, pitch=50000, ws_bytes=8), -1, "workspace"), (dict(vocab=50000, pitch=50000, ws=P + 8), -1, "aligned"), (dict(dtype=7), -1, "dtype"), (dict(logits=P + 1), -1, "aligned")])
 def test_forward_refusals(kw, code, text):
     assert _fwd(**kw) == code and text in _lib.lib().ma_last_error().decode()
 
