@@ -217,6 +217,50 @@ int ma_token_logprobs_bwd(const void* logits, int64_t pitch, const int64_t* targ
                           int64_t ignore_index, float softcap, float temperature, const float* stats, const float* entropy,
                           const float* dlogp, const float* dentropy, void* dlogits, int64_t dpitch, int dtype, void* stream);
 
+/* ---- AdamW over many tensors ---------------------------------------------------------------------------
+ * The step that applies a training step's gradients: AdamW with decoupled weight decay over any number
+ * of tensors in a few launches (48 tensors each), with the global norm of the gradients and clipping by
+ * it, states in fp32 or in 8 bits.  The reference leaves both to torch (maester/optimizers.py; gradient
+ * clipping in train.py).  With c the clip factor and t the step counter after its increment:
+ *   g = c g;  m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2
+ *   p = p (1 - lr wd) - lr / (1-b1^t) * m / (sqrt(v) / sqrt(1-b2^t) + eps)
+ * evaluated in fp32 in this order, from `master` where one is given (then param is its rounding).
+ * state_bits 32: exp_avg = m, exp_avg_sq = v, fp32 [n].  state_bits 8: exp_avg = m and exp_avg_sq =
+ * sqrt(v) as e4m3 codes [n], with scales fp32 [ceil(n / MA_ADAMW_BLOCK)]: element i is code i *
+ * scale[i / MA_ADAMW_BLOCK].  The scale is the smallest power of two that brings the block's largest
+ * magnitude to 448 or less (1 for a block of zeros, NaN for one with a NaN or an infinity); codes are
+ * rounded stochastically from a hash of (seed, t, index in the list, element), and a nonzero sqrt(v) is
+ * never rounded to 0.
+ * tensors: HOST array, copied before the call returns (its pointers are device pointers); tensors of one
+ * call must not overlap.  lr_device: fp32 on the device, used in place of lr (NULL: lr).  clip: fp32 on
+ * the device, multiplies the gradients (NULL: 1).  max_norm >= 0: the norm of all gradients of the call
+ * is formed first (in fp64) and they are multiplied by min(1, max_norm / (norm + 1e-6)) instead; norm_out
+ * (fp32, may be NULL) receives it.  step: int64 on the device, incremented.
+ * ma_grad_norm: norm and factor alone; norm and / or clip fp32 on the device (max_norm < 0: factor 1).
+ * workspace: at least ma_adamw_workspace_bytes(count) bytes, 16-byte aligned.  Elements past a tensor's
+ * end are not touched.  Any alignment; 16-byte aligned tensors move in 16-byte accesses. */
+#define MA_ADAMW_BLOCK 128
+#define MA_ADAMW_MAX_TENSOR ((int64_t)1 << 34)   /* elements of one tensor */
+#define MA_ADAMW_MAX_ELEMENTS ((int64_t)1 << 37) /* elements of one call */
+typedef struct ma_adamw_tensor {
+    void* param;            /* [n] of param_dtype */
+    const void* grad;       /* [n] of grad_dtype */
+    void* exp_avg;          /* [n] fp32 or codes */
+    void* exp_avg_sq;       /* [n] fp32 or codes */
+    float* exp_avg_scale;   /* 8-bit states only */
+    float* exp_avg_sq_scale;
+    float* master;          /* [n] fp32 weights behind a bf16 param, or NULL */
+    int64_t n;
+    int32_t param_dtype, grad_dtype;
+    int32_t aligned, reserved; /* of the library's own copy; ignored in the caller's */
+} ma_adamw_tensor;
+size_t ma_adamw_workspace_bytes(int count);
+int ma_adamw_step(const ma_adamw_tensor* tensors, int count, int state_bits, double lr, const float* lr_device, double beta1,
+                  double beta2, double eps, double weight_decay, double max_norm, const float* clip, float* norm_out,
+                  int64_t* step, uint32_t seed, void* workspace, size_t workspace_bytes, void* stream);
+int ma_grad_norm(const ma_adamw_tensor* tensors, int count, double max_norm, float* norm, float* clip, void* workspace,
+                 size_t workspace_bytes, void* stream);
+
 /* ---- fused QK-RMSNorm + RoPE prologue ------------------------------------------------------------
  * Replaces query_norm/key_norm (model.py:135-172, 366-368) followed by apply_rotary_emb
  * (model.py:97-106, 371-372) with the table gather by position_ids (model.py:744-747):

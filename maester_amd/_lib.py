@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import (POINTER, Structure, c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p)
+from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p)
 
 import torch
 
@@ -25,10 +25,11 @@ MA_DOC_BLOCK = 32
 MA_WORK_COUNTERS = 64
 MA_TILE_MAP_STATIC_BYTES = 4 << 20
 MA_LOGPROBS_MAX_TOP = 64
+MA_ADAMW_BLOCK = 128
 MA_BWD_DELTA, MA_BWD_DKV, MA_BWD_DQ, MA_BWD_ALL = 1, 2, 4, 7
 
 EXPORTS = (
-    "ma_version", "ma_last_error", "ma_probe_mfma", "ma_tile_map_workspace_bytes", "ma_tile_map_build", "ma_tile_map_build_static", "ma_packed_ids_build", "ma_rmsnorm_bwd_workspace_bytes", "ma_rmsnorm_fwd", "ma_rmsnorm_bwd", "ma_ce_valid_count", "ma_ce_rows", "ma_ce_loss_reduce", "ma_transpose", "ma_token_logprobs_workspace_bytes", "ma_token_logprobs_fwd", "ma_token_logprobs_bwd", "ma_prologue_fwd",
+    "ma_version", "ma_last_error", "ma_probe_mfma", "ma_tile_map_workspace_bytes", "ma_tile_map_build", "ma_tile_map_build_static", "ma_packed_ids_build", "ma_rmsnorm_bwd_workspace_bytes", "ma_rmsnorm_fwd", "ma_rmsnorm_bwd", "ma_ce_valid_count", "ma_ce_rows", "ma_ce_loss_reduce", "ma_transpose", "ma_token_logprobs_workspace_bytes", "ma_token_logprobs_fwd", "ma_token_logprobs_bwd", "ma_adamw_workspace_bytes", "ma_adamw_step", "ma_grad_norm", "ma_prologue_fwd",
     "ma_prologue_bwd_workspace_bytes", "ma_prologue_bwd", "ma_attn_fwd", "ma_attn_bwd_workspace_bytes", "ma_attn_bwd_ds_workspace_bytes",
     "ma_attn_bwd", "ma_attn_bwd_stages",
 )
@@ -43,6 +44,11 @@ class MaTileMap(Structure):
         "kv_num_blocks", "kv_indices", "full_kv_num_blocks", "full_kv_indices",
         "q_num_blocks", "q_indices", "full_q_num_blocks", "full_q_indices", "q_tile_order", "kv_tile_order",
         "block_doc_range", "work_counters", "tile_slot", "tile_count")] + [("visited_tiles", c_int64)]
+
+
+class MaAdamwTensor(Structure):
+    _fields_ = [(n, c_void_p) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master")] + [
+        ("n", c_int64), ("param_dtype", c_int32), ("grad_dtype", c_int32), ("aligned", c_int32), ("reserved", c_int32)]
 
 
 class MaesterAttnError(RuntimeError):
@@ -105,6 +111,13 @@ def lib() -> ctypes.CDLL:
     L.ma_token_logprobs_bwd.restype = c_int
     L.ma_token_logprobs_bwd.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_float, c_float, c_void_p, c_void_p,
                                         c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]
+    L.ma_adamw_workspace_bytes.restype = c_size_t
+    L.ma_adamw_workspace_bytes.argtypes = [c_int]
+    L.ma_adamw_step.restype = c_int
+    L.ma_adamw_step.argtypes = [POINTER(MaAdamwTensor), c_int, c_int, c_double, c_void_p, c_double, c_double, c_double, c_double,
+                                c_double, c_void_p, c_void_p, c_void_p, c_uint32, c_void_p, c_size_t, c_void_p]
+    L.ma_grad_norm.restype = c_int
+    L.ma_grad_norm.argtypes = [POINTER(MaAdamwTensor), c_int, c_double, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
     L.ma_rmsnorm_bwd.restype = c_int
     L.ma_rmsnorm_bwd.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_int64, c_int,
                                  c_int, c_int, c_void_p]

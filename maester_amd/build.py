@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(HERE, "csrc", "build")
 LIB_PATH = os.path.join(HERE, "libmaester_attn.so")
 
-SOURCES = ["api.hip", "probe.hip", "tile_map.hip", "packed_ids.hip", "rmsnorm.hip", "cross_entropy.hip", "token_logprobs.hip", "prologue.hip", "attn_f32.hip", "attn_fwd_bf16.hip", "attn_fwd_pair_bf16.hip",
+SOURCES = ["api.hip", "probe.hip", "tile_map.hip", "packed_ids.hip", "rmsnorm.hip", "cross_entropy.hip", "token_logprobs.hip", "adamw.hip", "prologue.hip", "attn_f32.hip", "attn_fwd_bf16.hip", "attn_fwd_pair_bf16.hip",
            "attn_bwd_bf16.hip"]
 
 # -packed-fp32-ops is switched off on purpose: fp32 arithmetic is issued as scalar-per-lane VALU
@@ -26,6 +26,10 @@ HIPCC_FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-function",
 ]
+
+# sources whose results are those of their formulas in IEEE single precision, operation by operation
+EXACT_SOURCES = {"adamw.hip"}
+EXACT_FLAGS = ["-fno-fast-math", "-ffp-contract=off"]
 
 
 def _hipcc() -> str:
@@ -37,7 +41,7 @@ def _hipcc() -> str:
 
 def _compile(src: str, verbose: bool) -> str:
     obj = os.path.join(OBJ_DIR, os.path.splitext(src)[0] + ".o")
-    cmd = [_hipcc(), *HIPCC_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]
+    cmd = [_hipcc(), *HIPCC_FLAGS, *(EXACT_FLAGS if src in EXACT_SOURCES else []), "-c", os.path.join(CSRC, src), "-o", obj]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)

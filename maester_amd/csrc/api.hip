@@ -279,6 +279,67 @@ int ma_token_logprobs_bwd(const void* logits, int64_t pitch, const int64_t* targ
     return launch_token_logprobs_bwd(a, dtype, (hipStream_t)stream);
 }
 
+size_t ma_adamw_workspace_bytes(int count) { return count < 0 ? 0 : adamw_workspace_bytes(count); }
+
+static int check_adamw(const char* who, const ma_adamw_tensor* tensors, int count, int state_bits, double max_norm, const void* workspace,
+                       size_t workspace_bytes) {
+    if (count < 0 || (count > 0 && !tensors)) return fail(MA_ERR_BAD_ARG, "%s: tensors is NULL or count=%d negative", who, count);
+    if (max_norm != max_norm) return fail(MA_ERR_BAD_ARG, "%s: max_norm is NaN", who);
+    if (!workspace || workspace_bytes < ma_adamw_workspace_bytes(count) || ((uintptr_t)workspace & 15) != 0)
+        return fail(MA_ERR_BAD_ARG, "%s: workspace of %zu bytes, need %zu, 16-byte aligned", who, workspace ? workspace_bytes : (size_t)0,
+                    ma_adamw_workspace_bytes(count));
+    int64_t total = 0;
+    for (int i = 0; i < count; ++i) {
+        const ma_adamw_tensor& t = tensors[i];
+        if (t.n < 0) return fail(MA_ERR_BAD_ARG, "%s: tensor %d has n=%lld", who, i, (long long)t.n);
+        if (t.n > MA_ADAMW_MAX_TENSOR) return fail(MA_ERR_UNSUPPORTED, "%s: tensor %d has n=%lld elements, more than 2^34", who, i, (long long)t.n);
+        total += t.n;
+        if (total > MA_ADAMW_MAX_ELEMENTS) return fail(MA_ERR_UNSUPPORTED, "%s: more than 2^37 elements", who);
+        if (t.n == 0) continue;
+        MA_TRY(check_dtype(who, t.grad_dtype));
+        if (!t.grad) return fail(MA_ERR_BAD_ARG, "%s: grad of tensor %d is NULL", who, i);
+        if (((uintptr_t)t.grad & (t.grad_dtype == MA_DTYPE_BF16 ? 1 : 3)) != 0)
+            return fail(MA_ERR_BAD_ARG, "%s: grad of tensor %d is not aligned to its element size", who, i);
+        if (!state_bits) continue;        // the norm reads the gradients alone
+        MA_TRY(check_dtype(who, t.param_dtype));
+        if (!t.param || !t.exp_avg || !t.exp_avg_sq) return fail(MA_ERR_BAD_ARG, "%s: param / exp_avg / exp_avg_sq of tensor %d is NULL", who, i);
+        if (state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)) return fail(MA_ERR_BAD_ARG, "%s: scales of tensor %d are NULL", who, i);
+        if (t.master && t.param_dtype != MA_DTYPE_BF16) return fail(MA_ERR_BAD_ARG, "%s: master of tensor %d needs a bf16 param", who, i);
+        uintptr_t word = (uintptr_t)t.master;
+        if (t.param_dtype == MA_DTYPE_F32) word |= (uintptr_t)t.param;
+        if (state_bits == 32) word |= (uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq;
+        else word |= (uintptr_t)t.exp_avg_scale | (uintptr_t)t.exp_avg_sq_scale;
+        if ((word & 3) != 0 || ((uintptr_t)t.param & 1) != 0)
+            return fail(MA_ERR_BAD_ARG, "%s: tensor %d is not aligned to its element size", who, i);
+    }
+    return MA_OK;
+}
+
+int ma_adamw_step(const ma_adamw_tensor* tensors, int count, int state_bits, double lr, const float* lr_device, double beta1,
+                  double beta2, double eps, double weight_decay, double max_norm, const float* clip, float* norm_out,
+                  int64_t* step, uint32_t seed, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "ma_adamw_step";
+    if (state_bits != 32 && state_bits != 8) return fail(MA_ERR_BAD_ARG, "%s: state_bits=%d is neither 32 nor 8", who, state_bits);
+    MA_TRY(check_adamw(who, tensors, count, state_bits, max_norm, workspace, workspace_bytes));
+    if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0))
+        return fail(MA_ERR_BAD_ARG, "%s: betas (%g, %g) must be in [0, 1)", who, beta1, beta2);
+    if (!(eps >= 0.0) || !(weight_decay >= 0.0) || (!lr_device && !(lr >= 0.0)))
+        return fail(MA_ERR_BAD_ARG, "%s: lr=%g, eps=%g and weight_decay=%g must be >= 0", who, lr, eps, weight_decay);
+    if (!step || ((uintptr_t)step & 7) != 0) return fail(MA_ERR_BAD_ARG, "%s: step is NULL or not 8-byte aligned", who);
+    const AdamwArgs a = {tensors, count, state_bits, max_norm >= 0.0 ? 1 : 0, lr, beta1, beta2, eps, weight_decay, max_norm, seed,
+                         lr_device, clip, norm_out, nullptr, step, workspace};
+    return launch_adamw(a, (hipStream_t)stream);
+}
+
+int ma_grad_norm(const ma_adamw_tensor* tensors, int count, double max_norm, float* norm, float* clip, void* workspace,
+                 size_t workspace_bytes, void* stream) {
+    const char* who = "ma_grad_norm";
+    MA_TRY(check_adamw(who, tensors, count, 0, max_norm, workspace, workspace_bytes));
+    if (!norm && !clip) return fail(MA_ERR_BAD_ARG, "%s: both outputs are NULL", who);
+    const AdamwArgs a = {tensors, count, 0, 1, 0.0, 0.0, 0.0, 0.0, 0.0, max_norm, 0, nullptr, nullptr, norm, clip, nullptr, workspace};
+    return launch_adamw(a, (hipStream_t)stream);
+}
+
 int ma_packed_ids_build(const int32_t* starts, const int32_t* lengths, const int32_t* counts, int B, int max_docs, int S,
                         int64_t* position_ids, int64_t* document_ids, void* stream) {
     const char* who = "ma_packed_ids_build";

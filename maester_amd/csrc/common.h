@@ -79,6 +79,19 @@ int token_logprobs_bwd_chunks(int64_t vocab);
 int launch_token_logprobs_fwd(const TokenLogprobsArgs& a, int dtype, hipStream_t st);
 int launch_token_logprobs_bwd(const TokenLogprobsArgs& a, int dtype, hipStream_t st);
 
+struct AdamwArgs {
+    const ma_adamw_tensor* list;      // host memory
+    int count, state_bits, want_norm;
+    double lr, b1, b2, eps, weight_decay, max_norm;
+    uint32_t seed;
+    const float *lr_device, *clip_in;
+    float *norm_out, *clip_out;
+    int64_t* step;                    // NULL: the norm only
+    void* ws;
+};
+size_t adamw_workspace_bytes(int count);
+int launch_adamw(const AdamwArgs& a, hipStream_t st);
+
 struct AttnArgs {
     ma_tensor4 q, k, v, o, dout, dq, dk, dv;
     float* lse;
