@@ -217,6 +217,22 @@ int ma_token_logprobs_bwd(const void* logits, int64_t pitch, const int64_t* targ
                           int64_t ignore_index, float softcap, float temperature, const float* stats, const float* entropy,
                           const float* dlogp, const float* dentropy, void* dlogits, int64_t dpitch, int dtype, void* stream);
 
+/* The same from hidden states and the classifier, without the logits: x = e c^T for e [rows, dim] and
+ * c [vocab, dim] of dtype (rows e_stride / c_stride elements apart, 16-byte aligned rows, dim a multiple
+ * of 8 in bf16 and of 4 in fp32), products of the inputs as they are, sums and everything after them in fp32.  Outputs as
+ * ma_token_logprobs_fwd's.  workspace: ma_linear_logprobs_workspace_bytes(rows, vocab) bytes, 16-byte aligned.
+ * ma_linear_logprobs_dlogits writes d x for the gradients dlogp / dentropy (either may be NULL) into
+ * dlogits, rows `pitch` elements apart (a multiple of 8; up to 3 elements of the padding behind a row are
+ * written too), in dtype: the caller multiplies it with c and e (library GEMMs), a block of rows at a time. */
+size_t ma_linear_logprobs_workspace_bytes(int64_t rows, int64_t vocab);
+int ma_linear_logprobs_fwd(const void* e, int64_t e_stride, const void* c, int64_t c_stride, const int64_t* targets, int64_t rows,
+                           int64_t vocab, int64_t dim, int64_t ignore_index, float softcap, float temperature, float* logp,
+                           float* entropy, float* stats, void* workspace, size_t workspace_bytes, int dtype, void* stream);
+int ma_linear_logprobs_dlogits(const void* e, int64_t e_stride, const void* c, int64_t c_stride, const int64_t* targets, int64_t rows,
+                               int64_t vocab, int64_t dim, int64_t ignore_index, float softcap, float temperature, const float* stats,
+                               const float* entropy, const float* dlogp, const float* dentropy, void* dlogits, int64_t pitch,
+                               int dtype, void* stream);
+
 /* ---- AdamW over many tensors ---------------------------------------------------------------------------
  * The step that applies a training step's gradients: AdamW with decoupled weight decay over any number
  * of tensors in a few launches (48 tensors each), with the global norm of the gradients and clipping by

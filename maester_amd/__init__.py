@@ -14,6 +14,7 @@ from .gemma_attention import GemmaAttention, GemmaAttentionConfig
 from .rmsnorm import RMSNorm, rms_norm
 from .linear_ce import ce_rows, linear_cross_entropy
 from .token_logprobs import TokenLogprobs, token_logprobs
+from .linear_logprobs import linear_token_logprobs
 from .adamw import AdamW, Blocks8, adamw_step, global_grad_norm
 from .gemma_layers import GemmaLayerConfig, GemmaMLP, Gemma2DecoderLayer, GemmaModel, GemmaTextModel
 from .packed_ids import (generate_position_ids, generate_document_ids, packed_collate_ids, boundaries_to_tensors,
@@ -24,5 +25,6 @@ __all__ = [
     "qk_norm_rope", "doc_masked_attention", "GemmaAttention", "GemmaAttentionConfig",
     "generate_position_ids", "generate_document_ids", "packed_collate_ids", "boundaries_to_tensors",
     "device_packed_ids", "RMSNorm", "rms_norm", "ce_rows", "linear_cross_entropy",
-    "AdamW", "Blocks8", "adamw_step", "global_grad_norm", "TokenLogprobs", "token_logprobs", "GemmaLayerConfig", "GemmaMLP", "Gemma2DecoderLayer", "GemmaModel", "GemmaTextModel",
+    "AdamW", "Blocks8", "adamw_step", "global_grad_norm", "TokenLogprobs", "token_logprobs",
+    "linear_token_logprobs", "GemmaLayerConfig", "GemmaMLP", "Gemma2DecoderLayer", "GemmaModel", "GemmaTextModel",
 ]

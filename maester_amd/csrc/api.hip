@@ -279,6 +279,59 @@ int ma_token_logprobs_bwd(const void* logits, int64_t pitch, const int64_t* targ
     return launch_token_logprobs_bwd(a, dtype, (hipStream_t)stream);
 }
 
+static int check_linear_logprobs(const char* who, const void* e, int64_t e_stride, const void* c, int64_t c_stride, const int64_t* targets,
+                                 int64_t rows, int64_t vocab, int64_t dim, float softcap, float temperature, int dtype) {
+    MA_TRY(check_dtype(who, dtype));
+    const int64_t al = dtype == MA_DTYPE_BF16 ? 8 : 4;
+    if (!e || !c || !targets) return fail(MA_ERR_BAD_ARG, "%s: e / c / targets is NULL", who);
+    if (((uintptr_t)e & 15) != 0 || ((uintptr_t)c & 15) != 0) return fail(MA_ERR_BAD_ARG, "%s: e / c not 16-byte aligned", who);
+    if (rows <= 0 || rows > ((int64_t)1 << 26)) return fail(MA_ERR_BAD_ARG, "%s: rows=%lld must be in 1 .. 2^26", who, (long long)rows);
+    if (vocab <= 0 || vocab > MA_LOGPROBS_MAX_VOCAB) return fail(MA_ERR_BAD_ARG, "%s: vocab=%lld out of range", who, (long long)vocab);
+    if (dim <= 0 || dim % al != 0 || dim > 65536)
+        return fail(MA_ERR_UNSUPPORTED, "%s: dim=%lld must be a multiple of %lld, at most 65536", who, (long long)dim, (long long)al);
+    if (e_stride < dim || c_stride < dim || e_stride % al || c_stride % al)
+        return fail(MA_ERR_BAD_ARG, "%s: row strides %lld, %lld must be multiples of %lld elements, at least dim", who, (long long)e_stride,
+                    (long long)c_stride, (long long)al);
+    // the rows of a 256-row tile are addressed with 31-bit byte offsets
+    if (e_stride > (1 << 20) || c_stride > (1 << 20)) return fail(MA_ERR_UNSUPPORTED, "%s: row strides above 2^20 elements", who);
+    if (!(softcap >= 0.f) || softcap > 1e30f) return fail(MA_ERR_BAD_ARG, "%s: softcap must be >= 0 (0 = none) and finite", who);
+    if (!(temperature > 1e-6f) || temperature > 1e6f) return fail(MA_ERR_BAD_ARG, "%s: temperature must be in (1e-6, 1e6]", who);
+    return MA_OK;
+}
+
+size_t ma_linear_logprobs_workspace_bytes(int64_t rows, int64_t vocab) {
+    return rows <= 0 || vocab <= 0 ? 0 : linear_logprobs_workspace_bytes(rows, vocab);
+}
+
+int ma_linear_logprobs_fwd(const void* e, int64_t e_stride, const void* c, int64_t c_stride, const int64_t* targets, int64_t rows,
+                           int64_t vocab, int64_t dim, int64_t ignore_index, float softcap, float temperature, float* logp,
+                           float* entropy, float* stats, void* workspace, size_t workspace_bytes, int dtype, void* stream) {
+    const char* who = "ma_linear_logprobs_fwd";
+    MA_TRY(check_linear_logprobs(who, e, e_stride, c, c_stride, targets, rows, vocab, dim, softcap, temperature, dtype));
+    if (!logp || !entropy) return fail(MA_ERR_BAD_ARG, "%s: logp / entropy is NULL", who);
+    if (((uintptr_t)stats & 7) != 0) return fail(MA_ERR_BAD_ARG, "%s: stats not 8-byte aligned", who);
+    if (!workspace || workspace_bytes < linear_logprobs_workspace_bytes(rows, vocab) || ((uintptr_t)workspace & 15) != 0)
+        return fail(MA_ERR_BAD_ARG, "%s: workspace of %zu bytes, need %zu, 16-byte aligned", who, workspace ? workspace_bytes : (size_t)0,
+                    linear_logprobs_workspace_bytes(rows, vocab));
+    const LinearLogprobsArgs a = {e, c, e_stride, c_stride, targets, rows, vocab, dim, ignore_index, softcap, temperature, logp, entropy,
+                                  stats, nullptr, nullptr, nullptr, 0, workspace};
+    return launch_linear_logprobs_fwd(a, dtype, (hipStream_t)stream);
+}
+
+int ma_linear_logprobs_dlogits(const void* e, int64_t e_stride, const void* c, int64_t c_stride, const int64_t* targets, int64_t rows,
+                               int64_t vocab, int64_t dim, int64_t ignore_index, float softcap, float temperature, const float* stats,
+                               const float* entropy, const float* dlogp, const float* dentropy, void* dlogits, int64_t pitch,
+                               int dtype, void* stream) {
+    const char* who = "ma_linear_logprobs_dlogits";
+    MA_TRY(check_linear_logprobs(who, e, e_stride, c, c_stride, targets, rows, vocab, dim, softcap, temperature, dtype));
+    if (!stats || !entropy || !dlogits) return fail(MA_ERR_BAD_ARG, "%s: stats / entropy / dlogits is NULL", who);
+    if (((uintptr_t)dlogits & 15) != 0) return fail(MA_ERR_BAD_ARG, "%s: dlogits not 16-byte aligned", who);
+    if (pitch % 8 != 0 || pitch < vocab) return fail(MA_ERR_BAD_ARG, "%s: pitch=%lld must be a multiple of 8, at least vocab", who, (long long)pitch);
+    const LinearLogprobsArgs a = {e, c, e_stride, c_stride, targets, rows, vocab, dim, ignore_index, softcap, temperature, nullptr,
+                                  (float*)entropy, (float*)stats, dlogp, dentropy, dlogits, pitch, nullptr};
+    return launch_linear_logprobs_dlogits(a, dtype, (hipStream_t)stream);
+}
+
 size_t ma_adamw_workspace_bytes(int count) { return count < 0 ? 0 : adamw_workspace_bytes(count); }
 
 static int check_adamw(const char* who, const ma_adamw_tensor* tensors, int count, int state_bits, double max_norm, const void* workspace,

@@ -79,6 +79,22 @@ int token_logprobs_bwd_chunks(int64_t vocab);
 int launch_token_logprobs_fwd(const TokenLogprobsArgs& a, int dtype, hipStream_t st);
 int launch_token_logprobs_bwd(const TokenLogprobsArgs& a, int dtype, hipStream_t st);
 
+struct LinearLogprobsArgs {
+    const void *e, *c;
+    int64_t e_stride, c_stride;       // elements
+    const int64_t* targets;
+    int64_t rows, vocab, dim, ignore_index;
+    float softcap, temperature;
+    float *logp, *entropy, *stats;    // outputs of the forward, entropy and stats inputs of the gradient
+    const float *dlogp, *dentropy;
+    void* dlogits;
+    int64_t pitch;
+    void* ws;
+};
+size_t linear_logprobs_workspace_bytes(int64_t rows, int64_t vocab);
+int launch_linear_logprobs_fwd(const LinearLogprobsArgs& a, int dtype, hipStream_t st);
+int launch_linear_logprobs_dlogits(const LinearLogprobsArgs& a, int dtype, hipStream_t st);
+
 struct AdamwArgs {
     const ma_adamw_tensor* list;      // host memory
     int count, state_bits, want_norm;

@@ -1,0 +1,440 @@
+// Log-probabilities of given tokens and entropy from hidden states e [rows, K] and the classifier c [vocab, K],
+// without the [rows, vocab] logits x = e c^T: a matrix product whose epilogue keeps, per row, the running maximum and
+// sums of token_logprobs.hip in registers.  The same product with another epilogue forms d loss / d x a block of rows
+// at a time for the two gradient products.
+//
+// Tiles are computed transposed, x^T = c e^T (M: vocabulary, N: tokens), because of where the matrix instruction
+// leaves its result: a lane of a 32 x 32 tile holds 16 rows of ONE column, so with the vocabulary along the rows a
+// lane folds its logits of one token without talking to another lane; lanes, waves and workgroups that share a token
+// join their statistics once at the end of a workgroup's whole vocabulary range.
+//
+// A workgroup of four waves owns BN tokens and a range of the vocabulary that it walks in tiles of 256.  Both operands
+// are staged 128 bytes of K at a time, global memory -> LDS without registers; rows past the end of the range or of
+// the tokens lie outside the loads' descriptors and arrive as zeros.  A row of a stage is 8 chunks of 16 bytes, chunk c
+// of row r stored in place c ^ (r % 8): the 64 lanes of a fragment read (32 rows, one chunk each for its two halves) then
+// spread over all banks.  Which chunk a lane of a load fetches is decided on the global side, so the exchange costs
+// nothing.  A load for step q + STAGES is issued when the last fragment of step q has been read by all waves, a
+// quarter of a step before its products are done, so one barrier a step is enough and the first fragments of the next
+// step are read while the last products of this one run.
+#include <hip/hip_runtime.h>
+
+#include "common.h"
+#include "logprobs.h"
+#include "mfma.h"
+#include "rowio.h"
+
+namespace ma {
+
+namespace {
+
+constexpr int kBM = 256;                     // vocabulary rows of a tile
+constexpr int kStepBytes = 128;              // of K per step and row
+
+struct LinArgs {
+    const char *e, *c;
+    int64_t e_stride, c_stride;              // bytes between rows
+    int rows, vocab, k_bytes;
+    int row_blocks, splits, span;            // workgroups: row_blocks * splits, each `span` of the vocabulary
+    LpShape sh;
+    const int64_t* targets;
+    int64_t ignore_index;
+    LpStats* part;                           // forward: [splits, rows]
+    float* picked;                           // forward: [rows], the target's capped logit
+    const float *stats, *entropy, *dlogp, *dentropy;   // gradient
+    void* dlogits;
+    int64_t pitch;                           // elements between its rows
+};
+
+template <typename T>
+struct Product;
+template <>
+struct Product<uint16_t> {
+    static __device__ __forceinline__ f32x16 mac(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(bf16x8*)&a, *(bf16x8*)&b, c, 0, 0, 0);
+    }
+};
+// fp32: a lane's 16 bytes are four K values, taken one per instruction (both operands in the same order)
+template <>
+struct Product<float> {
+    static __device__ __forceinline__ f32x16 mac(u32x4 a, u32x4 b, f32x16 c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
+        return c;
+    }
+};
+
+template <int BN>
+struct Tiling {
+    static constexpr int kWaveM = BN >= 128 ? 128 : 64, kWaveN = BN >= 128 ? BN / 2 : BN;
+    static constexpr int kMT = kWaveM / 32, kNT = kWaveN / 32;
+    static constexpr int kARuns = kBM / 8 / 4, kBRuns = BN / 8 / 4;      // 1 KB loads per wave and step
+    static constexpr int kStage = (kBM + BN) * kStepBytes;
+    static constexpr int kStages = BN == 256 ? 2 : 3;
+    static constexpr int kLds = kStage * kStages;
+    static_assert(kLds <= 160 * 1024, "LDS");
+};
+
+// workgroup -> (row block, split).  Workgroups go to the 8 XCDs in turn; each XCD gets a contiguous run of the order
+// below, groups of 8 row blocks times all splits, so that the workgroups of one XCD share both operands through its L2:
+// 32 of them then read 8 blocks of e and 4 of c.
+__device__ __forceinline__ bool place(const LinArgs& a, int& rb, int& split) {
+    const int total = a.row_blocks * a.splits, per = (total + kXcds - 1) / kXcds;
+    const int j = (blockIdx.x % kXcds) * per + blockIdx.x / kXcds;
+    if (j >= total) return false;
+    const int super = j / (8 * a.splits), in = j - super * 8 * a.splits;
+    const int height = min(8, a.row_blocks - super * 8);
+    // (integer division runs on the vector ALU: the results go back to scalar registers, where descriptors live)
+    split = __builtin_amdgcn_readfirstlane(in / height);
+    rb = __builtin_amdgcn_readfirstlane(super * 8 + in % height);
+    return true;
+}
+
+// descriptor of wave-uniform values, in scalar registers whatever the compiler has made of them
+__device__ __forceinline__ u32x4 uniform_rsrc(uint64_t base, uint32_t bytes) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)base), hi = __builtin_amdgcn_readfirstlane((uint32_t)(base >> 32));
+    return tile_rsrc((uint64_t)hi << 32 | lo, __builtin_amdgcn_readfirstlane(bytes));
+}
+
+template <typename T, int BN, bool CAP, bool GRAD>
+__global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a) {
+    using L = Tiling<BN>;
+    constexpr int MT = L::kMT, NT = L::kNT, STAGES = L::kStages;
+    extern __shared__ __align__(16) char smem_raw[];
+    const lds_ptr smem = (lds_ptr)smem_raw;
+    int rb, split;
+    if (!place(a, rb, split)) return;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, hh = lane >> 5;
+    const int wm = BN >= 128 ? (w & 1) * L::kWaveM : w * L::kWaveM, wn = BN >= 128 ? (w >> 1) * L::kWaveN : 0;
+    const int n0 = rb * BN, v0 = split * a.span, v1 = min(v0 + a.span, a.vocab);
+    const int tiles = (v1 - v0 + kBM - 1) / kBM, ksteps = (a.k_bytes + kStepBytes - 1) / kStepBytes;
+
+    // ---- loads: run t of 8 rows; this lane fetches chunk `chunk` of row 8 t + lane / 8
+    const int chunk = (lane & 7) ^ (lane >> 3);
+    uint32_t a_off[L::kARuns], b_off[L::kBRuns];
+#pragma unroll
+    for (int p = 0; p < L::kARuns; ++p) a_off[p] = (uint32_t)((w + 4 * p) * 8 + (lane >> 3)) * (uint32_t)a.c_stride + chunk * 16;
+#pragma unroll
+    for (int p = 0; p < L::kBRuns; ++p) b_off[p] = (uint32_t)((w + 4 * p) * 8 + (lane >> 3)) * (uint32_t)a.e_stride + chunk * 16;
+    const uint32_t lds0 = lds_addr(smem);
+    int ld_tile = 0, ld_k = 0;
+    auto load_step = [&](int stage) {
+        const int rows_a = ld_tile < tiles ? min(kBM, v1 - v0 - ld_tile * kBM) : 0;
+        const int rows_b = ld_tile < tiles ? min(BN, a.rows - n0) : 0;
+        const int left = a.k_bytes - ld_k * kStepBytes;
+        const u32x4 ra = uniform_rsrc((uint64_t)a.c + (uint64_t)(v0 + ld_tile * kBM) * a.c_stride + ld_k * kStepBytes,
+                                   rows_a ? (uint32_t)((rows_a - 1) * a.c_stride + left) : 0u);
+        const u32x4 rbv = uniform_rsrc((uint64_t)a.e + (uint64_t)n0 * a.e_stride + ld_k * kStepBytes,
+                                    rows_b ? (uint32_t)((rows_b - 1) * a.e_stride + left) : 0u);
+        // chunks past the end of a row are the next row's first: out of any descriptor's range
+        const uint32_t past = chunk * 16 < left ? 0u : 0x80000000u;
+        const uint32_t at = __builtin_amdgcn_readfirstlane(lds0 + stage * L::kStage + w * 1024);
+#pragma unroll
+        for (int p = 0; p < L::kARuns; ++p) buffer_to_lds_run(ra, a_off[p] | past, at + p * 4096);
+#pragma unroll
+        for (int p = 0; p < L::kBRuns; ++p) buffer_to_lds_run(rbv, b_off[p] | past, at + kBM * kStepBytes + p * 4096);
+        if (++ld_k == ksteps) {
+            ld_k = 0;
+            ++ld_tile;
+        }
+    };
+
+    // ---- fragments: 32 rows, chunks 2 s and 2 s + 1 of a step
+    uint32_t frag[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) frag[s] = r * kStepBytes + (((2 * s + hh) ^ (r & 7)) << 4);
+    u32x4 fa[2][MT], fb[2][NT];
+    auto read = [&](int buf, int stage, int s) {
+        const lds_ptr at = smem + stage * L::kStage + frag[s];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) fa[buf][i] = *(MA_LDS u32x4*)(at + (wm + 32 * i) * kStepBytes);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) fb[buf][j] = *(MA_LDS u32x4*)(at + (kBM + wn + 32 * j) * kStepBytes);
+    };
+    f32x16 acc[MT][NT];
+    auto clear = [&]() {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = f32x16(0.f);
+    };
+    auto multiply = [&](int buf) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i][j] = Product<T>::mac(fa[buf][i], fb[buf][j], acc[i][j]);
+    };
+
+    // ---- this lane's tokens
+    int target[NT];
+    LpStats run[NT];
+    float ga[NT], gb[NT], top[NT], log_l[NT], ent[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int n = n0 + wn + 32 * j + r;
+        const int64_t t = n < a.rows ? a.targets[n] : -1;
+        const bool valid = t != a.ignore_index && t >= 0 && t < a.vocab;
+        target[j] = valid ? (int)t : -1;
+        run[j] = {-INFINITY, 0.f, 0.f};
+        if (GRAD) {
+            ga[j] = valid && a.dlogp ? a.dlogp[n] : 0.f;
+            gb[j] = valid && a.dentropy ? a.dentropy[n] : 0.f;
+            top[j] = valid ? a.stats[2 * n] : 0.f;
+            log_l[j] = valid ? a.stats[2 * n + 1] : 0.f;
+            ent[j] = valid ? a.entropy[n] : 0.f;
+        }
+    }
+
+    auto finish_tile = [&](int tile) {
+        const int m0 = v0 + tile * kBM + wm;           // this lane's rows: m0 + 32 i + 8 (v / 4) + 4 hh + v % 4
+        const bool partial = m0 + L::kWaveM > v1;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int t = target[j] - m0 - 4 * hh;     // the target's row of this tile, if it is one of this lane's
+            const bool here = t >= 0 && t < L::kWaveM && (t & 4) == 0 && target[j] >= 0;
+            if (!GRAD) {
+                // one token's column at a time: the accumulators of the others stay where they are
+                __builtin_amdgcn_sched_barrier(0);
+                if (CAP) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) acc[i][j][v] = lp_capped<CAP>(acc[i][j][v], a.sh);
+                }
+                if (partial) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v)
+                            if (m0 + 32 * i + 8 * (v / 4) + 4 * hh + v % 4 >= v1) acc[i][j][v] = -INFINITY;
+                }
+                if (__any(here)) {
+                    float x = 0.f;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v)
+                            if (32 * i + 8 * (v / 4) + v % 4 == t) x = acc[i][j][v];
+                    // (a target past v1 belongs to the next range's workgroup)
+                    if (here && target[j] < v1) a.picked[n0 + wn + 32 * j + r] = x;
+                }
+                float m = run[j].m;
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) m = fmaxf(m, acc[i][j][v]);
+                lp_rescale(run[j], m, a.sh.inv_temp);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) lp_add(run[j], acc[i][j][v], a.sh.inv_temp);
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                const int n = n0 + wn + 32 * j + r;
+                T* out = (T*)a.dlogits + (int64_t)n * a.pitch;
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int m = m0 + 32 * i + 8 * q + 4 * hh;
+                        float d[4];
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) {
+                            const float x = acc[i][j][4 * q + v];
+                            const float th = CAP ? tanhf(x * a.sh.inv_cap) : 0.f;
+                            const float lp = fmaf((CAP ? a.sh.cap * th : x) - top[j], a.sh.inv_temp, -log_l[j]);
+                            const float p = __builtin_amdgcn_exp2f(lp * kLpLog2e);
+                            d[v] = -p * fmaf(gb[j], fmaxf(lp, -1e30f) + ent[j], ga[j]);
+                            if (here && 32 * i + 8 * q + v == t) d[v] += ga[j];
+                            d[v] *= CAP ? (1.f - th * th) * a.sh.inv_temp : a.sh.inv_temp;
+                            if (target[j] < 0) d[v] = 0.f;
+                        }
+                        if (n < a.rows && m < v1) {     // up to three columns past the vocabulary lie in the row's padding
+                            if constexpr (sizeof(T) == 2) {
+                                bf16x4 o;
+#pragma unroll
+                                for (int v = 0; v < 4; ++v) o[v] = (__bf16)d[v];
+                                *(bf16x4*)(out + m) = o;
+                            } else {
+                                *(float4*)(out + m) = make_float4(d[0], d[1], d[2], d[3]);
+                            }
+                        }
+                    }
+            }
+        }
+    };
+
+    // loads that may still be in flight when a step's operands must have landed
+    constexpr int kInFlight = (STAGES - 2) * (L::kARuns + L::kBRuns);
+    for (int s = 0; s < STAGES; ++s) load_step(s);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kInFlight + L::kARuns + L::kBRuns) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    clear();
+    int stage = 0;
+    read(0, 0, 0);
+    for (int tile = 0; tile < tiles; ++tile) {
+        for (int k = 0; k < ksteps; ++k) {
+            read(1, stage, 1);
+            multiply(0);
+            read(0, stage, 2);
+            multiply(1);
+            read(1, stage, 3);
+            multiply(0);
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kInFlight) : "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            load_step(stage);
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            read(0, stage, 0);
+            multiply(1);
+        }
+        finish_tile(tile);
+        clear();
+    }
+    // the last loads (of steps that do not exist) must not land in LDS that is used again
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (GRAD) return;
+    // lanes l and l + 32 share a token, and so do the waves along the vocabulary
+    constexpr int kMWaves = BN >= 128 ? 2 : 4;
+    MA_LDS LpStats* box = (MA_LDS LpStats*)smem;       // [kMWaves][BN]
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const LpStats t = lp_merged(run[j], lp_shuffled(run[j], 32), a.sh.inv_temp);
+        if (hh == 0) {
+            MA_LDS LpStats* at = box + (BN >= 128 ? (w & 1) : w) * BN + wn + 32 * j + r;
+            at->m = t.m;
+            at->l = t.l;
+            at->s = t.s;
+        }
+    }
+    __syncthreads();
+    for (int n = tid; n < BN && n0 + n < a.rows; n += 256) {
+        LpStats t = {box[n].m, box[n].l, box[n].s};
+#pragma unroll
+        for (int m = 1; m < kMWaves; ++m) {
+            MA_LDS LpStats* o = box + m * BN + n;
+            t = lp_merged(t, {o->m, o->l, o->s}, a.sh.inv_temp);
+        }
+        a.part[(int64_t)split * a.rows + n0 + n] = t;
+    }
+}
+
+// a wave per token joins the splits
+__global__ __launch_bounds__(256) void linear_logprobs_join_kernel(const LinArgs a, float* __restrict__ logp, float* __restrict__ entropy,
+                                                                   float* __restrict__ stats) {
+    const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (n >= a.rows) return;
+    LpStats t = {-INFINITY, 0.f, 0.f};
+    for (int s = lane; s < a.splits; s += 64) t = lp_merged(t, a.part[(int64_t)s * a.rows + n], a.sh.inv_temp);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) t = lp_merged(t, lp_shuffled(t, off), a.sh.inv_temp);
+    if (lane) return;
+    const int64_t target = a.targets[n];
+    const bool valid = target != a.ignore_index && target >= 0 && target < a.vocab;
+    const float log_l = log2f(t.l) * kLpLn2;
+    logp[n] = valid ? (a.picked[n] - t.m) * a.sh.inv_temp - log_l : 0.f;
+    entropy[n] = valid ? log_l - t.s / t.l : 0.f;
+    if (stats) *(float2*)(stats + 2 * (int64_t)n) = make_float2(t.m, log_l);
+}
+
+int tokens_per_block(int64_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+
+// Splits of the vocabulary: as many workgroups as the chip has compute units, or as little over a whole multiple of them
+// as there is, ranges a multiple of 32 long so that the few tokens' case, bound by reading c, shares it out evenly.
+void plan(LinArgs& a, int bn, int tiles_whole) {
+    a.row_blocks = (a.rows + bn - 1) / bn;
+    const int cus = 256;
+    int64_t best = INT64_MAX;
+    const int most = (a.vocab + kBM - 1) / kBM;
+    for (int splits = 1; splits <= most && splits <= cus; ++splits) {
+        int span = (a.vocab + splits - 1) / splits;
+        const int unit = tiles_whole ? kBM : 32;
+        span = (span + unit - 1) / unit * unit;
+        const int64_t rounds = ((int64_t)a.row_blocks * splits + cus - 1) / cus, tiles = (span + kBM - 1) / kBM;
+        const int64_t cost = tiles_whole ? rounds * tiles * kBM : rounds * span;
+        if (cost < best) {
+            best = cost;
+            a.splits = splits;
+            a.span = span;
+        }
+    }
+    a.splits = (a.vocab + a.span - 1) / a.span;        // none of them empty
+}
+
+LinArgs args_of(const LinearLogprobsArgs& p, int dtype) {
+    LinArgs a = {};
+    const int elt = dtype == MA_DTYPE_BF16 ? 2 : 4;
+    a.e = (const char*)p.e;
+    a.c = (const char*)p.c;
+    a.e_stride = p.e_stride * elt;
+    a.c_stride = p.c_stride * elt;
+    a.rows = (int)p.rows;
+    a.vocab = (int)p.vocab;
+    a.k_bytes = (int)p.dim * elt;
+    a.sh = lp_shape(p.softcap, p.temperature);
+    a.targets = p.targets;
+    a.ignore_index = p.ignore_index;
+    plan(a, tokens_per_block(p.rows), p.rows > 64);
+    return a;
+}
+
+template <typename T, int BN, bool CAP, bool GRAD>
+int start(const LinArgs& a, hipStream_t st) {
+    auto kernel = linear_logprobs_kernel<T, BN, CAP, GRAD>;
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, Tiling<BN>::kLds);
+    if (e != hipSuccess) return fail(MA_ERR_LAUNCH, "linear_logprobs_kernel: %s", hipGetErrorString(e));
+    const int grid = (a.row_blocks * a.splits + kXcds - 1) / kXcds * kXcds;
+    kernel<<<grid, 256, Tiling<BN>::kLds, st>>>(a);
+    return check_launch("linear_logprobs_kernel");
+}
+template <typename T, bool CAP, bool GRAD>
+int by_rows(const LinArgs& a, hipStream_t st) {
+    switch (tokens_per_block(a.rows)) {
+        case 32: return start<T, 32, CAP, GRAD>(a, st);
+        case 64: return start<T, 64, CAP, GRAD>(a, st);
+        case 128: return start<T, 128, CAP, GRAD>(a, st);
+        default: return start<T, 256, CAP, GRAD>(a, st);
+    }
+}
+template <bool GRAD>
+int by_type(const LinArgs& a, int dtype, hipStream_t st) {
+    if (a.sh.cap > 0.f) return dtype == MA_DTYPE_BF16 ? by_rows<uint16_t, true, GRAD>(a, st) : by_rows<float, true, GRAD>(a, st);
+    return dtype == MA_DTYPE_BF16 ? by_rows<uint16_t, false, GRAD>(a, st) : by_rows<float, false, GRAD>(a, st);
+}
+
+}  // namespace
+
+// picked [rows] (rounded up to 16 bytes), then part [splits, rows] for at most 256 splits of 256 or more
+size_t linear_logprobs_workspace_bytes(int64_t rows, int64_t vocab) {
+    int64_t splits = (vocab + kBM - 1) / kBM;
+    if (splits > 256) splits = 256;
+    return (((size_t)rows * 4 + 15) & ~(size_t)15) + (size_t)splits * rows * sizeof(LpStats);
+}
+
+int launch_linear_logprobs_fwd(const LinearLogprobsArgs& p, int dtype, hipStream_t st) {
+    LinArgs a = args_of(p, dtype);
+    a.picked = (float*)p.ws;
+    a.part = (LpStats*)((char*)p.ws + (((size_t)p.rows * 4 + 15) & ~(size_t)15));
+    const int rc = by_type<false>(a, dtype, st);
+    if (rc) return rc;
+    linear_logprobs_join_kernel<<<(unsigned)((p.rows + 3) / 4), 256, 0, st>>>(a, p.logp, p.entropy, p.stats);
+    return check_launch("linear_logprobs_join_kernel");
+}
+
+int launch_linear_logprobs_dlogits(const LinearLogprobsArgs& p, int dtype, hipStream_t st) {
+    LinArgs a = args_of(p, dtype);
+    a.stats = p.stats;
+    a.entropy = p.entropy;
+    a.dlogp = p.dlogp;
+    a.dentropy = p.dentropy;
+    a.dlogits = p.dlogits;
+    a.pitch = p.pitch;
+    return by_type<true>(a, dtype, st);
+}
+
+}  // namespace ma

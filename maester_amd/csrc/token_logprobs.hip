@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include "common.h"
+#include "logprobs.h"
 #include "rowio.h"
 
 #define MA_TRY(expr)            \
@@ -20,16 +21,12 @@
         if (rc__) return rc__;  \
     } while (0)
 
-#pragma clang fp reassociate(off)
-
 namespace ma {
 
 namespace {
 
 constexpr int kLpThreads = 512;       // >= 8 * MA_LOGPROBS_MAX_TOP: the waves' best keys, one a thread
 constexpr int kLpWaves = kLpThreads / 64;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 template <typename T>
 __device__ __forceinline__ float ld1(const T* p);
@@ -71,56 +68,17 @@ struct Row {
     }
 };
 
-struct Shape {
-    float cap, inv_cap, inv_temp;
-};
-template <bool CAP>
-__device__ __forceinline__ float capped(float x, const Shape& s) { return CAP ? s.cap * tanhf(x * s.inv_cap) : x; }
-
-// running maximum (in units of the capped logits), sum of exponentials and of (y - m) exp(y - m)
-struct Stats {
-    float m, l, s;
-};
-__device__ __forceinline__ Stats merged(const Stats& a, const Stats& b, float inv_temp) {
-    const float m = fmaxf(a.m, b.m);
-    const float base = m == -INFINITY ? 0.f : m;
-    const float da = fmaxf((a.m - base) * inv_temp, -1e30f), db = fmaxf((b.m - base) * inv_temp, -1e30f);
-    const float fa = __builtin_amdgcn_exp2f(da * kLog2e), fb = __builtin_amdgcn_exp2f(db * kLog2e);
-    return {m, a.l * fa + b.l * fb, fa * (a.s + da * a.l) + fb * (b.s + db * b.l)};
-}
-// 8 capped logits.  A NaN among them (or +inf, as inf - inf) makes l NaN, and with it every output.
-__device__ __forceinline__ void fold8(const float* y, float inv_temp, Stats& t) {
-    float vm = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
-    vm = fmaxf(vm, fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
-    const float m = fmaxf(t.m, vm);
-    const float base = m == -INFINITY ? 0.f : m;    // nothing but -inf so far: l and s stay 0
-    const float dt = fmaxf((t.m - base) * inv_temp, -1e30f);
-    const float f = __builtin_amdgcn_exp2f(dt * kLog2e);
-    float l = 0.f, s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float d = (y[i] - base) * inv_temp;
-        const float e = __builtin_amdgcn_exp2f(d * kLog2e);
-        l += e;
-        s = fmaf(fmaxf(d, -1e30f), e, s);           // 0 * -inf would be NaN: a term of weight 0 adds nothing
-    }
-    t.s = f * (t.s + dt * t.l) + s;
-    t.l = t.l * f + l;
-    t.m = m;
-}
-
 // the statistics of the whole workgroup, in every thread; box: one slot per wave
-__device__ __forceinline__ Stats workgroup_stats(Stats t, float inv_temp, Stats* box) {
+__device__ __forceinline__ LpStats workgroup_stats(LpStats t, float inv_temp, LpStats* box) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
-        const Stats o = {__shfl_xor(t.m, off, 64), __shfl_xor(t.l, off, 64), __shfl_xor(t.s, off, 64)};
-        t = merged(t, o, inv_temp);
+        t = lp_merged(t, lp_shuffled(t, off), inv_temp);
     }
     if ((threadIdx.x & 63) == 0) box[threadIdx.x >> 6] = t;
     __syncthreads();
     t = box[0];
 #pragma unroll
-    for (int w = 1; w < kLpWaves; ++w) t = merged(t, box[w], inv_temp);
+    for (int w = 1; w < kLpWaves; ++w) t = lp_merged(t, box[w], inv_temp);
     return t;
 }
 
@@ -213,31 +171,31 @@ struct Outputs {
     float* top_logp;
 };
 struct Workspace {
-    Stats* stats;      // [rows, parts]
+    LpStats* stats;      // [rows, parts]
     uint64_t* keys;    // [rows, parts, top_k]
 };
 
 template <typename T, bool CAP>
-__device__ __forceinline__ void write_row(const Row<T>& r, int64_t row, int64_t target, bool valid, const Shape& sh, const Stats& t,
+__device__ __forceinline__ void write_row(const Row<T>& r, int64_t row, int64_t target, bool valid, const LpShape& sh, const LpStats& t,
                                           const Outputs& out) {
-    const float log_l = log2f(t.l) * kLn2;
-    const float y = valid ? capped<CAP>(ld1<T>(r.p + target), sh) : 0.f;
+    const float log_l = log2f(t.l) * kLpLn2;
+    const float y = valid ? lp_capped<CAP>(ld1<T>(r.p + target), sh) : 0.f;
     out.logp[row] = valid ? (y - t.m) * sh.inv_temp - log_l : 0.f;
     out.entropy[row] = valid ? log_l - t.s / t.l : 0.f;
     if (out.stats) *(float2*)(out.stats + 2 * row) = make_float2(t.m, log_l);
 }
 template <bool CAP>
-__device__ __forceinline__ void write_alternative(uint64_t key, int64_t at, const Shape& sh, const Stats& t, const Outputs& out) {
+__device__ __forceinline__ void write_alternative(uint64_t key, int64_t at, const LpShape& sh, const LpStats& t, const Outputs& out) {
     out.top_ids[at] = (int64_t)(int)~(uint32_t)key;
-    out.top_logp[at] = (capped<CAP>(unordered((uint32_t)(key >> 32)), sh) - t.m) * sh.inv_temp - log2f(t.l) * kLn2;
+    out.top_logp[at] = (lp_capped<CAP>(unordered((uint32_t)(key >> 32)), sh) - t.m) * sh.inv_temp - log2f(t.l) * kLpLn2;
 }
 
 template <typename T, bool CAP, bool TOP>
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_fwd_kernel(const T* __restrict__ logits, int64_t pitch,
                                                                         const int64_t* __restrict__ targets, int vocab,
-                                                                        int64_t ignore_index, Shape sh, int top_k, int parts,
+                                                                        int64_t ignore_index, LpShape sh, int top_k, int parts,
                                                                         Workspace ws, Outputs out) {
-    __shared__ Stats s_box[kLpWaves];
+    __shared__ LpStats s_box[kLpWaves];
     __shared__ Selection s_sel;
     __shared__ uint64_t s_found[kLpThreads];
     __shared__ uint64_t s_key[kLpWaves];
@@ -263,7 +221,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_fwd_kernel(const T*
         }
         return;
     }
-    Stats t = {-INFINITY, 0.f, 0.f};
+    LpStats t = {-INFINITY, 0.f, 0.f};
     float best = -INFINITY;
     int best_g = g0 + tid;
     for (int g = g0 + tid; g < g1; g += kLpThreads) {
@@ -279,9 +237,9 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_fwd_kernel(const T*
         }
         if (CAP) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = capped<CAP>(v[i], sh);
+            for (int i = 0; i < 8; ++i) v[i] = lp_capped<CAP>(v[i], sh);
         }
-        fold8(v, sh.inv_temp, t);
+        lp_fold<8>(v, sh.inv_temp, t);
     }
     t = workgroup_stats(t, sh.inv_temp, s_box);
     if (tid == 0) {
@@ -358,15 +316,15 @@ constexpr int kLpMaxParts = 64;
 template <typename T, bool CAP>
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(const T* __restrict__ logits, int64_t pitch,
                                                                          const int64_t* __restrict__ targets, int vocab,
-                                                                         int64_t ignore_index, Shape sh, int top_k, int parts,
+                                                                         int64_t ignore_index, LpShape sh, int top_k, int parts,
                                                                          Workspace ws, Outputs out) {
-    __shared__ Stats s_box[kLpWaves];
+    __shared__ LpStats s_box[kLpWaves];
     __shared__ Selection s_sel;
     __shared__ uint64_t s_found[kLpThreads];
     __shared__ int s_found_n;
     const int tid = threadIdx.x;
     const int64_t row = blockIdx.x;
-    Stats t = {-INFINITY, 0.f, 0.f};
+    LpStats t = {-INFINITY, 0.f, 0.f};
     if (tid < parts) t = ws.stats[row * parts + tid];
     t = workgroup_stats(t, sh.inv_temp, s_box);
     if (tid == 0) {
@@ -397,7 +355,7 @@ constexpr int kLpBwdThreads = 256, kLpBwdGroups = 4;      // groups of 8 per thr
 template <typename T, bool CAP>
 __global__ __launch_bounds__(kLpBwdThreads) void token_logprobs_bwd_kernel(const T* __restrict__ logits, int64_t pitch,
                                                                            const int64_t* __restrict__ targets, int vocab,
-                                                                           int64_t ignore_index, Shape sh,
+                                                                           int64_t ignore_index, LpShape sh,
                                                                            const float* __restrict__ stats,
                                                                            const float* __restrict__ entropy_in,
                                                                            const float* __restrict__ dlogp,
@@ -433,7 +391,7 @@ __global__ __launch_bounds__(kLpBwdThreads) void token_logprobs_bwd_kernel(const
             for (int i = 0; i < 8; ++i) {
                 const float th = CAP ? tanhf(v[i] * sh.inv_cap) : 0.f;
                 const float lp = fmaf((CAP ? sh.cap * th : v[i]) - top, sh.inv_temp, -log_l);
-                const float p = __builtin_amdgcn_exp2f(lp * kLog2e);
+                const float p = __builtin_amdgcn_exp2f(lp * kLpLog2e);
                 d[i] = -p * fmaf(b, fmaxf(lp, -1e30f) + h, a);
                 if (j + i == target) d[i] += a;
                 d[i] *= CAP ? (1.f - th * th) * sh.inv_temp : sh.inv_temp;
@@ -458,7 +416,7 @@ int token_logprobs_parts(int64_t rows, int64_t vocab) {
     const int64_t parts = want < most ? want : most;
     return (int)(parts < 1 ? 1 : parts > kLpMaxParts ? kLpMaxParts : parts);
 }
-static size_t stats_bytes(int64_t rows, int parts) { return ((size_t)rows * parts * sizeof(Stats) + 15) & ~(size_t)15; }
+static size_t stats_bytes(int64_t rows, int parts) { return ((size_t)rows * parts * sizeof(LpStats) + 15) & ~(size_t)15; }
 size_t token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_k) {
     const int parts = token_logprobs_parts(rows, vocab);
     return parts == 1 ? 0 : stats_bytes(rows, parts) + (size_t)rows * parts * top_k * sizeof(uint64_t);
@@ -472,15 +430,11 @@ int token_logprobs_bwd_chunks(int64_t vocab) {
 
 namespace {
 
-Shape shape_of(float softcap, float temperature) {
-    return {softcap, softcap > 0.f ? 1.f / softcap : 0.f, 1.f / temperature};
-}
-
 template <typename T, bool CAP>
 int fwd(const TokenLogprobsArgs& a, hipStream_t st) {
-    const Shape sh = shape_of(a.softcap, a.temperature);
+    const LpShape sh = lp_shape(a.softcap, a.temperature);
     const int parts = token_logprobs_parts(a.rows, a.vocab);
-    const Workspace ws = {(Stats*)a.ws, (uint64_t*)((char*)a.ws + stats_bytes(a.rows, parts))};
+    const Workspace ws = {(LpStats*)a.ws, (uint64_t*)((char*)a.ws + stats_bytes(a.rows, parts))};
     const Outputs out = {a.logp, a.entropy, a.stats, a.top_ids, a.top_logp};
     auto kernel = a.top_k ? token_logprobs_fwd_kernel<T, CAP, true> : token_logprobs_fwd_kernel<T, CAP, false>;
     kernel<<<(unsigned)(a.rows * parts), kLpThreads, 0, st>>>((const T*)a.logits, a.pitch, a.targets, (int)a.vocab, a.ignore_index, sh,
@@ -494,7 +448,7 @@ int fwd(const TokenLogprobsArgs& a, hipStream_t st) {
 }
 template <typename T>
 int bwd(const TokenLogprobsArgs& a, hipStream_t st) {
-    const Shape sh = shape_of(a.softcap, a.temperature);
+    const LpShape sh = lp_shape(a.softcap, a.temperature);
     const int chunks = token_logprobs_bwd_chunks(a.vocab);
     const dim3 grid((unsigned)(a.rows * chunks));
     auto kernel = a.softcap > 0.f ? token_logprobs_bwd_kernel<T, true> : token_logprobs_bwd_kernel<T, false>;

@@ -1,0 +1,145 @@
+"""Log-probabilities of given tokens and entropy from hidden states and the classifier, without the logits.
+
+``token_logprobs`` of ``e @ c.T`` in one matrix-core kernel whose epilogue keeps the softmax statistics of every token: the
+``[tokens, vocab]`` matrix never exists and its entries stay in fp32 (``linear_cross_entropy`` rounds a block of them to the
+activation dtype between its GEMM and its softmax kernel).  The backward forms the gradient of the logits a block of rows
+at a time, from the statistics that the forward kept, in the activation dtype, and leaves the two products with the
+classifier and the hidden states to the library's GEMMs, as ``linear_cross_entropy`` does.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .linear_ce import default_chunk_rows, transpose
+from .token_logprobs import check_softmax_arguments
+
+
+def _check(e, c, targets):
+    _lib.require_gpu(e, "linear_token_logprobs")
+    if e.dim() != 2 or c.dim() != 2 or e.shape[1] != c.shape[1]:
+        raise ValueError(f"e {tuple(e.shape)} and c {tuple(c.shape)} must be [N, K] and [V, K]")
+    if e.dtype != c.dtype or e.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("e and c must share a dtype, bf16 or fp32")
+    if targets.shape != (e.shape[0],) or targets.dtype != torch.int64:
+        raise ValueError("targets must be int64 [N]")
+    if c.device != e.device or targets.device != e.device:
+        raise ValueError("e, c and targets must be on one device")
+    unit = 16 // e.element_size()
+    if e.shape[1] == 0 or e.shape[1] % unit or c.shape[0] == 0:
+        raise ValueError(f"K must be a positive multiple of {unit} in {e.dtype} and V positive, got K={e.shape[1]}, V={c.shape[0]}")
+
+
+def _rows_in_place(x: torch.Tensor) -> torch.Tensor:
+    """``x`` itself where the kernels can read its rows where they are, else a contiguous copy."""
+    unit = 16 // x.element_size()
+    ok = x.stride(1) == 1 and (x.shape[0] <= 1 or (x.stride(0) >= x.shape[1] and x.stride(0) % unit == 0 and x.stride(0) <= 1 << 20))
+    return x if ok and x.data_ptr() % 16 == 0 else x.contiguous().clone() if x.data_ptr() % 16 and x.is_contiguous() else x.contiguous()
+
+
+def _pitch(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def linear_token_logprobs_forward(e, c, targets, ignore_index=-100, softcap=None, temperature=1.0):
+    """``(logp, entropy, stats)`` for ``e`` ``[N, K]``, ``c`` ``[V, K]``, int64 ``targets`` ``[N]``."""
+    _check(e, c, targets)
+    softcap, temperature = check_softmax_arguments(softcap, temperature)
+    e, c, targets = _rows_in_place(e), _rows_in_place(c), targets.contiguous()
+    n, vocab = e.shape[0], c.shape[0]
+    logp, entropy = torch.empty(2, n, dtype=torch.float32, device=e.device).unbind()
+    stats = torch.empty(n, 2, dtype=torch.float32, device=e.device)
+    if n:
+        L = _lib.lib()
+        ws_bytes = L.ma_linear_logprobs_workspace_bytes(n, vocab)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=e.device)
+        with torch.cuda.device(e.device):
+            rc = L.ma_linear_logprobs_fwd(_lib.ptr(e), _pitch(e), _lib.ptr(c), _pitch(c), _lib.ptr(targets), n, vocab, e.shape[1],
+                                          int(ignore_index), softcap, temperature, _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(stats),
+                                          _lib.ptr(ws), ws_bytes, _lib.dtype_code(e.dtype), _lib.current_stream(e.device))
+        _lib.check(rc)
+    return logp, entropy, stats
+
+
+def _dlogits(e, c, targets, stats, entropy, dlogp, dentropy, ignore_index, softcap, temperature, out):
+    """Gradient of the logits of a block of rows into ``out`` ``[rows, pitch]``."""
+    with torch.cuda.device(e.device):
+        rc = _lib.lib().ma_linear_logprobs_dlogits(
+            _lib.ptr(e), _pitch(e), _lib.ptr(c), _pitch(c), _lib.ptr(targets), e.shape[0], c.shape[0], e.shape[1], int(ignore_index),
+            softcap, temperature, _lib.ptr(stats), _lib.ptr(entropy), _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.ptr(out), out.shape[1],
+            _lib.dtype_code(e.dtype), _lib.current_stream(e.device))
+    _lib.check(rc)
+
+
+def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentropy, ignore_index=-100, softcap=None,
+                                   temperature=1.0, chunk_rows=None, need_de=True, need_dc=True):
+    """``(de, dc)`` (None where not needed) from the gradients of ``logp`` and ``entropy`` (either may be None)."""
+    softcap, temperature = check_softmax_arguments(softcap, temperature)
+    e, c, targets = _rows_in_place(e), _rows_in_place(c), targets.contiguous()
+    dlogp, dentropy = (None if t is None else t.float().contiguous() for t in (dlogp, dentropy))
+    n, k = e.shape
+    vocab = c.shape[0]
+    de = torch.empty(n, k, dtype=e.dtype, device=e.device) if need_de else None
+    if n == 0:
+        return de, torch.zeros(vocab, k, dtype=c.dtype, device=c.device) if need_dc else None
+    step = int(chunk_rows) if chunk_rows else default_chunk_rows(vocab, e.element_size(), n)
+    step = max(1, min(step, n))
+    block = torch.empty(step, -(-vocab // 8) * 8, dtype=e.dtype, device=e.device)
+    c_t = transpose(c.contiguous()) if need_de else None     # the library's faster operand order, as in linear_cross_entropy
+    mixed = {"out_dtype": torch.float32} if e.dtype != torch.float32 else {}
+    dc_t = None
+    for r0 in range(0, n, step):
+        rows = slice(r0, min(n, r0 + step))
+        buf = block[: rows.stop - r0]
+        _dlogits(e[rows], c, targets[rows], stats[rows], entropy[rows], None if dlogp is None else dlogp[rows],
+                 None if dentropy is None else dentropy[rows], ignore_index, softcap, temperature, buf)
+        x = buf[:, :vocab]
+        if need_de:
+            torch.mm(x, c_t.t(), out=de[rows])
+        if need_dc:
+            e_t = transpose(e[rows].contiguous())
+            if n <= step:
+                dc_t = torch.mm(e_t, x)
+            elif dc_t is None:                   # several blocks: summed in fp32, rounded once at the end
+                dc_t = torch.mm(e_t, x, **mixed)
+            else:
+                torch.addmm(dc_t, e_t, x, out=dc_t, **mixed)
+    return de, transpose(dc_t, c.dtype) if need_dc else None
+
+
+class _LinearTokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, e, c, targets, ignore_index, softcap, temperature, chunk_rows):
+        logp, entropy, stats = linear_token_logprobs_forward(e, c, targets, ignore_index, softcap, temperature)
+        ctx.save_for_backward(e, c, targets, stats, entropy)
+        ctx.args = (ignore_index, softcap, temperature, chunk_rows)
+        ctx.set_materialize_grads(False)
+        return logp, entropy
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlogp, dentropy):
+        if dlogp is None and dentropy is None:
+            return (None,) * 7
+        e, c, targets, stats, entropy = ctx.saved_tensors
+        de, dc = linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentropy, *ctx.args,
+                                                ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return de, dc, None, None, None, None, None
+
+
+def linear_token_logprobs(e: torch.Tensor, c: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
+                          softcap: float | None = None, temperature: float = 1.0,
+                          chunk_rows: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(logp, entropy)`` of ``token_logprobs(e @ c.T, targets)``, fp32 of the shape of ``targets``, differentiable (once)
+    in ``e`` and ``c``.
+
+    ``e`` ``[..., K]`` hidden states, ``c`` ``[V, K]`` classifier (Gemma: the tied embedding table), bf16 or fp32 alike,
+    ``K`` a multiple of 8 (fp32: 4); the logits are products of the inputs summed in fp32 and never stored.  ``softcap``,
+    ``temperature`` and ignored targets as in ``token_logprobs``.  ``chunk_rows``: rows per block of the backward (default:
+    about 4 GiB of gradient of the logits at a time)."""
+    if e.dim() < 1 or targets.shape != e.shape[:-1]:
+        raise ValueError(f"targets shape {tuple(targets.shape)} != leading shape of e {tuple(e.shape[:-1])}")
+    lead = targets.shape
+    logp, entropy = _LinearTokenLogprobsFn.apply(e.reshape(targets.numel(), e.shape[-1]), c, targets.reshape(-1), int(ignore_index),
+                                                 softcap, temperature, chunk_rows)
+    return logp.view(lead), entropy.view(lead)

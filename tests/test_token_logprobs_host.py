@@ -59,3 +59,36 @@ def test_oracle_against_torch(softcap, temperature):
     assert np.allclose(out["logp"], logp.detach().numpy(), atol=1e-12) and np.allclose(out["entropy"], entropy.detach().numpy(), atol=1e-12)
     assert np.allclose(out["dx"], dx.numpy(), atol=1e-12)
     assert np.array_equal(out["top_ids"], torch.sort(x.detach(), dim=1, descending=True, stable=True).indices[:, :5].numpy())
+
+
+def _lin(e=P, es=64, c=P, cs=64, targets=P, rows=4, vocab=100, dim=64, cap=0.0, temp=1.0, logp=P, stats=P, ws=P, ws_bytes=1 << 20, dtype=1):
+    return _lib.lib().ma_linear_logprobs_fwd(e, es, c, cs, targets, rows, vocab, dim, -100, cap, temp, logp, P, stats, ws, ws_bytes, dtype, None)
+
+
+LINEAR = [(dict(e=None), -1, "NULL"), (dict(c=P + 8), -1, "aligned"), (dict(rows=0), -1, "rows"), (dict(rows=(1 << 26) + 1), -1, "rows"),
+          (dict(vocab=0), -1, "vocab"), (dict(dim=60), -2, "dim"), (dict(dim=65544, es=65544, cs=65544), -2, "dim"), (dict(es=56), -1, "strides"),
+          (dict(cs=68), -1, "strides"), (dict(es=(1 << 20) + 8), -2, "strides"), (dict(cap=-1.0), -1, "softcap"), (dict(temp=NAN), -1, "temperature"),
+          (dict(dtype=3), -1, "dtype")]
+
+
+@pytest.mark.parametrize("kw,code,text", LINEAR + [(dict(logp=None), -1, "logp"), (dict(stats=P + 4), -1, "stats"), (dict(ws=None), -1, "workspace"),
+                                                   (dict(ws_bytes=20), -1, "workspace"), (dict(ws=P + 8), -1, "aligned")])
+def test_linear_forward_refusals(kw, code, text):
+    assert _lin(**kw) == code and text in _lib.lib().ma_last_error().decode()
+
+
+def _dlogits(e=P, es=64, c=P, cs=64, targets=P, rows=4, vocab=100, dim=64, cap=0.0, temp=1.0, stats=P, out=P, pitch=104, dtype=1):
+    return _lib.lib().ma_linear_logprobs_dlogits(e, es, c, cs, targets, rows, vocab, dim, -100, cap, temp, stats, P, P, P, out, pitch, dtype, None)
+
+
+@pytest.mark.parametrize("kw,code,text", LINEAR + [(dict(stats=None), -1, "stats"), (dict(out=P + 8), -1, "aligned"), (dict(pitch=100), -1, "pitch"),
+                                                   (dict(pitch=96), -1, "pitch")])
+def test_linear_gradient_refusals(kw, code, text):
+    assert _dlogits(**kw) == code and text in _lib.lib().ma_last_error().decode()
+
+
+def test_linear_workspace():
+    L = _lib.lib()
+    assert L.ma_linear_logprobs_workspace_bytes(0, 100) == 0
+    assert L.ma_linear_logprobs_workspace_bytes(5, 600) == 32 + 3 * 5 * 12          # targets' logits, three ranges' statistics
+    assert L.ma_linear_logprobs_workspace_bytes(8, 262208) == 32 + 256 * 8 * 12
