@@ -117,26 +117,46 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
     for (int p = 0; p < L::kARuns; ++p) a_off[p] = (uint32_t)((w + 4 * p) * 8 + (lane >> 3)) * (uint32_t)a.c_stride + chunk * 16;
 #pragma unroll
     for (int p = 0; p < L::kBRuns; ++p) b_off[p] = (uint32_t)((w + 4 * p) * 8 + (lane >> 3)) * (uint32_t)a.e_stride + chunk * 16;
-    const uint32_t lds0 = lds_addr(smem);
-    int ld_tile = 0, ld_k = 0;
-    auto load_step = [&](int stage) {
+    const uint32_t lds0 = lds_addr(smem) + w * 1024;
+    // the next step to load: addresses and bytes in range of both operands move on by a step's 128 bytes, and start
+    // over with the next tile's rows; past the last tile nothing is in range
+    int ld_tile = 0, ld_left = a.k_bytes;
+    uint64_t a_at, b_at;
+    uint32_t a_bytes, b_bytes;
+    auto open_tile = [&]() {
         const int rows_a = ld_tile < tiles ? min(kBM, v1 - v0 - ld_tile * kBM) : 0;
         const int rows_b = ld_tile < tiles ? min(BN, a.rows - n0) : 0;
-        const int left = a.k_bytes - ld_k * kStepBytes;
-        const u32x4 ra = uniform_rsrc((uint64_t)a.c + (uint64_t)(v0 + ld_tile * kBM) * a.c_stride + ld_k * kStepBytes,
-                                   rows_a ? (uint32_t)((rows_a - 1) * a.c_stride + left) : 0u);
-        const u32x4 rbv = uniform_rsrc((uint64_t)a.e + (uint64_t)n0 * a.e_stride + ld_k * kStepBytes,
-                                    rows_b ? (uint32_t)((rows_b - 1) * a.e_stride + left) : 0u);
+        a_at = (uint64_t)a.c + (uint64_t)(v0 + ld_tile * kBM) * a.c_stride;
+        b_at = (uint64_t)a.e + (uint64_t)n0 * a.e_stride;
+        a_bytes = rows_a ? (uint32_t)((rows_a - 1) * a.c_stride) + a.k_bytes : 0u;
+        b_bytes = rows_b ? (uint32_t)((rows_b - 1) * a.e_stride) + a.k_bytes : 0u;
+        ld_left = a.k_bytes;
+    };
+    open_tile();
+    u32x4 ra, rbv;
+    uint32_t past, ld_at;
+    auto load_begin = [&](int stage) {
+        ra = uniform_rsrc(a_at, a_bytes);
+        rbv = uniform_rsrc(b_at, b_bytes);
         // chunks past the end of a row are the next row's first: out of any descriptor's range
-        const uint32_t past = chunk * 16 < left ? 0u : 0x80000000u;
-        const uint32_t at = __builtin_amdgcn_readfirstlane(lds0 + stage * L::kStage + w * 1024);
-#pragma unroll
-        for (int p = 0; p < L::kARuns; ++p) buffer_to_lds_run(ra, a_off[p] | past, at + p * 4096);
-#pragma unroll
-        for (int p = 0; p < L::kBRuns; ++p) buffer_to_lds_run(rbv, b_off[p] | past, at + kBM * kStepBytes + p * 4096);
-        if (++ld_k == ksteps) {
-            ld_k = 0;
+        past = chunk * 16 < ld_left ? 0u : 0x80000000u;
+        ld_at = __builtin_amdgcn_readfirstlane(lds0 + stage * L::kStage);
+    };
+    constexpr int kRuns = L::kARuns + L::kBRuns;
+    auto load_run = [&](auto run) {
+        constexpr int p = decltype(run)::value;
+        if constexpr (p < L::kARuns) buffer_to_lds_run_at<p * 4096>(ra, a_off[p] | past, ld_at);
+        else buffer_to_lds_run_at<kBM * kStepBytes + (p - L::kARuns) * 4096>(rbv, b_off[p - L::kARuns] | past, ld_at);
+    };
+    auto load_end = [&]() {
+        a_at += kStepBytes;
+        b_at += kStepBytes;
+        a_bytes = a_bytes ? a_bytes - kStepBytes : 0u;      // (the last step of a tile may wrap: it is opened anew)
+        b_bytes = b_bytes ? b_bytes - kStepBytes : 0u;
+        ld_left -= kStepBytes;
+        if (ld_left <= 0) {
             ++ld_tile;
+            open_tile();
         }
     };
 
@@ -145,12 +165,10 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
 #pragma unroll
     for (int s = 0; s < 4; ++s) frag[s] = r * kStepBytes + (((2 * s + hh) ^ (r & 7)) << 4);
     u32x4 fa[2][MT], fb[2][NT];
-    auto read = [&](int buf, int stage, int s) {
-        const lds_ptr at = smem + stage * L::kStage + frag[s];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) fa[buf][i] = *(MA_LDS u32x4*)(at + (wm + 32 * i) * kStepBytes);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) fb[buf][j] = *(MA_LDS u32x4*)(at + (kBM + wn + 32 * j) * kStepBytes);
+    auto read_one = [&](int buf, lds_ptr at, auto which) {
+        constexpr int i = decltype(which)::value;
+        if constexpr (i < MT) fa[buf][i] = *(MA_LDS u32x4*)(at + (wm + 32 * i) * kStepBytes);
+        else fb[buf][i - MT] = *(MA_LDS u32x4*)(at + (kBM + wn + 32 * (i - MT)) * kStepBytes);
     };
     f32x16 acc[MT][NT];
     auto clear = [&]() {
@@ -159,11 +177,18 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
 #pragma unroll
             for (int j = 0; j < NT; ++j) acc[i][j] = f32x16(0.f);
     };
-    auto multiply = [&](int buf) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int i = 0; i < MT; ++i) acc[i][j] = Product<T>::mac(fa[buf][i], fb[buf][j], acc[i][j]);
+    // The products of one quarter step on fragments `buf`, with the reads of the next quarter's fragments (into the other
+    // buffer) and, in the last quarter, the loads of a later step between them, an instruction or two to each product:
+    // a wave has its SIMD to itself, and what it issues between two products runs in their shadow.
+    auto quarter = [&](int buf, lds_ptr next, auto with_loads) {
+        constexpr int P = MT * NT, R = MT + NT, W = decltype(with_loads)::value ? kRuns : 0;
+        static_for<0, P>([&](auto step) {
+            constexpr int i = decltype(step)::value;
+            static_for<i * R / P, (i + 1) * R / P>([&](auto k) { read_one(buf ^ 1, next, k); });
+            static_for<i * W / P, (i + 1) * W / P>([&](auto k) { load_run(k); });
+            acc[i % MT][i / MT] = Product<T>::mac(fa[buf][i % MT], fb[buf][i / MT], acc[i % MT][i / MT]);
+            __builtin_amdgcn_sched_barrier(0);
+        });
     };
 
     // ---- this lane's tokens
@@ -186,51 +211,39 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
         }
     }
 
-    auto finish_tile = [&](int tile) {
-        const int m0 = v0 + tile * kBM + wm;           // this lane's rows: m0 + 32 i + 8 (v / 4) + 4 hh + v % 4
-        const bool partial = m0 + L::kWaveM > v1;
+    // this lane's rows of a tile: m0 + row_of(16 i + v) + 4 hh for accumulator i's register v
+    auto row_of = [](int i) constexpr { return 32 * (i / 16) + 8 * (i % 16 / 4) + i % 4; };
+    auto finish_tile = [&](int m0, auto is_partial) {
+        constexpr bool PARTIAL = decltype(is_partial)::value;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int t = target[j] - m0 - 4 * hh;     // the target's row of this tile, if it is one of this lane's
             const bool here = t >= 0 && t < L::kWaveM && (t & 4) == 0 && target[j] >= 0;
             if (!GRAD) {
-                // one token's column at a time: the accumulators of the others stay where they are
-                __builtin_amdgcn_sched_barrier(0);
-                if (CAP) {
+                // two accumulators of one token's column at a time: the others stay where they are
+                static_for<0, MT / 2>([&](auto half) {
+                    constexpr int i0 = decltype(half)::value * 32;
+                    __builtin_amdgcn_sched_barrier(0);
+                    float y[32];
 #pragma unroll
-                    for (int i = 0; i < MT; ++i)
+                    for (int i = 0; i < 32; ++i) y[i] = lp_capped<CAP>(acc[(i0 + i) / 16][j][i % 16], a.sh);
+                    if constexpr (PARTIAL) {
+                        const int left = v1 - m0 - 4 * hh;
 #pragma unroll
-                        for (int v = 0; v < 16; ++v) acc[i][j][v] = lp_capped<CAP>(acc[i][j][v], a.sh);
-                }
-                if (partial) {
+                        for (int i = 0; i < 32; ++i) y[i] = row_of(i0 + i) < left ? y[i] : -INFINITY;
+                    }
+                    if (__any(here)) {
+                        float x = 0.f;
 #pragma unroll
-                    for (int i = 0; i < MT; ++i)
-#pragma unroll
-                        for (int v = 0; v < 16; ++v)
-                            if (m0 + 32 * i + 8 * (v / 4) + 4 * hh + v % 4 >= v1) acc[i][j][v] = -INFINITY;
-                }
-                if (__any(here)) {
-                    float x = 0.f;
-#pragma unroll
-                    for (int i = 0; i < MT; ++i)
-#pragma unroll
-                        for (int v = 0; v < 16; ++v)
-                            if (32 * i + 8 * (v / 4) + v % 4 == t) x = acc[i][j][v];
-                    // (a target past v1 belongs to the next range's workgroup)
-                    if (here && target[j] < v1) a.picked[n0 + wn + 32 * j + r] = x;
-                }
-                float m = run[j].m;
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) m = fmaxf(m, acc[i][j][v]);
-                lp_rescale(run[j], m, a.sh.inv_temp);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) lp_add(run[j], acc[i][j][v], a.sh.inv_temp);
-                __builtin_amdgcn_sched_barrier(0);
+                        for (int i = 0; i < 32; ++i) x = row_of(i0 + i) == t ? y[i] : x;
+                        // (a target past v1 belongs to the next range's workgroup)
+                        if (here && t / 64 == decltype(half)::value && target[j] < v1) a.picked[n0 + wn + 32 * j + r] = x;
+                    }
+                    lp_fold2<32>(y, a.sh.inv_temp * kLpLog2e, run[j]);
+                    // done here, not where the sums are next needed (which would keep every column's logits in registers)
+                    asm volatile("" : "+v"(run[j].m), "+v"(run[j].l), "+v"(run[j].s));
+                    __builtin_amdgcn_sched_barrier(0);
+                });
             } else {
                 const int n = n0 + wn + 32 * j + r;
                 T* out = (T*)a.dlogits + (int64_t)n * a.pitch;
@@ -267,31 +280,37 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
     };
 
     // loads that may still be in flight when a step's operands must have landed
-    constexpr int kInFlight = (STAGES - 2) * (L::kARuns + L::kBRuns);
-    for (int s = 0; s < STAGES; ++s) load_step(s);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kInFlight + L::kARuns + L::kBRuns) : "memory");
+    constexpr int kInFlight = (STAGES - 2) * kRuns;
+    for (int s = 0; s < STAGES; ++s) {
+        load_begin(s);
+        static_for<0, kRuns>([&](auto k) { load_run(k); });
+        load_end();
+    }
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kInFlight + kRuns) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     clear();
     int stage = 0;
-    read(0, 0, 0);
+    constexpr std::integral_constant<bool, false> no{};
+    constexpr std::integral_constant<bool, true> yes{};
+    static_for<0, MT + NT>([&](auto k) { read_one(0, smem + frag[0], k); });
     for (int tile = 0; tile < tiles; ++tile) {
         for (int k = 0; k < ksteps; ++k) {
-            read(1, stage, 1);
-            multiply(0);
-            read(0, stage, 2);
-            multiply(1);
-            read(1, stage, 3);
-            multiply(0);
+            const lds_ptr at = smem + stage * L::kStage;
+            quarter(0, at + frag[1], no);
+            quarter(1, at + frag[2], no);
+            quarter(0, at + frag[3], no);
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kInFlight) : "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            load_step(stage);
+            load_begin(stage);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
-            read(0, stage, 0);
-            multiply(1);
+            quarter(1, smem + stage * L::kStage + frag[0], yes);
+            load_end();
         }
-        finish_tile(tile);
+        const int m0 = v0 + tile * kBM + wm;
+        if (m0 + L::kWaveM > v1) finish_tile(m0, yes);
+        else finish_tile(m0, no);
         clear();
     }
     // the last loads (of steps that do not exist) must not land in LDS that is used again
@@ -304,6 +323,7 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
     MA_LDS LpStats* box = (MA_LDS LpStats*)smem;       // [kMWaves][BN]
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
+        run[j].s *= kLpLn2;
         const LpStats t = lp_merged(run[j], lp_shuffled(run[j], 32), a.sh.inv_temp);
         if (hh == 0) {
             MA_LDS LpStats* at = box + (BN >= 128 ? (w & 1) : w) * BN + wn + 32 * j + r;

@@ -60,6 +60,28 @@ __device__ __forceinline__ void lp_fold(const float* y, float inv_temp, LpStats&
     t.l += one.l;
     t.s += one.s;
 }
+// The same for logits that are sums of products, with s in units of log2 e and scale = log2 e / T: one multiply-add forms
+// the exponent, (y - m) scale = y scale - m scale.  Logits whose product with the scale overflows come out NaN.
+template <int N>
+__device__ __forceinline__ void lp_fold2(const float* y, float scale, LpStats& t) {
+    float m = t.m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, y[i]);
+    const float base = m == -INFINITY ? 0.f : m * scale;
+    const float d = fmaxf(fmaf(t.m, scale, -base), -1e30f);
+    const float f = __builtin_amdgcn_exp2f(d);
+    float l = 0.f, s = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float x = fmaf(y[i], scale, -base);
+        const float e = __builtin_amdgcn_exp2f(x);
+        l += e;
+        s = fmaf(fmaxf(x, -1e30f), e, s);
+    }
+    t.s = f * (t.s + d * t.l) + s;
+    t.l = t.l * f + l;
+    t.m = m;
+}
 __device__ __forceinline__ LpStats lp_shuffled(const LpStats& t, int off) {
     return {__shfl_xor(t.m, off, 64), __shfl_xor(t.l, off, 64), __shfl_xor(t.s, off, 64)};
 }
