@@ -9,13 +9,13 @@
 // join their statistics once at the end of a workgroup's whole vocabulary range.
 //
 // A workgroup of four waves owns BN tokens and a range of the vocabulary that it walks in tiles of 256.  Both operands
-// are staged 128 bytes of K at a time, global memory -> LDS without registers; rows past the end of the range or of
-// the tokens lie outside the loads' descriptors and arrive as zeros.  A row of a stage is 8 chunks of 16 bytes, chunk c
-// of row r stored in place c ^ (r % 8): the 64 lanes of a fragment read (32 rows, one chunk each for its two halves) then
-// spread over all banks.  Which chunk a lane of a load fetches is decided on the global side, so the exchange costs
-// nothing.  A load for step q + STAGES is issued when the last fragment of step q has been read by all waves, a
-// quarter of a step before its products are done, so one barrier a step is enough and the first fragments of the next
-// step are read while the last products of this one run.
+// are staged 128 (64) bytes of K at a time, global memory -> LDS without registers; rows past the end of the range or of
+// the tokens lie outside the loads' descriptors and arrive as zeros.  A row of a stage is 8 (4) chunks of 16 bytes, chunk
+// c of row r stored in place c ^ (r / 2 % 8) (c ^ (r / 4 % 4)): the 16 lanes that read together (16 rows, one chunk each)
+// then touch all 64 banks once.  Which chunk a lane of a load fetches is decided on the global side, so the exchange
+// costs nothing.  The loads of step q + STAGES are issued when the last fragment of step q has been read by all waves,
+// before its last products, so one barrier a step is enough and the first fragments of the next step are read while the
+// last products of this one run.
 #include <hip/hip_runtime.h>
 
 #include "common.h"
@@ -28,7 +28,6 @@ namespace ma {
 namespace {
 
 constexpr int kBM = 256;                     // vocabulary rows of a tile
-constexpr int kStepBytes = 128;              // of K per step and row
 
 struct LinArgs {
     const char *e, *c;
@@ -68,9 +67,13 @@ template <int BN>
 struct Tiling {
     static constexpr int kWaveM = BN >= 128 ? 128 : 64, kWaveN = BN >= 128 ? BN / 2 : BN;
     static constexpr int kMT = kWaveM / 32, kNT = kWaveN / 32;
-    static constexpr int kARuns = kBM / 8 / 4, kBRuns = BN / 8 / 4;      // 1 KB loads per wave and step
-    static constexpr int kStage = (kBM + BN) * kStepBytes;
-    static constexpr int kStages = BN == 256 ? 2 : 3;
+    static constexpr int kStep = 128, kStages = BN == 256 ? 2 : 3;     // bytes of K per step and row
+    static constexpr int kGroups = BN == 256 ? 2 : 4;                 // of a step's loads
+    static constexpr int kSubs = kStep / 32, kChunks = kStep / 16, kRunRows = 1024 / kStep;
+    static constexpr int kARuns = kBM / kRunRows / 4, kBRuns = BN / kRunRows / 4;       // 1 KB loads per wave and step
+    static constexpr int kStage = (kBM + BN) * kStep;
+    // place of chunk c of row r of a stage: c ^ key(r)
+    static constexpr __host__ __device__ int key(int r) { return kStep == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
     static constexpr int kLds = kStage * kStages;
     static_assert(kLds <= 160 * 1024, "LDS");
 };
@@ -108,17 +111,18 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
     const int r = lane & 31, hh = lane >> 5;
     const int wm = BN >= 128 ? (w & 1) * L::kWaveM : w * L::kWaveM, wn = BN >= 128 ? (w >> 1) * L::kWaveN : 0;
     const int n0 = rb * BN, v0 = split * a.span, v1 = min(v0 + a.span, a.vocab);
-    const int tiles = (v1 - v0 + kBM - 1) / kBM, ksteps = (a.k_bytes + kStepBytes - 1) / kStepBytes;
+    const int tiles = (v1 - v0 + kBM - 1) / kBM, ksteps = (a.k_bytes + L::kStep - 1) / L::kStep;
 
-    // ---- loads: run t of 8 rows; this lane fetches chunk `chunk` of row 8 t + lane / 8
-    const int chunk = (lane & 7) ^ (lane >> 3);
+    // ---- loads: run t of kRunRows rows, of which this lane fetches one chunk of one row (key(row) is the same for all
+    // runs of a wave, which are four apart)
+    const int run_row = lane / L::kChunks, chunk = (lane % L::kChunks) ^ L::key(w * L::kRunRows + run_row);
     uint32_t a_off[L::kARuns], b_off[L::kBRuns];
 #pragma unroll
-    for (int p = 0; p < L::kARuns; ++p) a_off[p] = (uint32_t)((w + 4 * p) * 8 + (lane >> 3)) * (uint32_t)a.c_stride + chunk * 16;
+    for (int p = 0; p < L::kARuns; ++p) a_off[p] = (uint32_t)((w + 4 * p) * L::kRunRows + run_row) * (uint32_t)a.c_stride + chunk * 16;
 #pragma unroll
-    for (int p = 0; p < L::kBRuns; ++p) b_off[p] = (uint32_t)((w + 4 * p) * 8 + (lane >> 3)) * (uint32_t)a.e_stride + chunk * 16;
+    for (int p = 0; p < L::kBRuns; ++p) b_off[p] = (uint32_t)((w + 4 * p) * L::kRunRows + run_row) * (uint32_t)a.e_stride + chunk * 16;
     const uint32_t lds0 = lds_addr(smem) + w * 1024;
-    // the next step to load: addresses and bytes in range of both operands move on by a step's 128 bytes, and start
+    // the next step to load: addresses and bytes in range of both operands move on by a step's bytes, and start
     // over with the next tile's rows; past the last tile nothing is in range
     int ld_tile = 0, ld_left = a.k_bytes;
     uint64_t a_at, b_at;
@@ -142,18 +146,21 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
         past = chunk * 16 < ld_left ? 0u : 0x80000000u;
         ld_at = __builtin_amdgcn_readfirstlane(lds0 + stage * L::kStage);
     };
+    // a step's loads go out in as many groups as it has parts: the first in the last part of a step, when its stage has
+    // become free, the others in the first parts of the next step
     constexpr int kRuns = L::kARuns + L::kBRuns;
+    constexpr auto group_begin = [](int g) constexpr { return (g < L::kGroups ? g : L::kGroups) * kRuns / L::kGroups; };
     auto load_run = [&](auto run) {
         constexpr int p = decltype(run)::value;
         if constexpr (p < L::kARuns) buffer_to_lds_run_at<p * 4096>(ra, a_off[p] | past, ld_at);
-        else buffer_to_lds_run_at<kBM * kStepBytes + (p - L::kARuns) * 4096>(rbv, b_off[p - L::kARuns] | past, ld_at);
+        else buffer_to_lds_run_at<kBM * L::kStep + (p - L::kARuns) * 4096>(rbv, b_off[p - L::kARuns] | past, ld_at);
     };
     auto load_end = [&]() {
-        a_at += kStepBytes;
-        b_at += kStepBytes;
-        a_bytes = a_bytes ? a_bytes - kStepBytes : 0u;      // (the last step of a tile may wrap: it is opened anew)
-        b_bytes = b_bytes ? b_bytes - kStepBytes : 0u;
-        ld_left -= kStepBytes;
+        a_at += L::kStep;
+        b_at += L::kStep;
+        a_bytes = a_bytes ? a_bytes - L::kStep : 0u;      // (the last step of a tile may wrap: it is opened anew)
+        b_bytes = b_bytes ? b_bytes - L::kStep : 0u;
+        ld_left -= L::kStep;
         if (ld_left <= 0) {
             ++ld_tile;
             open_tile();
@@ -161,14 +168,14 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
     };
 
     // ---- fragments: 32 rows, chunks 2 s and 2 s + 1 of a step
-    uint32_t frag[4];
+    uint32_t frag[L::kSubs];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) frag[s] = r * kStepBytes + (((2 * s + hh) ^ (r & 7)) << 4);
+    for (int s = 0; s < L::kSubs; ++s) frag[s] = r * L::kStep + (((2 * s + hh) ^ L::key(r)) << 4);
     u32x4 fa[2][MT], fb[2][NT];
     auto read_one = [&](int buf, lds_ptr at, auto which) {
         constexpr int i = decltype(which)::value;
-        if constexpr (i < MT) fa[buf][i] = *(MA_LDS u32x4*)(at + (wm + 32 * i) * kStepBytes);
-        else fb[buf][i - MT] = *(MA_LDS u32x4*)(at + (kBM + wn + 32 * (i - MT)) * kStepBytes);
+        if constexpr (i < MT) fa[buf][i] = *(MA_LDS u32x4*)(at + (wm + 32 * i) * L::kStep);
+        else fb[buf][i - MT] = *(MA_LDS u32x4*)(at + (kBM + wn + 32 * (i - MT)) * L::kStep);
     };
     f32x16 acc[MT][NT];
     auto clear = [&]() {
@@ -177,15 +184,16 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
 #pragma unroll
             for (int j = 0; j < NT; ++j) acc[i][j] = f32x16(0.f);
     };
-    // The products of one quarter step on fragments `buf`, with the reads of the next quarter's fragments (into the other
-    // buffer) and, in the last quarter, the loads of a later step between them, an instruction or two to each product:
-    // a wave has its SIMD to itself, and what it issues between two products runs in their shadow.
-    auto quarter = [&](int buf, lds_ptr next, auto with_loads) {
-        constexpr int P = MT * NT, R = MT + NT, W = decltype(with_loads)::value ? kRuns : 0;
+    // The products of a step's 32 bytes on fragments `buf`, with the reads of the next 32's fragments (into the other buffer)
+    // and a share `group` of a later step's loads between them, an instruction or two to each product: a wave has its SIMD
+    // to itself, and what it issues between two products runs in their shadow.
+    auto part = [&](int buf, lds_ptr next, auto group) {
+        constexpr int P = MT * NT, H = P / 2, R = MT + NT, W0 = group_begin(decltype(group)::value), W = group_begin(decltype(group)::value + 1) - W0;
         static_for<0, P>([&](auto step) {
             constexpr int i = decltype(step)::value;
-            static_for<i * R / P, (i + 1) * R / P>([&](auto k) { read_one(buf ^ 1, next, k); });
-            static_for<i * W / P, (i + 1) * W / P>([&](auto k) { load_run(k); });
+            // the reads in the first half: what the next part begins with has arrived by then
+            if constexpr (i < H) static_for<i * R / H, (i + 1) * R / H>([&](auto k) { read_one(buf ^ 1, next, k); });
+            else static_for<W0 + (i - H) * W / (P - H), W0 + (i - H + 1) * W / (P - H)>([&](auto k) { load_run(k); });
             acc[i % MT][i / MT] = Product<T>::mac(fa[buf][i % MT], fb[buf][i / MT], acc[i % MT][i / MT]);
             __builtin_amdgcn_sched_barrier(0);
         });
@@ -281,12 +289,14 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
 
     // loads that may still be in flight when a step's operands must have landed
     constexpr int kInFlight = (STAGES - 2) * kRuns;
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < STAGES - 1; ++s) {
         load_begin(s);
         static_for<0, kRuns>([&](auto k) { load_run(k); });
         load_end();
     }
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kInFlight + kRuns) : "memory");
+    load_begin(STAGES - 1);
+    static_for<0, group_begin(1)>([&](auto k) { load_run(k); });
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kInFlight + group_begin(1)) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     clear();
@@ -297,16 +307,17 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
     for (int tile = 0; tile < tiles; ++tile) {
         for (int k = 0; k < ksteps; ++k) {
             const lds_ptr at = smem + stage * L::kStage;
-            quarter(0, at + frag[1], no);
-            quarter(1, at + frag[2], no);
-            quarter(0, at + frag[3], no);
+            static_for<0, L::kSubs - 1>([&](auto s) {
+                constexpr int i = decltype(s)::value;
+                part(i & 1, at + frag[i + 1], std::integral_constant<int, i + 1>{});
+            });
+            load_end();
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kInFlight) : "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
             load_begin(stage);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
-            quarter(1, smem + stage * L::kStage + frag[0], yes);
-            load_end();
+            part(1, smem + stage * L::kStage + frag[0], std::integral_constant<int, 0>{});
         }
         const int m0 = v0 + tile * kBM + wm;
         if (m0 + L::kWaveM > v1) finish_tile(m0, yes);
