@@ -122,10 +122,10 @@ def lib() -> ctypes.CDLL:
     L.ma_adamw_workspace_bytes.restype = c_size_t
     L.ma_adamw_workspace_bytes.argtypes = [c_int]
     L.ma_adamw_step.restype = c_int
-    L.ma_adamw_step.argtypes = [POINTER(MaAdamwTensor), c_int, c_int, c_double, c_void_p, c_double, c_double, c_double, c_double,
+    L.ma_adamw_step.argtypes = [c_void_p, c_int, c_int, c_double, c_void_p, c_double, c_double, c_double, c_double,
                                 c_double, c_void_p, c_void_p, c_void_p, c_uint32, c_void_p, c_size_t, c_void_p]
     L.ma_grad_norm.restype = c_int
-    L.ma_grad_norm.argtypes = [POINTER(MaAdamwTensor), c_int, c_double, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+    L.ma_grad_norm.argtypes = [c_void_p, c_int, c_double, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
     L.ma_rmsnorm_bwd.restype = c_int
     L.ma_rmsnorm_bwd.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_int64, c_int,
                                  c_int, c_int, c_void_p]
@@ -180,6 +180,19 @@ def ptr(t: torch.Tensor | None):
 
 def current_stream(device) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def launch(dev: torch.device, fn, *args) -> None:
+    """Calls a C entry point on the current stream of ``dev``, its last argument, with ``dev`` current, and checks the
+    return code.  For calls whose host time counts: nothing is set up that is in place already."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != MA_OK:
+        check(rc)
 
 
 def require_gpu(t: torch.Tensor, what: str) -> None:

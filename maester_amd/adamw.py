@@ -11,9 +11,10 @@ stochastically from a hash of (seed, step, index of the tensor, element): the sa
 """
 from __future__ import annotations
 
-import ctypes
+from operator import attrgetter
 from typing import NamedTuple, Sequence
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -38,28 +39,39 @@ class Blocks8(NamedTuple):
         return (flat * self.scales.repeat_interleave(BLOCK)[:flat.numel()]).view(self.codes.shape)
 
 
-def _dense(t: torch.Tensor, what: str, like: torch.Tensor, dtypes) -> int:
-    if t.dtype not in dtypes:
-        raise TypeError(f"{what} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if t.shape != like.shape or not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous and of its parameter's shape {tuple(like.shape)}, got {tuple(t.shape)}")
-    if t.device != like.device:
-        raise ValueError(f"{what} must be on its parameter's device {like.device}, got {t.device}")
-    return t.data_ptr()
+_ACTIVATION = frozenset((torch.bfloat16, torch.float32))
+_F32 = frozenset((torch.float32,))
+_E4M3 = frozenset((torch.float8_e4m3fn,))
+_CODE = {torch.bfloat16: _lib.MA_DTYPE_BF16, torch.float32: _lib.MA_DTYPE_F32}
+_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
+# the C struct's layout, for columns filled at once
+_ROW = np.dtype(_lib.MaAdamwTensor)
 
 
-_ACTIVATION = (torch.bfloat16, torch.float32)
-_F32 = (torch.float32,)
-_E4M3 = (torch.float8_e4m3fn,)
+def _device(tensors, who: str) -> torch.device:
+    """The one GPU that all of ``tensors`` are on."""
+    _lib.require_gpu(tensors[0], who)
+    indices = set(map(torch.Tensor.get_device, tensors))
+    if len(indices) > 1:
+        raise (RuntimeError if -1 in indices else ValueError)(f"{who}: tensors on several devices; one call takes one GPU's")
+    return tensors[0].device
 
 
-def _one_device(tensors, who: str) -> torch.device:
-    for t in tensors:
-        _lib.require_gpu(t, who)
-    devices = {t.device for t in tensors}
-    if len(devices) > 1:
-        raise ValueError(f"{who}: tensors on several devices ({', '.join(sorted(map(str, devices)))}); one call per device")
-    return next(iter(devices))
+def _addresses(tensors, what: str, shapes: list, dtypes: frozenset, dev: torch.device) -> list:
+    """Data pointers of ``tensors`` after checking them against the parameters' shapes and device (whole lists at a time:
+    a step over hundreds of small tensors is as fast as its host code)."""
+    found = set(map(_dtype, tensors))
+    if not found <= dtypes:
+        raise TypeError(f"{what} must be {' or '.join(sorted(map(str, dtypes)))}, got {', '.join(sorted(map(str, found - dtypes)))}")
+    if list(map(_shape, tensors)) != shapes or not all(map(torch.Tensor.is_contiguous, tensors)):
+        raise ValueError(f"{what} must be contiguous and of its parameter's shape")
+    if set(map(torch.Tensor.get_device, tensors)) != {dev.index}:
+        raise ValueError(f"{what} must be on its parameter's device {dev}")
+    return list(map(torch.Tensor.data_ptr, tensors))
+
+
+def _codes(tensors) -> list:
+    return [_CODE[t.dtype] for t in tensors]
 
 
 def _scalar(t: torch.Tensor, what: str, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
@@ -81,16 +93,15 @@ def global_grad_norm(grads: Sequence[torch.Tensor], max_norm: float | None = Non
         raise ValueError("no gradients")
     if max_norm is not None and not float(max_norm) >= 0:
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
-    dev = _one_device(grads, "global_grad_norm")
-    table = (_lib.MaAdamwTensor * len(grads))()
-    for row, g in zip(table, grads):
-        row.grad, row.n, row.grad_dtype = _dense(g, "a gradient", g, _ACTIVATION), g.numel(), _lib.dtype_code(g.dtype)
+    dev = _device(grads, "global_grad_norm")
+    table = np.zeros(len(grads), dtype=_ROW)
+    table["grad"] = _addresses(grads, "a gradient", list(map(_shape, grads)), _ACTIVATION, dev)
+    table["n"] = list(map(torch.Tensor.numel, grads))
+    table["grad_dtype"] = _codes(grads)
     out = torch.empty(2, dtype=torch.float32, device=dev)
     ws, n = _workspace(len(grads), dev)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().ma_grad_norm(table, len(grads), -1.0 if max_norm is None else float(max_norm), out.data_ptr(),
-                                     out.data_ptr() + 4, ws.data_ptr(), n, _lib.current_stream(dev))
-    _lib.check(rc)
+    _lib.launch(dev, _lib.lib().ma_grad_norm, table.ctypes.data, len(grads), -1.0 if max_norm is None else float(max_norm),
+                out.data_ptr(), out.data_ptr() + 4, ws.data_ptr(), n)
     return out[0] if max_norm is None else (out[0], out[1])
 
 
@@ -120,30 +131,29 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         raise ValueError("max_grad_norm must be >= 0 and cannot be given together with clip")
     if not 0 <= int(seed) < 1 << 32:
         raise ValueError("seed must be in [0, 2^32)")
-    dev = _one_device(params, "adamw_step")
-    eight = isinstance(exp_avgs[0], Blocks8)
-    table = (_lib.MaAdamwTensor * n)()
-    for row, p, g, m, v, w in zip(table, params, grads, exp_avgs, exp_avg_sqs, masters):
-        if isinstance(m, Blocks8) != eight or isinstance(v, Blocks8) != eight:
-            raise ValueError("exp_avgs and exp_avg_sqs must all be tensors or all Blocks8")
-        row.param, row.param_dtype = _dense(p, "a parameter", p, _ACTIVATION), _lib.dtype_code(p.dtype)
-        row.grad, row.grad_dtype = _dense(g, "a gradient", p, _ACTIVATION), _lib.dtype_code(g.dtype)
-        row.n = p.numel()
-        if eight:
-            row.exp_avg, row.exp_avg_sq = _dense(m.codes, "codes", p, _E4M3), _dense(v.codes, "codes", p, _E4M3)
-            blocks = -(-p.numel() // BLOCK)
-            for s in (m.scales, v.scales):
-                if s.dtype != torch.float32 or s.shape != (blocks,) or not s.is_contiguous() or s.device != dev:
-                    raise ValueError(f"scales must be contiguous fp32 [{blocks}] on {dev}")
-            row.exp_avg_scale, row.exp_avg_sq_scale = m.scales.data_ptr(), v.scales.data_ptr()
-        else:
-            row.exp_avg, row.exp_avg_sq = _dense(m, "exp_avg", p, _F32), _dense(v, "exp_avg_sq", p, _F32)
-        if w is not None:
-            if p.dtype != torch.bfloat16:
-                raise ValueError("a master belongs to a bf16 parameter")
-            row.master = _dense(w, "a master", p, _F32)
-    if len({row.param for row in table if row.n}) < sum(1 for row in table if row.n):
+    dev = _device(params, "adamw_step")
+    kinds = set(map(type, exp_avgs)) | set(map(type, exp_avg_sqs))
+    eight = Blocks8 in kinds
+    if eight and len(kinds) > 1:
+        raise ValueError("exp_avgs and exp_avg_sqs must all be tensors or all Blocks8")
+    shapes, sizes = list(map(_shape, params)), list(map(torch.Tensor.numel, params))
+    table = np.zeros(n, dtype=_ROW)
+    where = _addresses(params, "a parameter", shapes, _ACTIVATION, dev)
+    if len(set(where)) < n and len({a for a, k in zip(where, sizes) if k}) < sum(map(bool, sizes)):
         raise ValueError("a parameter is listed twice")
+    table["param"], table["param_dtype"], table["n"] = where, _codes(params), sizes
+    table["grad"], table["grad_dtype"] = _addresses(grads, "a gradient", shapes, _ACTIVATION, dev), _codes(grads)
+    for name, states in (("exp_avg", exp_avgs), ("exp_avg_sq", exp_avg_sqs)):
+        if eight:
+            table[name] = _addresses([q.codes for q in states], "codes", shapes, _E4M3, dev)
+            table[name + "_scale"] = _addresses([q.scales for q in states], "scales", [(-(-k // BLOCK),) for k in sizes], _F32, dev)
+        else:
+            table[name] = _addresses(states, name, shapes, _F32, dev)
+    held = [i for i, w in enumerate(masters) if w is not None]
+    if held:
+        if any(params[i].dtype != torch.bfloat16 for i in held):
+            raise ValueError("a master belongs to a bf16 parameter")
+        table["master"][held] = _addresses([masters[i] for i in held], "a master", [shapes[i] for i in held], _F32, dev)
     _scalar(step, "step", torch.int64, dev)
     on_device = isinstance(lr, torch.Tensor)
     if on_device:
@@ -152,12 +162,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         _scalar(clip, "clip", torch.float32, dev)
     norm = torch.empty((), dtype=torch.float32, device=dev) if max_grad_norm is not None else None
     ws, ws_bytes = _workspace(n, dev)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().ma_adamw_step(
-            table, n, 8 if eight else 32, 0.0 if on_device else float(lr), _lib.ptr(lr) if on_device else None, float(betas[0]),
-            float(betas[1]), float(eps), float(weight_decay), -1.0 if max_grad_norm is None else float(max_grad_norm),
-            _lib.ptr(clip), _lib.ptr(norm), _lib.ptr(step), int(seed), ws.data_ptr(), ws_bytes, _lib.current_stream(dev))
-    _lib.check(rc)
+    _lib.launch(dev, _lib.lib().ma_adamw_step, table.ctypes.data, n, 8 if eight else 32, 0.0 if on_device else float(lr),
+                lr.data_ptr() if on_device else None, float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
+                -1.0 if max_grad_norm is None else float(max_grad_norm), None if clip is None else clip.data_ptr(),
+                None if norm is None else norm.data_ptr(), step.data_ptr(), int(seed), ws.data_ptr(), ws_bytes)
     return norm
 
 

@@ -53,22 +53,17 @@ def linear_token_logprobs_forward(e, c, targets, ignore_index=-100, softcap=None
         L = _lib.lib()
         ws_bytes = L.ma_linear_logprobs_workspace_bytes(n, vocab)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=e.device)
-        with torch.cuda.device(e.device):
-            rc = L.ma_linear_logprobs_fwd(_lib.ptr(e), _pitch(e), _lib.ptr(c), _pitch(c), _lib.ptr(targets), n, vocab, e.shape[1],
-                                          int(ignore_index), softcap, temperature, _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(stats),
-                                          _lib.ptr(ws), ws_bytes, _lib.dtype_code(e.dtype), _lib.current_stream(e.device))
-        _lib.check(rc)
+        _lib.launch(e.device, L.ma_linear_logprobs_fwd, e.data_ptr(), _pitch(e), c.data_ptr(), _pitch(c), targets.data_ptr(), n, vocab,
+                    e.shape[1], int(ignore_index), softcap, temperature, logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
+                    ws.data_ptr(), ws_bytes, _lib.dtype_code(e.dtype))
     return logp, entropy, stats
 
 
 def _dlogits(e, c, targets, stats, entropy, dlogp, dentropy, ignore_index, softcap, temperature, out):
     """Gradient of the logits of a block of rows into ``out`` ``[rows, pitch]``."""
-    with torch.cuda.device(e.device):
-        rc = _lib.lib().ma_linear_logprobs_dlogits(
-            _lib.ptr(e), _pitch(e), _lib.ptr(c), _pitch(c), _lib.ptr(targets), e.shape[0], c.shape[0], e.shape[1], int(ignore_index),
-            softcap, temperature, _lib.ptr(stats), _lib.ptr(entropy), _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.ptr(out), out.shape[1],
-            _lib.dtype_code(e.dtype), _lib.current_stream(e.device))
-    _lib.check(rc)
+    _lib.launch(e.device, _lib.lib().ma_linear_logprobs_dlogits, _lib.ptr(e), _pitch(e), _lib.ptr(c), _pitch(c), _lib.ptr(targets),
+                e.shape[0], c.shape[0], e.shape[1], int(ignore_index), softcap, temperature, _lib.ptr(stats), _lib.ptr(entropy),
+                _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.ptr(out), out.shape[1], _lib.dtype_code(e.dtype))
 
 
 def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentropy, ignore_index=-100, softcap=None,
@@ -140,6 +135,10 @@ def linear_token_logprobs(e: torch.Tensor, c: torch.Tensor, targets: torch.Tenso
     if e.dim() < 1 or targets.shape != e.shape[:-1]:
         raise ValueError(f"targets shape {tuple(targets.shape)} != leading shape of e {tuple(e.shape[:-1])}")
     lead = targets.shape
-    logp, entropy = _LinearTokenLogprobsFn.apply(e.reshape(targets.numel(), e.shape[-1]), c, targets.reshape(-1), int(ignore_index),
-                                                 softcap, temperature, chunk_rows)
-    return logp.view(lead), entropy.view(lead)
+    if len(lead) != 1:
+        e, targets = e.reshape(targets.numel(), e.shape[-1]), targets.reshape(-1)
+    if torch.is_grad_enabled() and (e.requires_grad or c.requires_grad):
+        logp, entropy = _LinearTokenLogprobsFn.apply(e, c, targets, int(ignore_index), softcap, temperature, chunk_rows)
+    else:
+        logp, entropy, _ = linear_token_logprobs_forward(e, c, targets, ignore_index, softcap, temperature)
+    return (logp, entropy) if len(lead) == 1 else (logp.view(lead), entropy.view(lead))

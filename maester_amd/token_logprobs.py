@@ -33,36 +33,34 @@ def check_softmax_arguments(softcap, temperature) -> tuple[float, float]:
     return softcap, float(temperature)
 
 
-def token_logprobs_forward(logits, targets, top_k=0, ignore_index=-100, softcap=None, temperature=1.0):
+def token_logprobs_forward(logits, targets, top_k=0, ignore_index=-100, softcap=None, temperature=1.0, need_stats=True):
     """``(logp, entropy, stats, top_ids, top_logp)`` of ``logits`` ``[rows, vocab]`` (rows may be strided) and int64
-    ``targets`` ``[rows]``; ``stats`` ``[rows, 2]`` is what the gradient needs of the forward."""
+    ``targets`` ``[rows]``; ``stats`` ``[rows, 2]`` is what the gradient needs of the forward (``need_stats=False``: None)."""
     _lib.require_gpu(logits, "token_logprobs")
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError("logits must be [rows, vocab] with unit stride along the vocabulary")
     rows, vocab = logits.shape
-    if targets.shape != (rows,) or targets.dtype != torch.int64 or targets.device != logits.device:
-        raise ValueError("targets must be int64 [rows] on the device of the logits")
-    if not 0 <= int(top_k) <= min(_lib.MA_LOGPROBS_MAX_TOP, vocab):
-        raise ValueError(f"top_k must be in 0 .. {_lib.MA_LOGPROBS_MAX_TOP} and at most the vocabulary of {vocab}, got {top_k}")
-    top_k = int(top_k)
-    softcap, temperature = check_softmax_arguments(softcap, temperature)
-    targets = targets.contiguous()
     dev = logits.device
+    if targets.shape != (rows,) or targets.dtype != torch.int64 or targets.device != dev:
+        raise ValueError("targets must be int64 [rows] on the device of the logits")
+    top_k = int(top_k)
+    if not 0 <= top_k <= min(_lib.MA_LOGPROBS_MAX_TOP, vocab):
+        raise ValueError(f"top_k must be in 0 .. {_lib.MA_LOGPROBS_MAX_TOP} and at most the vocabulary of {vocab}, got {top_k}")
+    softcap, temperature = check_softmax_arguments(softcap, temperature)
+    code = _lib.dtype_code(logits.dtype)
+    targets = targets.contiguous()
     logp, entropy = torch.empty(2, rows, dtype=torch.float32, device=dev).unbind()
-    stats = torch.empty(rows, 2, dtype=torch.float32, device=dev)
+    stats = torch.empty(rows, 2, dtype=torch.float32, device=dev) if need_stats else None
     top_ids = torch.empty(rows, top_k, dtype=torch.int64, device=dev) if top_k else None
     top_logp = torch.empty(rows, top_k, dtype=torch.float32, device=dev) if top_k else None
-    code = _lib.dtype_code(logits.dtype)
     if rows:
         L = _lib.lib()
         ws_bytes = L.ma_token_logprobs_workspace_bytes(rows, vocab, top_k)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-        with torch.cuda.device(dev):
-            rc = L.ma_token_logprobs_fwd(
-                _lib.ptr(logits), _row_pitch(logits), _lib.ptr(targets), rows, vocab, int(ignore_index), softcap, temperature,
-                top_k, _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(stats), _lib.ptr(top_ids), _lib.ptr(top_logp),
-                _lib.ptr(ws), ws_bytes, code, _lib.current_stream(dev))
-        _lib.check(rc)
+        _lib.launch(dev, L.ma_token_logprobs_fwd, logits.data_ptr(), _row_pitch(logits), targets.data_ptr(), rows, vocab, int(ignore_index),
+                    softcap, temperature, top_k, logp.data_ptr(), entropy.data_ptr(), stats.data_ptr() if need_stats else None,
+                    top_ids.data_ptr() if top_k else None, top_logp.data_ptr() if top_k else None, ws.data_ptr() if ws_bytes else None,
+                    ws_bytes, code)
     return logp, entropy, stats, top_ids, top_logp
 
 
@@ -79,12 +77,9 @@ def token_logprobs_backward(logits, targets, stats, entropy, dlogp, dentropy, ig
     rows, vocab = logits.shape
     dlogp, dentropy = (None if t is None else t.float().contiguous() for t in (dlogp, dentropy))
     if rows:
-        with torch.cuda.device(logits.device):
-            rc = _lib.lib().ma_token_logprobs_bwd(
-                _lib.ptr(logits), _row_pitch(logits), _lib.ptr(targets), rows, vocab, int(ignore_index), softcap, temperature,
-                _lib.ptr(stats), _lib.ptr(entropy), _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.ptr(dlogits), vocab,
-                _lib.dtype_code(logits.dtype), _lib.current_stream(logits.device))
-        _lib.check(rc)
+        _lib.launch(logits.device, _lib.lib().ma_token_logprobs_bwd, _lib.ptr(logits), _row_pitch(logits), _lib.ptr(targets), rows, vocab,
+                    int(ignore_index), softcap, temperature, _lib.ptr(stats), _lib.ptr(entropy), _lib.ptr(dlogp), _lib.ptr(dentropy),
+                    _lib.ptr(dlogits), vocab, _lib.dtype_code(logits.dtype))
     return dlogits
 
 
@@ -123,9 +118,12 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
     lead, vocab = targets.shape, logits.shape[-1]
     if vocab < 1:
         raise ValueError("empty vocabulary")
-    rows = targets.numel()
-    out = _TokenLogprobsFn.apply(logits.reshape(rows, vocab), targets.reshape(rows), int(top_k), int(ignore_index), softcap, temperature)
-    logp, entropy, top_ids, top_logp = out
+    if len(lead) != 1:
+        logits, targets = logits.reshape(targets.numel(), vocab), targets.reshape(-1)
+    if logits.requires_grad and torch.is_grad_enabled():
+        logp, entropy, top_ids, top_logp = _TokenLogprobsFn.apply(logits, targets, int(top_k), int(ignore_index), softcap, temperature)
+    else:
+        logp, entropy, _, top_ids, top_logp = token_logprobs_forward(logits, targets, top_k, ignore_index, softcap, temperature, False)
     if len(lead) != 1:
         logp, entropy = logp.view(lead), entropy.view(lead)
         if top_ids is not None:
