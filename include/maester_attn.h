@@ -202,8 +202,8 @@ int ma_transpose(const void* src, void* dst, int64_t rows, int64_t cols, int src
  *   ascending index (a NaN logit ranks with -inf), for every row; NULL with top_k = 0.
  *   workspace: at least ma_token_logprobs_workspace_bytes(...) bytes (0 with many rows: then it may be
  *   NULL), 16-byte aligned, where the parts that few rows are cut into leave their results.
- * Logits of -inf have probability 0.  A row with a NaN or +inf, or with nothing but -inf, has NaN
- * outputs.  ma_token_logprobs_bwd: dlogits (rows `dpitch` apart, may alias logits) =
+ * Logits of -inf have probability 0 (with a soft cap they are -softcap).  A row with a NaN or +inf (with
+ * a soft cap: a NaN), or with nothing but -inf, has NaN outputs.  ma_token_logprobs_bwd: dlogits (rows `dpitch` apart, may alias logits) =
  *   dlogp * d logp + dentropy * d entropy, zeros for a row that does not count; either of dlogp /
  *   dentropy (fp32 [rows]) may be NULL (= 0); stats and entropy as the forward wrote them. */
 #define MA_LOGPROBS_MAX_TOP 64

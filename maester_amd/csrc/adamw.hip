@@ -129,12 +129,6 @@ __device__ __forceinline__ int scale_field(float top) {
     const int k = (int)((__float_as_uint(top) + 0x1FFFFFu) >> 23) - 8;
     return k < 1 ? 1 : k;
 }
-// |x| * 2^-k as an e4m3 code: 20 bits below the code's last are rounded up with probability their value (r: 20 random bits)
-__device__ __forceinline__ uint32_t code_of(float y, uint32_t r) {
-    const uint32_t normal = ((__float_as_uint(y) + r) >> 20) - 960u;       // 120 << 3: e4m3's exponent starts at 2^-7
-    const uint32_t small = ((uint32_t)(y * 536870912.f) + r) >> 20;        // multiples of 2^-9 below 2^-6
-    return y >= 0.015625f ? normal : small;
-}
 // the largest of a block's 128 magnitudes, 8 in each of 16 neighbouring lanes; NaN if one is
 __device__ __forceinline__ float block_top(const float* v) {
     uint32_t m = 0;      // magnitudes compare as integers, NaN above all
@@ -144,6 +138,10 @@ __device__ __forceinline__ float block_top(const float* v) {
     for (int off = 8; off > 0; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, 64));
     return __uint_as_float(m);
 }
+// Codes of y = |x| * 2^-k: the 20 bits below a code's last are rounded up with probability their value (r: 20 random
+// bits).  From 2^-6 on a code is the float's own exponent and first three mantissa bits (less 120 << 3: e4m3's exponent
+// starts at 2^-7); below, multiples of 2^-9.  The second kind costs twice as much and is rare (a code there is less than
+// 3.5e-5 to 7e-5 of its block's largest), so a wave without one leaves it out.
 template <bool POSITIVE>
 __device__ __forceinline__ void encode(const float* v, const uint32_t* h, uint32_t* w, float& scale) {
     const float top = block_top(v);
@@ -151,15 +149,52 @@ __device__ __forceinline__ void encode(const float* v, const uint32_t* h, uint32
     const int k = scale_field(top);
     scale = finite ? __uint_as_float((uint32_t)k << 23) : NAN;     // a block with an inf or a NaN is NaN from here on
     const float inv = __uint_as_float((uint32_t)(254 - k) << 23);
+    float y[8];
+    uint32_t c[8], r[8];
+    float least = INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        y[e] = fabsf(v[e]) * inv;
+        least = fminf(least, y[e]);
+        r[e] = ((POSITIVE ? h[e] >> 12 : h[e] << 4) & 0xffff0u) | 8u;
+        c[e] = (__float_as_uint(y[e]) + (r[e] - (960u << 20))) >> 20;
+    }
+    if (__any(least < 0.015625f)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t small = ((uint32_t)(y[e] * 536870912.f) + r[e]) >> 20;
+            c[e] = y[e] >= 0.015625f ? c[e] : small;
+            if (POSITIVE) c[e] = max(c[e], min(__float_as_uint(v[e]), 1u));
+        }
+    }
     w[0] = w[1] = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const uint32_t bits = __float_as_uint(v[e]);
-        const uint32_t r = (POSITIVE ? h[e] >> 16 : h[e] & 0xffffu) * 16u + 8u;
-        uint32_t c = code_of(__uint_as_float(bits & 0x7fffffffu) * inv, r);
-        if (POSITIVE) c = bits && c == 0 ? 1u : c;
-        else c |= (bits >> 24) & 0x80u;
-        w[e >> 2] |= (finite ? c : 0u) << (8 * (e & 3));
+        if (!POSITIVE) c[e] |= (__float_as_uint(v[e]) >> 24) & 0x80u;
+        w[e >> 2] |= c[e] << (8 * (e & 3));
+    }
+    w[0] = finite ? w[0] : 0u;
+    w[1] = finite ? w[1] : 0u;
+}
+
+// sqrt of 8 values, correctly rounded: the hardware's root (one step off at most) and one correction with its exact
+// residual, taken one step lower, as the root's curvature lies below its tangent (without that 4^k (1 - 2^-24), whose root
+// lies 2^-51 beside a midpoint, comes out a step high; with it every float of seven binades agrees with the fp64 root).  Residuals of values near the end of the exponent range would underflow, and infinity has none:
+// those waves take the library's root.
+__device__ __forceinline__ void roots8(const float* v, float* r) {
+    uint32_t low = 0xffffffffu, high = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float s = __builtin_amdgcn_sqrtf(v[e]);
+        const float half = 0.5f * __builtin_amdgcn_rcpf(fmaxf(s, 1e-30f));
+        const float left = fmaf(-s, s, v[e]);
+        r[e] = fmaf(fmaf(-fabsf(left), 0x1p-23f, left), half, s);
+        low = min(low, __float_as_uint(v[e]) - 1u);          // (zero, whose residual is zero, wraps to the top)
+        high = max(high, __float_as_uint(v[e]));
+    }
+    if (__any(low < 0x0f800000u || high >= 0x7f800000u)) {   // 2^-96
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = sqrtf(v[e]);
     }
 }
 
@@ -194,8 +229,13 @@ __device__ __forceinline__ void step8(const ma_adamw_tensor& t, int64_t i, uint3
         const float ge = g[e] * s.clip;
         m[e] = m[e] * s.b1 + ge * s.one_b1;
         v[e] = v[e] * s.b2 + ge * ge * s.one_b2;
-        r[e] = sqrtf(v[e]);
-        p[e] = p[e] * s.decay - s.step_size * (m[e] / (r[e] * s.inv_root_bc + s.eps));
+    }
+    roots8(v, r);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        // (the reciprocal is one step off at most, of an update that is a fraction of the weight)
+        const float update = s.step_size * (m[e] * __builtin_amdgcn_rcpf(r[e] * s.inv_root_bc + s.eps));
+        p[e] = p[e] * s.decay - update;
     }
     if (BITS == 32) {
         store8<float>((float*)t.exp_avg, i, n, whole, m);
@@ -206,7 +246,7 @@ __device__ __forceinline__ void step8(const ma_adamw_tensor& t, int64_t i, uint3
         float sm, sr;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            h[e] = mix((uint32_t)(i + e) * 0x9E3779B9u + key);
+            h[e] = mix((uint32_t)i * 0x9E3779B9u + (e * 0x9E3779B9u + key));
             if (e >= n) m[e] = r[e] = 0.f;
         }
         encode<false>(m, h, wm, sm);

@@ -264,7 +264,7 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
 #pragma unroll
                         for (int v = 0; v < 4; ++v) {
                             const float x = acc[i][j][4 * q + v];
-                            const float th = CAP ? tanhf(x * a.sh.inv_cap) : 0.f;
+                            const float th = CAP ? lp_tanh(x * a.sh.inv_cap) : 0.f;
                             const float lp = fmaf((CAP ? a.sh.cap * th : x) - top[j], a.sh.inv_temp, -log_l[j]);
                             const float p = __builtin_amdgcn_exp2f(lp * kLpLog2e);
                             d[v] = -p * fmaf(gb[j], fmaxf(lp, -1e30f) + ent[j], ga[j]);

@@ -16,8 +16,21 @@ struct LpShape {
     float cap, inv_cap, inv_temp;
 };
 inline LpShape lp_shape(float softcap, float temperature) { return {softcap, softcap > 0.f ? 1.f / softcap : 0.f, 1.f / temperature}; }
+// tanh: its series up to 0.35 (six terms; the seventh is below 2^-26 of the value there), 1 - 2 / (exp(2 |z|) + 1) above
+// (off by 2^-23 at most); 18 instructions, where the library's function made a capped fp32 row bound by arithmetic
+// (48 x 262208 in 40 us against 25).
+__device__ __forceinline__ float lp_tanh(float z) {
+    const float a = fabsf(z), q = z * z;
+    const float big = fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(a * (2.f * kLpLog2e)) + 1.f), 1.f);
+    float t = fmaf(q, -1382.f / 155925.f, 62.f / 2835.f);
+    t = fmaf(q, t, -17.f / 315.f);
+    t = fmaf(q, t, 2.f / 15.f);
+    t = fmaf(q, t, -1.f / 3.f);
+    t = fmaf(a * q, t, a);
+    return copysignf(a < 0.35f ? t : big, z);
+}
 template <bool CAP>
-__device__ __forceinline__ float lp_capped(float x, const LpShape& s) { return CAP ? s.cap * tanhf(x * s.inv_cap) : x; }
+__device__ __forceinline__ float lp_capped(float x, const LpShape& s) { return CAP ? s.cap * lp_tanh(x * s.inv_cap) : x; }
 
 // running maximum (in units of the capped logits), sum of exp((y - m) / T) and of (y - m) / T * exp((y - m) / T)
 struct LpStats {

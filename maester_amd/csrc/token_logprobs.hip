@@ -66,6 +66,13 @@ struct Row {
             for (int i = 0; i < 8; ++i) v[i] = j + i >= 0 && j + i < vocab ? ld1<T>(p + j + i) : -INFINITY;
         }
     }
+    // -inf again for what lies outside the row, after a cap has made it finite
+    __device__ __forceinline__ void exclude(int g, float* v) const {
+        if (whole(g)) return;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (first(g) + i < 0 || first(g) + i >= vocab) v[i] = -INFINITY;
+    }
 };
 
 // the statistics of the whole workgroup, in every thread; box: one slot per wave
@@ -120,13 +127,20 @@ __device__ __forceinline__ uint64_t wave_sort_descending(uint64_t k) {
 
 // LDS of the selection: keys (one slot a thread), the number of them that are in use
 struct Selection {
-    uint64_t key[kLpThreads];
+    alignas(16) uint64_t key[kLpThreads];
     int count;
 };
 // Number of the n keys in LDS that are larger than `key`: its rank, as keys are unique.
 __device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int n) {
-    int rank = 0;
-    for (int i = 0; i < n; ++i) rank += keys[i] > key ? 1 : 0;
+    int rank = 0, i = 0;
+    for (; i + 8 <= n; i += 8) {      // eight reads in flight: one at a time costs a read's latency each
+        uint64_t k[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) k[e] = keys[i + e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rank += k[e] > key ? 1 : 0;
+    }
+    for (; i < n; ++i) rank += keys[i] > key ? 1 : 0;
     return rank;
 }
 // The `want` largest of the workgroup's per-thread keys (0: none), best first, in sel.key; returns how many there are
@@ -197,7 +211,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_fwd_kernel(const T*
                                                                         Workspace ws, Outputs out) {
     __shared__ LpStats s_box[kLpWaves];
     __shared__ Selection s_sel;
-    __shared__ uint64_t s_found[kLpThreads];
+    __shared__ alignas(16) uint64_t s_found[kLpThreads];
     __shared__ uint64_t s_key[kLpWaves];
     __shared__ int s_found_n;
     const int tid = threadIdx.x;
@@ -238,6 +252,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_fwd_kernel(const T*
         if (CAP) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = lp_capped<CAP>(v[i], sh);
+            r.exclude(g, v);
         }
         lp_fold<8>(v, sh.inv_temp, t);
     }
@@ -320,7 +335,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(const T
                                                                          Workspace ws, Outputs out) {
     __shared__ LpStats s_box[kLpWaves];
     __shared__ Selection s_sel;
-    __shared__ uint64_t s_found[kLpThreads];
+    __shared__ alignas(16) uint64_t s_found[kLpThreads];
     __shared__ int s_found_n;
     const int tid = threadIdx.x;
     const int64_t row = blockIdx.x;
@@ -389,7 +404,7 @@ __global__ __launch_bounds__(kLpBwdThreads) void token_logprobs_bwd_kernel(const
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float th = CAP ? tanhf(v[i] * sh.inv_cap) : 0.f;
+                const float th = CAP ? lp_tanh(v[i] * sh.inv_cap) : 0.f;
                 const float lp = fmaf((CAP ? sh.cap * th : v[i]) - top, sh.inv_temp, -log_l);
                 const float p = __builtin_amdgcn_exp2f(lp * kLpLog2e);
                 d[i] = -p * fmaf(b, fmaxf(lp, -1e30f) + h, a);

@@ -78,6 +78,26 @@ def test_softcap_and_temperature(gpu, softcap, temperature):
     assert np.array_equal(got.top_ids.cpu().numpy(), want["top_ids"])
 
 
+@pytest.mark.parametrize("vocab", [1, 3, 9, 4099])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_small_caps_on_ragged_rows(gpu, vocab, offset):
+    # a cap so low that an element beside the row, taken for a logit of -cap, would weigh as much as one of the row's
+    buf = torch.randn(7, vocab + 5, generator=torch.Generator().manual_seed(vocab))
+    x, t = buf[:, offset:offset + vocab], torch.arange(7) % vocab
+    got = token_logprobs(buf.to(gpu)[:, offset:offset + vocab], t.to(gpu), top_k=1, softcap=0.5)
+    want = O.rows(x.numpy(), t.numpy(), 1, softcap=0.5)
+    tol = rel_of_sums(vocab) + 16 * U
+    assert np.abs(got.logp.cpu().numpy() - want["logp"]).max() <= 4 * tol
+    assert np.abs(got.entropy.cpu().numpy() - want["entropy"]).max() <= 25 * tol
+    assert np.array_equal(got.top_ids.cpu().numpy(), want["top_ids"])
+    # tanh(-inf) = -1: a soft cap gives banned tokens -cap, as the formula says
+    x = x.clone()
+    x[:, 0] = float("-inf")
+    t = torch.full((7,), vocab - 1)
+    got = token_logprobs(x.contiguous().to(gpu), t.to(gpu), softcap=0.5)
+    assert np.abs(got.logp.cpu().numpy() - O.rows(x.numpy(), t.numpy(), softcap=0.5)["logp"]).max() <= 4 * tol
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_masked_rows(gpu, dtype):
     vocab = 9001
