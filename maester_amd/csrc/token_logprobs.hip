@@ -132,15 +132,8 @@ struct Selection {
 };
 // Number of the n keys in LDS that are larger than `key`: its rank, as keys are unique.
 __device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int n) {
-    int rank = 0, i = 0;
-    for (; i + 8 <= n; i += 8) {      // eight reads in flight: one at a time costs a read's latency each
-        uint64_t k[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) k[e] = keys[i + e];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) rank += k[e] > key ? 1 : 0;
-    }
-    for (; i < n; ++i) rank += keys[i] > key ? 1 : 0;
+    int rank = 0;
+    for (int i = 0; i < n; ++i) rank += keys[i] > key ? 1 : 0;
     return rank;
 }
 // The `want` largest of the workgroup's per-thread keys (0: none), best first, in sel.key; returns how many there are
@@ -238,9 +231,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_fwd_kernel(const T*
     LpStats t = {-INFINITY, 0.f, 0.f};
     float best = -INFINITY;
     int best_g = g0 + tid;
-    for (int g = g0 + tid; g < g1; g += kLpThreads) {
-        float v[8];
-        r.load(g, v);
+    auto take = [&](int g, float* v) {
         if (TOP) {
             float vm = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
             vm = fmaxf(vm, fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
@@ -255,6 +246,30 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_fwd_kernel(const T*
             r.exclude(g, v);
         }
         lp_fold<8>(v, sh.inv_temp, t);
+    };
+    // Four groups' loads at a time, then one: with a single load in flight per thread a row of 128257 comes at 3.3 TB/s.
+    // Only a row's first and last group can be cut, and only those go through the guarded load.
+    const int w0 = g0 + (g0 < g1 && !r.whole(g0) ? 1 : 0), w1 = g1 - (g1 > w0 && !r.whole(g1 - 1) ? 1 : 0);
+    int g = g0 + tid;
+    float v[4][8];
+    if (g < w0) {
+        r.load(g, v[0]);
+        take(g, v[0]);
+        g += kLpThreads;
+    }
+    for (; g + 3 * kLpThreads < w1; g += 4 * kLpThreads) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) ld8<T>(r.p + r.first(g + n * kLpThreads), v[n]);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) take(g + n * kLpThreads, v[n]);
+    }
+    for (; g < w1; g += kLpThreads) {
+        ld8<T>(r.p + r.first(g), v[0]);
+        take(g, v[0]);
+    }
+    if (g < g1) {
+        r.load(g, v[0]);
+        take(g, v[0]);
     }
     t = workgroup_stats(t, sh.inv_temp, s_box);
     if (tid == 0) {
@@ -424,10 +439,11 @@ __global__ __launch_bounds__(kLpBwdThreads) void token_logprobs_bwd_kernel(const
 
 }  // namespace
 
-// Parts that a row is cut into: workgroups for 16 rounds of the chip's 1024 resident ones, but none with fewer than 512
-// groups (a group per thread).
+// Parts that a row is cut into, none with fewer than 512 groups (a group per thread): few rows to two workgroups a compute
+// unit, as a part ends with some 10 us of selection (48 fp32 rows: 26 us, with 4096 workgroups 41); many rows to four
+// rounds of the 1024 resident ones, so that the last round is a small part of them all.
 int token_logprobs_parts(int64_t rows, int64_t vocab) {
-    const int64_t want = (4096 + rows - 1) / rows, most = (vocab / 8 + kLpThreads - 1) / kLpThreads;
+    const int64_t want = rows >= 1024 ? (4096 + rows - 1) / rows : 512 / rows, most = (vocab / 8 + kLpThreads - 1) / kLpThreads;
     const int64_t parts = want < most ? want : most;
     return (int)(parts < 1 ? 1 : parts > kLpMaxParts ? kLpMaxParts : parts);
 }
