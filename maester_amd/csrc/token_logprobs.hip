@@ -27,6 +27,7 @@ namespace {
 
 constexpr int kLpThreads = 512;       // >= 8 * MA_LOGPROBS_MAX_TOP: the waves' best keys, one a thread
 constexpr int kLpWaves = kLpThreads / 64;
+constexpr int kLpMaxParts = 64;       // of a row: a lane each in the join
 
 template <typename T>
 __device__ __forceinline__ float ld1(const T* p);
@@ -341,8 +342,24 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_fwd_kernel(const T*
     }
 }
 
+// The same without alternatives: a wave per row, a part a lane.
+template <typename T, bool CAP>
+__global__ __launch_bounds__(256) void token_logprobs_join_stats_kernel(const T* __restrict__ logits, int64_t pitch,
+                                                                        const int64_t* __restrict__ targets, int64_t rows, int vocab,
+                                                                        int64_t ignore_index, LpShape sh, int parts, Workspace ws,
+                                                                        Outputs out) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= rows) return;
+    LpStats t = {-INFINITY, 0.f, 0.f};
+    if (lane < parts) t = ws.stats[row * parts + lane];
+    for (int off = 1; off < parts; off <<= 1) t = lp_merged(t, lp_shuffled(t, off), sh.inv_temp);
+    if (lane) return;
+    const int64_t target = targets[row];
+    write_row<T, CAP>(Row<T>(logits + row * pitch, vocab), row, target, target != ignore_index && target >= 0 && target < vocab, sh, t, out);
+}
+
 // One workgroup per row of several parts: at most kLpMaxParts statistics and kLpMaxParts * 64 keys, 8 a thread.
-constexpr int kLpMaxParts = 64;
 template <typename T, bool CAP>
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(const T* __restrict__ logits, int64_t pitch,
                                                                          const int64_t* __restrict__ targets, int vocab,
@@ -361,7 +378,6 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(const T
         const int64_t target = targets[row];
         write_row<T, CAP>(Row<T>(logits + row * pitch, vocab), row, target, target != ignore_index && target >= 0 && target < vocab, sh, t, out);
     }
-    if (top_k == 0) return;
     const uint64_t* keys = ws.keys + row * parts * top_k;
     const int n = parts * top_k;
     uint64_t best = 0;
@@ -472,8 +488,12 @@ int fwd(const TokenLogprobsArgs& a, hipStream_t st) {
                                                               a.top_k, parts, ws, out);
     if (parts > 1) {
         MA_TRY(check_launch("token_logprobs_fwd_kernel"));
-        token_logprobs_join_kernel<T, CAP><<<(unsigned)a.rows, kLpThreads, 0, st>>>((const T*)a.logits, a.pitch, a.targets, (int)a.vocab,
-                                                                                     a.ignore_index, sh, a.top_k, parts, ws, out);
+        if (a.top_k)
+            token_logprobs_join_kernel<T, CAP><<<(unsigned)a.rows, kLpThreads, 0, st>>>((const T*)a.logits, a.pitch, a.targets, (int)a.vocab,
+                                                                                         a.ignore_index, sh, a.top_k, parts, ws, out);
+        else
+            token_logprobs_join_stats_kernel<T, CAP><<<(unsigned)((a.rows + 3) / 4), 256, 0, st>>>(
+                (const T*)a.logits, a.pitch, a.targets, a.rows, (int)a.vocab, a.ignore_index, sh, parts, ws, out);
     }
     return check_launch("token_logprobs_fwd_kernel");
 }
