@@ -66,6 +66,13 @@ def _dlogits(e, c, targets, stats, entropy, dlogp, dentropy, ignore_index, softc
                 _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.ptr(out), out.shape[1], _lib.dtype_code(e.dtype))
 
 
+# The library's operand orders for the two gradient products, by rows (262208 x 2560 bf16, ms):
+#   de = x c with c as it is 1.5 / 2.9 / 3.5 / 6.0 / 13.3 at 512 / 1433 / 2047 / 4096 / 8192 rows, with c transposed first
+#   2.0 / 3.3 / 3.3 / 4.7 / 8.9;  dc = x^T e with e as it is 0.9 / 2.0 / 2.7 / 4.9 / 9.7, with e transposed 1.0 / 2.1 /
+#   2.8 / 4.2 / 8.2.
+_TRANSPOSE_C_FROM, _TRANSPOSE_E_FROM = 2000, 3000
+
+
 def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentropy, ignore_index=-100, softcap=None,
                                    temperature=1.0, chunk_rows=None, need_de=True, need_dc=True):
     """``(de, dc)`` (None where not needed) from the gradients of ``logp`` and ``entropy`` (either may be None)."""
@@ -80,9 +87,9 @@ def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentrop
     step = int(chunk_rows) if chunk_rows else default_chunk_rows(vocab, e.element_size(), n)
     step = max(1, min(step, n))
     block = torch.empty(step, -(-vocab // 8) * 8, dtype=e.dtype, device=e.device)
-    c_t = transpose(c.contiguous()) if need_de else None     # the library's faster operand order, as in linear_cross_entropy
+    c_t = transpose(c.contiguous()) if need_de and n >= _TRANSPOSE_C_FROM else None
     mixed = {"out_dtype": torch.float32} if e.dtype != torch.float32 else {}
-    dc_t = None
+    dc = None
     for r0 in range(0, n, step):
         rows = slice(r0, min(n, r0 + step))
         buf = block[: rows.stop - r0]
@@ -90,55 +97,84 @@ def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentrop
                  None if dentropy is None else dentropy[rows], ignore_index, softcap, temperature, buf)
         x = buf[:, :vocab]
         if need_de:
-            torch.mm(x, c_t.t(), out=de[rows])
+            torch.mm(x, c if c_t is None else c_t.t(), out=de[rows])
         if need_dc:
-            e_t = transpose(e[rows].contiguous())
+            hidden = e[rows] if buf.shape[0] < _TRANSPOSE_E_FROM else transpose(e[rows].contiguous()).t()
             if n <= step:
-                dc_t = torch.mm(e_t, x)
-            elif dc_t is None:                   # several blocks: summed in fp32, rounded once at the end
-                dc_t = torch.mm(e_t, x, **mixed)
+                dc = torch.mm(x.t(), hidden)
+            elif dc is None:                     # several blocks: summed in fp32, rounded once at the end
+                dc = torch.mm(x.t(), hidden, **mixed)
             else:
-                torch.addmm(dc_t, e_t, x, out=dc_t, **mixed)
-    return de, transpose(dc_t, c.dtype) if need_dc else None
+                torch.addmm(dc, x.t(), hidden, out=dc, **mixed)
+    return de, dc.to(c.dtype) if need_dc else None
+
+
+# rows that a call has to have before ignored ones are dropped: up to here they fill one block of the kernel's anyway
+_FILTER_FROM = 257
+
+
+def _kept_rows(targets, ignore_index, vocab):
+    """Indices of the rows that count, or None for all of them (the one host synchronisation of a filtered call)."""
+    valid = (targets != ignore_index) & (targets >= 0) & (targets < vocab)
+    keep = torch.nonzero(valid).squeeze(1)
+    return None if keep.numel() == targets.numel() else keep
 
 
 class _LinearTokenLogprobsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, e, c, targets, ignore_index, softcap, temperature, chunk_rows):
+    def forward(ctx, e, c, targets, ignore_index, softcap, temperature, chunk_rows, keep):
+        ctx.rows = e.shape[0]
+        if keep is not None:
+            e, targets = e.index_select(0, keep), targets.index_select(0, keep)
         logp, entropy, stats = linear_token_logprobs_forward(e, c, targets, ignore_index, softcap, temperature)
-        ctx.save_for_backward(e, c, targets, stats, entropy)
+        ctx.save_for_backward(e, c, targets, stats, entropy, keep)
         ctx.args = (ignore_index, softcap, temperature, chunk_rows)
         ctx.set_materialize_grads(False)
-        return logp, entropy
+        return _spread(logp, keep, ctx.rows), _spread(entropy, keep, ctx.rows)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dlogp, dentropy):
         if dlogp is None and dentropy is None:
-            return (None,) * 7
-        e, c, targets, stats, entropy = ctx.saved_tensors
+            return (None,) * 8
+        e, c, targets, stats, entropy, keep = ctx.saved_tensors
+        if keep is not None:
+            dlogp, dentropy = (None if t is None else t.index_select(0, keep) for t in (dlogp, dentropy))
         de, dc = linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentropy, *ctx.args,
                                                 ctx.needs_input_grad[0], ctx.needs_input_grad[1])
-        return de, dc, None, None, None, None, None
+        return None if de is None else _spread(de, keep, ctx.rows), dc, None, None, None, None, None, None
+
+
+def _spread(x, keep, rows):
+    """``x`` of the kept rows as all rows', zeros elsewhere."""
+    return x if keep is None else x.new_zeros((rows, *x.shape[1:])).index_copy_(0, keep, x)
 
 
 def linear_token_logprobs(e: torch.Tensor, c: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
-                          softcap: float | None = None, temperature: float = 1.0,
-                          chunk_rows: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+                          softcap: float | None = None, temperature: float = 1.0, chunk_rows: int | None = None,
+                          filter_ignored: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
     """``(logp, entropy)`` of ``token_logprobs(e @ c.T, targets)``, fp32 of the shape of ``targets``, differentiable (once)
     in ``e`` and ``c``.
 
     ``e`` ``[..., K]`` hidden states, ``c`` ``[V, K]`` classifier (Gemma: the tied embedding table), bf16 or fp32 alike,
     ``K`` a multiple of 8 (fp32: 4); the logits are products of the inputs summed in fp32 and never stored.  ``softcap``,
     ``temperature`` and ignored targets as in ``token_logprobs``.  ``chunk_rows``: rows per block of the backward (default:
-    about 4 GiB of gradient of the logits at a time)."""
+    about 4 GiB of gradient of the logits at a time).  ``filter_ignored``: a call of more than 256 rows drops those whose
+    target does not count before any product, which costs its one host synchronisation; not under graph capture."""
     if e.dim() < 1 or targets.shape != e.shape[:-1]:
         raise ValueError(f"targets shape {tuple(targets.shape)} != leading shape of e {tuple(e.shape[:-1])}")
     lead = targets.shape
     if len(lead) != 1:
         e, targets = e.reshape(targets.numel(), e.shape[-1]), targets.reshape(-1)
+    _check(e, c, targets)
+    keep = None
+    if filter_ignored and e.shape[0] >= _FILTER_FROM and not torch.cuda.is_current_stream_capturing():
+        keep = _kept_rows(targets, ignore_index, c.shape[0])
     if torch.is_grad_enabled() and (e.requires_grad or c.requires_grad):
-        logp, entropy = _LinearTokenLogprobsFn.apply(e, c, targets, int(ignore_index), softcap, temperature, chunk_rows)
+        logp, entropy = _LinearTokenLogprobsFn.apply(e, c, targets, int(ignore_index), softcap, temperature, chunk_rows, keep)
     else:
+        if keep is not None:
+            e, targets = e.index_select(0, keep), targets.index_select(0, keep)
         logp, entropy, _ = linear_token_logprobs_forward(e, c, targets, ignore_index, softcap, temperature)
+        logp, entropy = (_spread(t, keep, lead.numel()) for t in (logp, entropy))
     return (logp, entropy) if len(lead) == 1 else (logp.view(lead), entropy.view(lead))

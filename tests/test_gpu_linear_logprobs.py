@@ -201,6 +201,31 @@ def test_same_bits_every_time_other_stream_and_graph(gpu):
         assert all(torch.equal(a, b) for a, b in zip(got, eager)), i
 
 
+@pytest.mark.parametrize("n,ignore", [(256, 0.5), (257, 0.5), (900, 0.9), (400, 1.0), (300, 0.0)])
+def test_dropped_rows_change_nothing(gpu, n, ignore):
+    e, c, t = problem(n, 64, 1003, torch.bfloat16, n, ignore=ignore)
+    t[0] = -100 if ignore == 1.0 else 5
+    if n == 900:
+        t[7], t[9] = 1003, -3                                 # out of the vocabulary: dropped as well
+    a = torch.randn(n, device=gpu)
+    out = []
+    for flag in (True, False):
+        eg, cg = e.to(gpu).requires_grad_(), c.to(gpu).requires_grad_()
+        logp, entropy = linear_token_logprobs(eg, cg, t.to(gpu), filter_ignored=flag)
+        de, dc = torch.autograd.grad((logp * a + entropy).sum(), (eg, cg))
+        with torch.no_grad():
+            again = linear_token_logprobs(eg, cg, t.to(gpu), filter_ignored=flag)
+        assert torch.equal(again[0], logp) and torch.equal(again[1], entropy)
+        out.append((logp, entropy, de, dc))
+    # a row's own results do not depend on the others up to the order in which the vocabulary's parts are joined; dc sums
+    # the same terms in another order of rows
+    assert float((out[0][0] - out[1][0]).abs().max()) <= 1e-4 and float((out[0][1] - out[1][1]).abs().max()) <= 1e-3
+    for x, y in zip(out[0][2:], out[1][2:]):
+        assert float((x.float() - y.float()).norm()) <= 2 * 2.0 ** -8 * float(y.float().norm()) + 1e-6
+    dead = (t == -100).to(gpu)
+    assert torch.all(out[0][0][dead] == 0) and torch.all(out[0][2][dead] == 0)
+
+
 def test_refusals(gpu):
     e, c, t = (x.to(gpu) for x in problem(4, 64, 30, torch.bfloat16, 6))
     for args, kw in [((e[:, :60], c[:, :60], t), {}), ((e, c.float(), t), {}), ((e, c[:, :32], t), {}), ((e, c, t[:3]), {}), ((e, c, t.int()), {}),
