@@ -67,14 +67,14 @@ template <int BN>
 struct Tiling {
     static constexpr int kWaveM = BN >= 128 ? 128 : 64, kWaveN = BN >= 128 ? BN / 2 : BN;
     static constexpr int kMT = kWaveM / 32, kNT = kWaveN / 32;
-    static constexpr int kStep = 128, kStages = BN == 256 ? 2 : 3;     // bytes of K per step and row
-    static constexpr int kGroups = BN == 256 ? 2 : 4;                 // of a step's loads
+    static constexpr bool kRing = BN == 256;                           // five slots of one operand, or stages of both
+    static constexpr int kStep = 128, kStages = 3;                     // bytes of K per step and row
     static constexpr int kSubs = kStep / 32, kChunks = kStep / 16, kRunRows = 1024 / kStep;
     static constexpr int kARuns = kBM / kRunRows / 4, kBRuns = BN / kRunRows / 4;       // 1 KB loads per wave and step
     static constexpr int kStage = (kBM + BN) * kStep;
     // place of chunk c of row r of a stage: c ^ key(r)
     static constexpr __host__ __device__ int key(int r) { return kStep == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
-    static constexpr int kLds = kStage * kStages;
+    static constexpr int kLds = kRing ? 5 * kBM * kStep : kStage * kStages;
     static_assert(kLds <= 160 * 1024, "LDS");
 };
 
@@ -122,49 +122,45 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
 #pragma unroll
     for (int p = 0; p < L::kBRuns; ++p) b_off[p] = (uint32_t)((w + 4 * p) * L::kRunRows + run_row) * (uint32_t)a.e_stride + chunk * 16;
     const uint32_t lds0 = lds_addr(smem) + w * 1024;
-    // the next step to load: addresses and bytes in range of both operands move on by a step's bytes, and start
-    // over with the next tile's rows; past the last tile nothing is in range
-    int ld_tile = 0, ld_left = a.k_bytes;
-    uint64_t a_at, b_at;
-    uint32_t a_bytes, b_bytes;
-    auto open_tile = [&]() {
-        const int rows_a = ld_tile < tiles ? min(kBM, v1 - v0 - ld_tile * kBM) : 0;
-        const int rows_b = ld_tile < tiles ? min(BN, a.rows - n0) : 0;
-        a_at = (uint64_t)a.c + (uint64_t)(v0 + ld_tile * kBM) * a.c_stride;
-        b_at = (uint64_t)a.e + (uint64_t)n0 * a.e_stride;
-        a_bytes = rows_a ? (uint32_t)((rows_a - 1) * a.c_stride) + a.k_bytes : 0u;
-        b_bytes = rows_b ? (uint32_t)((rows_b - 1) * a.e_stride) + a.k_bytes : 0u;
-        ld_left = a.k_bytes;
+    // the next step of an operand to load: address and bytes in range move on by a step's bytes and start over with the
+    // next tile's rows; past the last tile nothing is in range
+    struct Feed {
+        uint64_t at;
+        uint32_t bytes, past, lds;
+        int left, tile;
+        u32x4 rsrc;
+    } feed[2];                                // c, e
+    auto open = [&](Feed& f, bool is_c) {
+        const int rows = f.tile >= tiles ? 0 : is_c ? min(kBM, v1 - v0 - f.tile * kBM) : min(BN, a.rows - n0);
+        const int64_t stride = is_c ? a.c_stride : a.e_stride;
+        f.at = is_c ? (uint64_t)a.c + (uint64_t)(v0 + f.tile * kBM) * stride : (uint64_t)a.e + (uint64_t)n0 * stride;
+        f.bytes = rows ? (uint32_t)((rows - 1) * stride) + a.k_bytes : 0u;
+        f.left = a.k_bytes;
     };
-    open_tile();
-    u32x4 ra, rbv;
-    uint32_t past, ld_at;
-    auto load_begin = [&](int stage) {
-        ra = uniform_rsrc(a_at, a_bytes);
-        rbv = uniform_rsrc(b_at, b_bytes);
+    feed[0].tile = feed[1].tile = 0;
+    open(feed[0], true);
+    open(feed[1], false);
+    auto begin = [&](Feed& f, uint32_t lds) {
+        f.rsrc = uniform_rsrc(f.at, f.bytes);
         // chunks past the end of a row are the next row's first: out of any descriptor's range
-        past = chunk * 16 < ld_left ? 0u : 0x80000000u;
-        ld_at = __builtin_amdgcn_readfirstlane(lds0 + stage * L::kStage);
+        f.past = chunk * 16 < f.left ? 0u : 0x80000000u;
+        f.lds = __builtin_amdgcn_readfirstlane(lds0 + lds);
     };
-    // a step's loads go out in as many groups as it has parts: the first in the last part of a step, when its stage has
-    // become free, the others in the first parts of the next step
-    constexpr int kRuns = L::kARuns + L::kBRuns;
-    constexpr auto group_begin = [](int g) constexpr { return (g < L::kGroups ? g : L::kGroups) * kRuns / L::kGroups; };
-    auto load_run = [&](auto run) {
-        constexpr int p = decltype(run)::value;
-        if constexpr (p < L::kARuns) buffer_to_lds_run_at<p * 4096>(ra, a_off[p] | past, ld_at);
-        else buffer_to_lds_run_at<kBM * L::kStep + (p - L::kARuns) * 4096>(rbv, b_off[p - L::kARuns] | past, ld_at);
-    };
-    auto load_end = [&]() {
-        a_at += L::kStep;
-        b_at += L::kStep;
-        a_bytes = a_bytes ? a_bytes - L::kStep : 0u;      // (the last step of a tile may wrap: it is opened anew)
-        b_bytes = b_bytes ? b_bytes - L::kStep : 0u;
-        ld_left -= L::kStep;
-        if (ld_left <= 0) {
-            ++ld_tile;
-            open_tile();
+    auto advance = [&](Feed& f, bool is_c) {
+        f.at += L::kStep;
+        f.bytes = f.bytes ? f.bytes - L::kStep : 0u;      // (the last step of a tile may wrap: it is opened anew)
+        f.left -= L::kStep;
+        if (f.left <= 0) {
+            ++f.tile;
+            open(f, is_c);
         }
+    };
+    // runs 0 .. kARuns - 1 of a step are c's, the others e's
+    constexpr int kRuns = L::kARuns + L::kBRuns;
+    auto load_run = [&](auto run) {
+        constexpr int p = decltype(run)::value, q = p - L::kARuns;
+        if constexpr (q < 0) buffer_to_lds_run_at<p * 4096>(feed[0].rsrc, a_off[p] | feed[0].past, feed[0].lds);
+        else buffer_to_lds_run_at<q * 4096>(feed[1].rsrc, b_off[q] | feed[1].past, feed[1].lds);
     };
 
     // ---- fragments: 32 rows, chunks 2 s and 2 s + 1 of a step
@@ -172,10 +168,10 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
 #pragma unroll
     for (int s = 0; s < L::kSubs; ++s) frag[s] = r * L::kStep + (((2 * s + hh) ^ L::key(r)) << 4);
     u32x4 fa[2][MT], fb[2][NT];
-    auto read_one = [&](int buf, lds_ptr at, auto which) {
+    auto read_one = [&](int buf, lds_ptr at_c, lds_ptr at_e, auto which) {
         constexpr int i = decltype(which)::value;
-        if constexpr (i < MT) fa[buf][i] = *(MA_LDS u32x4*)(at + (wm + 32 * i) * L::kStep);
-        else fb[buf][i - MT] = *(MA_LDS u32x4*)(at + (kBM + wn + 32 * (i - MT)) * L::kStep);
+        if constexpr (i < MT) fa[buf][i] = *(MA_LDS u32x4*)(at_c + (wm + 32 * i) * L::kStep);
+        else fb[buf][i - MT] = *(MA_LDS u32x4*)(at_e + (wn + 32 * (i - MT)) * L::kStep);
     };
     f32x16 acc[MT][NT];
     auto clear = [&]() {
@@ -184,15 +180,15 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
 #pragma unroll
             for (int j = 0; j < NT; ++j) acc[i][j] = f32x16(0.f);
     };
-    // The products of a step's 32 bytes on fragments `buf`, with the reads of the next 32's fragments (into the other buffer)
-    // and a share `group` of a later step's loads between them, an instruction or two to each product: a wave has its SIMD
-    // to itself, and what it issues between two products runs in their shadow.
-    auto part = [&](int buf, lds_ptr next, auto group) {
-        constexpr int P = MT * NT, H = P / 2, R = MT + NT, W0 = group_begin(decltype(group)::value), W = group_begin(decltype(group)::value + 1) - W0;
+    // The products of a step's 32 bytes on fragments `buf`, with the reads of the next 32's fragments (into the other
+    // buffer) and runs FIRST .. LAST - 1 of a later step's loads between them, an instruction or two to each product: a
+    // wave has its SIMD to itself, and what it issues between two products runs in their shadow.
+    auto part = [&](int buf, lds_ptr next_c, lds_ptr next_e, auto first, auto last) {
+        constexpr int P = MT * NT, H = P / 2, R = MT + NT, W0 = decltype(first)::value, W = decltype(last)::value - W0;
         static_for<0, P>([&](auto step) {
             constexpr int i = decltype(step)::value;
             // the reads in the first half: what the next part begins with has arrived by then
-            if constexpr (i < H) static_for<i * R / H, (i + 1) * R / H>([&](auto k) { read_one(buf ^ 1, next, k); });
+            if constexpr (i < H) static_for<i * R / H, (i + 1) * R / H>([&](auto k) { read_one(buf ^ 1, next_c, next_e, k); });
             else static_for<W0 + (i - H) * W / (P - H), W0 + (i - H + 1) * W / (P - H)>([&](auto k) { load_run(k); });
             acc[i % MT][i / MT] = Product<T>::mac(fa[buf][i % MT], fb[buf][i / MT], acc[i % MT][i / MT]);
             __builtin_amdgcn_sched_barrier(0);
@@ -287,42 +283,100 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
         }
     };
 
-    // loads that may still be in flight when a step's operands must have landed
-    constexpr int kInFlight = (STAGES - 2) * kRuns;
-    for (int s = 0; s < STAGES - 1; ++s) {
-        load_begin(s);
-        static_for<0, kRuns>([&](auto k) { load_run(k); });
-        load_end();
-    }
-    load_begin(STAGES - 1);
-    static_for<0, group_begin(1)>([&](auto k) { load_run(k); });
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kInFlight + group_begin(1)) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    clear();
-    int stage = 0;
-    constexpr std::integral_constant<bool, false> no{};
-    constexpr std::integral_constant<bool, true> yes{};
-    static_for<0, MT + NT>([&](auto k) { read_one(0, smem + frag[0], k); });
-    for (int tile = 0; tile < tiles; ++tile) {
-        for (int k = 0; k < ksteps; ++k) {
-            const lds_ptr at = smem + stage * L::kStage;
-            static_for<0, L::kSubs - 1>([&](auto s) {
-                constexpr int i = decltype(s)::value;
-                part(i & 1, at + frag[i + 1], std::integral_constant<int, i + 1>{});
-            });
-            load_end();
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kInFlight) : "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            load_begin(stage);
-            stage = stage + 1 == STAGES ? 0 : stage + 1;
-            part(1, smem + stage * L::kStage + frag[0], std::integral_constant<int, 0>{});
-        }
+    const auto close_tile = [&](int tile) {
         const int m0 = v0 + tile * kBM + wm;
-        if (m0 + L::kWaveM > v1) finish_tile(m0, yes);
-        else finish_tile(m0, no);
+        if (m0 + L::kWaveM > v1) finish_tile(m0, std::integral_constant<bool, true>{});
+        else finish_tile(m0, std::integral_constant<bool, false>{});
         clear();
+    };
+    const auto barrier = [] {
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    clear();
+    if constexpr (L::kRing) {
+        // Five slots of one operand's step each, c and e in turn: while step t is computed from two of them, e of step t + 1
+        // and c of step t + 2 arrive in two others and c of step t + 1 has arrived or is about to.  After the barrier of
+        // step t, e of step t + 2 goes where c of step t was and c of step t + 3 where its e was.
+        static_assert(L::kSubs == 4 && L::kARuns == 8 && L::kBRuns == 8, "four parts, four loads each");
+        constexpr int kSlot = kBM * L::kStep;
+        begin(feed[0], 0);
+        static_for<0, 8>([&](auto k) { load_run(k); });
+        advance(feed[0], true);
+        begin(feed[1], kSlot);
+        static_for<8, 16>([&](auto k) { load_run(k); });
+        advance(feed[1], false);
+        begin(feed[0], 2 * kSlot);
+        static_for<0, 8>([&](auto k) { load_run(k); });
+        advance(feed[0], true);
+        begin(feed[1], 3 * kSlot);
+        static_for<8, 12>([&](auto k) { load_run(k); });
+        asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+        barrier();
+        static_for<0, MT + NT>([&](auto k) { read_one(0, smem + frag[0], smem + kSlot + frag[0], k); });
+        int slot = 0;                         // of this step's c; e of it and the units after it follow
+        const auto slot_at = [](int i) { return (i >= 5 ? i - 5 : i) * kSlot; };
+        for (int tile = 0; tile < tiles; ++tile) {
+            for (int k = 0; k < ksteps; ++k) {
+                const lds_ptr c = smem + slot_at(slot), e = smem + slot_at(slot + 1);
+                part(0, c + frag[1], e + frag[1], std::integral_constant<int, 12>{}, std::integral_constant<int, 16>{});
+                advance(feed[1], false);
+                begin(feed[0], slot_at(slot + 4));
+                part(1, c + frag[2], e + frag[2], std::integral_constant<int, 0>{}, std::integral_constant<int, 4>{});
+                part(0, c + frag[3], e + frag[3], std::integral_constant<int, 4>{}, std::integral_constant<int, 8>{});
+                advance(feed[0], true);
+                asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");   // all but c of step t + 2
+                barrier();
+                begin(feed[1], slot_at(slot));
+                slot = slot + 2 >= 5 ? slot - 3 : slot + 2;
+                part(1, smem + slot_at(slot) + frag[0], smem + slot_at(slot + 1) + frag[0], std::integral_constant<int, 8>{},
+                     std::integral_constant<int, 12>{});
+            }
+            close_tile(tile);
+        }
+    } else {
+        // Stages of both operands' step.  A step's loads go out in as many groups as it has parts: the first in the last part
+        // of a step, when its stage has become free, the others in the first parts of the next step.
+        constexpr int kInFlight = (STAGES - 2) * kRuns;      // loads in flight when a step's operands must have landed
+        constexpr auto group = [](int g) constexpr { return g * kRuns / L::kSubs; };
+        const auto begin_both = [&](int stage) {
+            begin(feed[0], stage * L::kStage);
+            begin(feed[1], stage * L::kStage + kBM * L::kStep);
+        };
+        const auto advance_both = [&]() {
+            advance(feed[0], true);
+            advance(feed[1], false);
+        };
+        for (int s = 0; s < STAGES - 1; ++s) {
+            begin_both(s);
+            static_for<0, kRuns>([&](auto k) { load_run(k); });
+            advance_both();
+        }
+        begin_both(STAGES - 1);
+        static_for<0, group(1)>([&](auto k) { load_run(k); });
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kInFlight + group(1)) : "memory");
+        barrier();
+        const auto e_of = [&](lds_ptr c) { return c + kBM * L::kStep; };
+        static_for<0, MT + NT>([&](auto k) { read_one(0, smem + frag[0], e_of(smem + frag[0]), k); });
+        int stage = 0;
+        for (int tile = 0; tile < tiles; ++tile) {
+            for (int k = 0; k < ksteps; ++k) {
+                const lds_ptr at = smem + stage * L::kStage;
+                static_for<0, L::kSubs - 1>([&](auto s) {
+                    constexpr int i = decltype(s)::value;
+                    part(i & 1, at + frag[i + 1], e_of(at + frag[i + 1]), std::integral_constant<int, group(i + 1)>{},
+                         std::integral_constant<int, group(i + 2)>{});
+                });
+                advance_both();
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kInFlight) : "memory");
+                barrier();
+                begin_both(stage);
+                stage = stage + 1 == STAGES ? 0 : stage + 1;
+                const lds_ptr next = smem + stage * L::kStage + frag[0];
+                part(1, next, e_of(next), std::integral_constant<int, 0>{}, std::integral_constant<int, group(1)>{});
+            }
+            close_tile(tile);
+        }
     }
     // the last loads (of steps that do not exist) must not land in LDS that is used again
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
