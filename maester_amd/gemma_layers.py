@@ -8,7 +8,8 @@ layers alternate as ``attn_types`` says; the four sandwich norms run as fused ke
 post-norms with their residual add folded in.  The projections and the MLP stay torch GEMMs.
 ``GemmaTextModel`` puts the token embedding in front and the tied-embedding loss behind
 (model.py:570-769): ``forward(tokens, labels, position_ids, document_ids)`` returns the loss of the
-fused linear + cross-entropy, or the logits without labels.
+fused linear + cross-entropy, or the logits without labels; ``token_logprobs`` returns the labels'
+log-probabilities one by one.
 """
 from __future__ import annotations
 
@@ -20,6 +21,7 @@ from torch import nn
 
 from .gemma_attention import GemmaAttention, GemmaAttentionConfig, StepInputs, build_step_inputs
 from .linear_ce import linear_cross_entropy
+from .linear_logprobs import linear_token_logprobs
 from .rmsnorm import RMSNorm
 
 
@@ -133,11 +135,22 @@ class GemmaTextModel(nn.Module):
         nn.init.normal_(self.tok_embeddings.weight, std=init_std)
         self.model.init_weights(init_std)
 
-    def forward(self, tokens: torch.Tensor, labels: torch.Tensor | None = None, position_ids=None, document_ids=None):
+    def _hidden_states(self, tokens: torch.Tensor, position_ids, document_ids):
         hidden_states = self.tok_embeddings(tokens)
         normalizer = torch.tensor(self.config.dim ** 0.5, dtype=hidden_states.dtype, device=hidden_states.device)
-        hidden_states = self.model(hidden_states * normalizer, position_ids, document_ids)
+        return self.model(hidden_states * normalizer, position_ids, document_ids)
+
+    def forward(self, tokens: torch.Tensor, labels: torch.Tensor | None = None, position_ids=None, document_ids=None):
+        hidden_states = self._hidden_states(tokens, position_ids, document_ids)
         weight = self.tok_embeddings.weight
         if labels is not None:
             return linear_cross_entropy(hidden_states, weight, labels)
         return torch.matmul(hidden_states, weight.t())
+
+    def token_logprobs(self, tokens: torch.Tensor, labels: torch.Tensor, position_ids=None, document_ids=None,
+                       temperature: float = 1.0):
+        """``(logp, entropy)``, fp32 ``[B, S]``: the log-probability of every label (aligned as ``forward`` takes them, -100
+        ignored: 0 there) and the entropy of its position, differentiable, without the logits: what a policy, preference
+        or distillation objective and the scoring of a packed batch start from."""
+        hidden_states = self._hidden_states(tokens, position_ids, document_ids)
+        return linear_token_logprobs(hidden_states, self.tok_embeddings.weight, labels, temperature=temperature)
