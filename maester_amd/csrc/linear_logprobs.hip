@@ -427,31 +427,39 @@ __global__ __launch_bounds__(256) void linear_logprobs_join_kernel(const LinArgs
     if (stats) *(float2*)(stats + 2 * (int64_t)n) = make_float2(t.m, log_l);
 }
 
-int tokens_per_block(int64_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
-
-// Splits of the vocabulary: as many workgroups as the chip has compute units, or as little over a whole multiple of them
-// as there is, ranges a multiple of 32 long so that the few tokens' case, bound by reading c, shares it out evenly.
-void plan(LinArgs& a, int bn, int tiles_whole) {
-    a.row_blocks = (a.rows + bn - 1) / bn;
-    const int cus = 256;
-    int64_t best = INT64_MAX;
+// Tokens per block and splits of the vocabulary.  A tile of 256 x BN takes (us, of 2560 bytes of K and per 1000 rows' run on
+// the full chip) 67, 39, 30, 26 in bf16 and 161, 82, 43, 24 in fp32 for BN = 256, 128, 64, 32: narrow blocks cost more per
+// token, wide ones leave compute units without work or rows without tokens when there are few rows.  The plan is the one
+// with the least of (rounds of 256 workgroups) * (tiles of a range) * (that weight).  Ranges are whole tiles, or for the
+// two narrow blocks, bound by reading c, multiples of 32 so that it is shared out evenly.  Measured at 262208 x 2560 bf16:
+// 48 tokens 248 us in one block of 64 against 309 in two of 32, 384 tokens 549 in three of 128 against 583 in two of 256;
+// at 32003 x 640 fp32, 210 tokens 94 us in two of 128 against 166 in one of 256.
+int plan(LinArgs& a, int dtype) {
+    constexpr int kWidths[4] = {32, 64, 128, 256};
+    constexpr double kWeight[2][4] = {{0.15, 0.27, 0.51, 1.0}, {0.39, 0.45, 0.58, 1.0}};     // MA_DTYPE_F32, MA_DTYPE_BF16
+    constexpr int kUnits = 256;                        // compute units
     const int most = (a.vocab + kBM - 1) / kBM;
-    for (int splits = 1; splits <= most && splits <= cus; ++splits) {
-        int span = (a.vocab + splits - 1) / splits;
-        const int unit = tiles_whole ? kBM : 32;
-        span = (span + unit - 1) / unit * unit;
-        const int64_t rounds = ((int64_t)a.row_blocks * splits + cus - 1) / cus, tiles = (span + kBM - 1) / kBM;
-        const int64_t cost = tiles_whole ? rounds * tiles * kBM : rounds * span;
-        if (cost < best) {
-            best = cost;
-            a.splits = splits;
-            a.span = span;
+    double best = 1e300;
+    int width = 256;
+    for (int w = 0; w < 4; ++w) {
+        const int blocks = (a.rows + kWidths[w] - 1) / kWidths[w], unit = w < 2 ? 32 : kBM;
+        for (int splits = 1; splits <= most && splits <= kUnits; ++splits) {
+            const int span = ((a.vocab + splits - 1) / splits + unit - 1) / unit * unit;
+            const int64_t rounds = ((int64_t)blocks * splits + kUnits - 1) / kUnits;
+            const double cost = (double)rounds * span * kWeight[dtype == MA_DTYPE_BF16][w];
+            if (cost < best) {
+                best = cost;
+                width = kWidths[w];
+                a.row_blocks = blocks;
+                a.span = span;
+            }
         }
     }
     a.splits = (a.vocab + a.span - 1) / a.span;        // none of them empty
+    return width;
 }
 
-LinArgs args_of(const LinearLogprobsArgs& p, int dtype) {
+LinArgs args_of(const LinearLogprobsArgs& p, int dtype, int& width) {
     LinArgs a = {};
     const int elt = dtype == MA_DTYPE_BF16 ? 2 : 4;
     a.e = (const char*)p.e;
@@ -464,7 +472,7 @@ LinArgs args_of(const LinearLogprobsArgs& p, int dtype) {
     a.sh = lp_shape(p.softcap, p.temperature);
     a.targets = p.targets;
     a.ignore_index = p.ignore_index;
-    plan(a, tokens_per_block(p.rows), p.rows > 64);
+    width = plan(a, dtype);
     return a;
 }
 
@@ -478,8 +486,8 @@ int start(const LinArgs& a, hipStream_t st) {
     return check_launch("linear_logprobs_kernel");
 }
 template <typename T, bool CAP, bool GRAD>
-int by_rows(const LinArgs& a, hipStream_t st) {
-    switch (tokens_per_block(a.rows)) {
+int by_width(const LinArgs& a, int width, hipStream_t st) {
+    switch (width) {
         case 32: return start<T, 32, CAP, GRAD>(a, st);
         case 64: return start<T, 64, CAP, GRAD>(a, st);
         case 128: return start<T, 128, CAP, GRAD>(a, st);
@@ -487,9 +495,10 @@ int by_rows(const LinArgs& a, hipStream_t st) {
     }
 }
 template <bool GRAD>
-int by_type(const LinArgs& a, int dtype, hipStream_t st) {
-    if (a.sh.cap > 0.f) return dtype == MA_DTYPE_BF16 ? by_rows<uint16_t, true, GRAD>(a, st) : by_rows<float, true, GRAD>(a, st);
-    return dtype == MA_DTYPE_BF16 ? by_rows<uint16_t, false, GRAD>(a, st) : by_rows<float, false, GRAD>(a, st);
+int by_type(const LinArgs& a, int width, int dtype, hipStream_t st) {
+    const bool bf16 = dtype == MA_DTYPE_BF16;
+    if (a.sh.cap > 0.f) return bf16 ? by_width<uint16_t, true, GRAD>(a, width, st) : by_width<float, true, GRAD>(a, width, st);
+    return bf16 ? by_width<uint16_t, false, GRAD>(a, width, st) : by_width<float, false, GRAD>(a, width, st);
 }
 
 }  // namespace
@@ -502,24 +511,26 @@ size_t linear_logprobs_workspace_bytes(int64_t rows, int64_t vocab) {
 }
 
 int launch_linear_logprobs_fwd(const LinearLogprobsArgs& p, int dtype, hipStream_t st) {
-    LinArgs a = args_of(p, dtype);
+    int width = 0;
+    LinArgs a = args_of(p, dtype, width);
     a.picked = (float*)p.ws;
     a.part = (LpStats*)((char*)p.ws + (((size_t)p.rows * 4 + 15) & ~(size_t)15));
-    const int rc = by_type<false>(a, dtype, st);
+    const int rc = by_type<false>(a, width, dtype, st);
     if (rc) return rc;
     linear_logprobs_join_kernel<<<(unsigned)((p.rows + 3) / 4), 256, 0, st>>>(a, p.logp, p.entropy, p.stats);
     return check_launch("linear_logprobs_join_kernel");
 }
 
 int launch_linear_logprobs_dlogits(const LinearLogprobsArgs& p, int dtype, hipStream_t st) {
-    LinArgs a = args_of(p, dtype);
+    int width = 0;
+    LinArgs a = args_of(p, dtype, width);
     a.stats = p.stats;
     a.entropy = p.entropy;
     a.dlogp = p.dlogp;
     a.dentropy = p.dentropy;
     a.dlogits = p.dlogits;
     a.pitch = p.pitch;
-    return by_type<true>(a, dtype, st);
+    return by_type<true>(a, width, dtype, st);
 }
 
 }  // namespace ma
