@@ -44,8 +44,6 @@ _F32 = frozenset((torch.float32,))
 _E4M3 = frozenset((torch.float8_e4m3fn,))
 _CODE = {torch.bfloat16: _lib.MA_DTYPE_BF16, torch.float32: _lib.MA_DTYPE_F32}
 _dtype, _shape = attrgetter("dtype"), attrgetter("shape")
-# the C struct's layout, for columns filled at once
-_ROW = np.dtype(_lib.MaAdamwTensor)
 
 
 def _device(tensors, who: str) -> torch.device:
@@ -70,8 +68,12 @@ def _addresses(tensors, what: str, shapes: list, dtypes: frozenset, dev: torch.d
     return list(map(torch.Tensor.data_ptr, tensors))
 
 
-def _codes(tensors) -> list:
-    return [_CODE[t.dtype] for t in tensors]
+def _table(n: int, sizes: list, params, grads, **columns) -> np.ndarray:
+    """The C array of ``ma_adamw_tensor``: seven addresses, the size, the two dtypes in one word, a word of the library's."""
+    none = [0] * n
+    names = ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master")
+    codes = [_CODE[p.dtype] | _CODE[g.dtype] << 32 for p, g in zip(params, grads)]
+    return np.array([*(columns.get(k, none) for k in names), sizes, codes, none], dtype=np.uint64).T.copy()
 
 
 def _scalar(t: torch.Tensor, what: str, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
@@ -94,10 +96,8 @@ def global_grad_norm(grads: Sequence[torch.Tensor], max_norm: float | None = Non
     if max_norm is not None and not float(max_norm) >= 0:
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
     dev = _device(grads, "global_grad_norm")
-    table = np.zeros(len(grads), dtype=_ROW)
-    table["grad"] = _addresses(grads, "a gradient", list(map(_shape, grads)), _ACTIVATION, dev)
-    table["n"] = list(map(torch.Tensor.numel, grads))
-    table["grad_dtype"] = _codes(grads)
+    table = _table(len(grads), list(map(torch.Tensor.numel, grads)), grads, grads,
+                   grad=_addresses(grads, "a gradient", list(map(_shape, grads)), _ACTIVATION, dev))
     out = torch.empty(2, dtype=torch.float32, device=dev)
     ws, n = _workspace(len(grads), dev)
     _lib.launch(dev, _lib.lib().ma_grad_norm, table.ctypes.data, len(grads), -1.0 if max_norm is None else float(max_norm),
@@ -137,23 +137,23 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     if eight and len(kinds) > 1:
         raise ValueError("exp_avgs and exp_avg_sqs must all be tensors or all Blocks8")
     shapes, sizes = list(map(_shape, params)), list(map(torch.Tensor.numel, params))
-    table = np.zeros(n, dtype=_ROW)
     where = _addresses(params, "a parameter", shapes, _ACTIVATION, dev)
     if len(set(where)) < n and len({a for a, k in zip(where, sizes) if k}) < sum(map(bool, sizes)):
         raise ValueError("a parameter is listed twice")
-    table["param"], table["param_dtype"], table["n"] = where, _codes(params), sizes
-    table["grad"], table["grad_dtype"] = _addresses(grads, "a gradient", shapes, _ACTIVATION, dev), _codes(grads)
+    columns = dict(param=where, grad=_addresses(grads, "a gradient", shapes, _ACTIVATION, dev))
     for name, states in (("exp_avg", exp_avgs), ("exp_avg_sq", exp_avg_sqs)):
         if eight:
-            table[name] = _addresses([q.codes for q in states], "codes", shapes, _E4M3, dev)
-            table[name + "_scale"] = _addresses([q.scales for q in states], "scales", [(-(-k // BLOCK),) for k in sizes], _F32, dev)
+            columns[name] = _addresses([q.codes for q in states], "codes", shapes, _E4M3, dev)
+            columns[name + "_scale"] = _addresses([q.scales for q in states], "scales", [(-(-k // BLOCK),) for k in sizes], _F32, dev)
         else:
-            table[name] = _addresses(states, name, shapes, _F32, dev)
+            columns[name] = _addresses(states, name, shapes, _F32, dev)
     held = [i for i, w in enumerate(masters) if w is not None]
     if held:
         if any(params[i].dtype != torch.bfloat16 for i in held):
             raise ValueError("a master belongs to a bf16 parameter")
-        table["master"][held] = _addresses([masters[i] for i in held], "a master", [shapes[i] for i in held], _F32, dev)
+        found = iter(_addresses([masters[i] for i in held], "a master", [shapes[i] for i in held], _F32, dev))
+        columns["master"] = [0 if w is None else next(found) for w in masters]
+    table = _table(n, sizes, params, grads, **columns)
     _scalar(step, "step", torch.int64, dev)
     on_device = isinstance(lr, torch.Tensor)
     if on_device:
