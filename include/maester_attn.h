@@ -219,8 +219,9 @@ int ma_token_logprobs_bwd(const void* logits, int64_t pitch, const int64_t* targ
 
 /* The same from hidden states and the classifier, without the logits: x = e c^T for e [rows, dim] and
  * c [vocab, dim] of dtype (rows e_stride / c_stride elements apart, 16-byte aligned rows, dim a multiple
- * of 8 in bf16 and of 4 in fp32), products of the inputs as they are, sums and everything after them in fp32.  Outputs as
- * ma_token_logprobs_fwd's.  workspace: ma_linear_logprobs_workspace_bytes(rows, vocab) bytes, 16-byte aligned.
+ * of 8 in bf16 and of 4 in fp32), products of the inputs as they are, sums and everything after them in
+ * fp32.  Outputs as ma_token_logprobs_fwd's, stats in units of log2 (for ma_linear_logprobs_dlogits only).
+ * workspace: ma_linear_logprobs_workspace_bytes(rows, vocab) bytes, 16-byte aligned.
  * ma_linear_logprobs_dlogits writes d x for the gradients dlogp / dentropy (either may be NULL) into
  * dlogits, rows `pitch` elements apart (a multiple of 8; up to 3 elements of the padding behind a row are
  * written too), in dtype: the caller multiplies it with c and e (library GEMMs), a block of rows at a time. */

@@ -37,7 +37,7 @@ struct LinArgs {
     LpShape sh;
     const int64_t* targets;
     int64_t ignore_index;
-    LpStats* part;                           // forward: [splits, rows]
+    LpStats* part;                           // forward: [splits, rows], in units of log2
     float* picked;                           // forward: [rows], the target's capped logit
     const float *stats, *entropy, *dlogp, *dentropy;   // gradient
     void* dlogits;
@@ -196,6 +196,7 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
     };
 
     // ---- this lane's tokens
+    const float scale = a.sh.inv_temp * kLpLog2e;
     int target[NT];
     LpStats run[NT];
     float ga[NT], gb[NT], top[NT], log_l[NT], ent[NT];
@@ -243,7 +244,7 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
                         // (a target past v1 belongs to the next range's workgroup)
                         if (here && t / 64 == decltype(half)::value && target[j] < v1) a.picked[n0 + wn + 32 * j + r] = x;
                     }
-                    lp_fold2<32>(y, a.sh.inv_temp * kLpLog2e, run[j]);
+                    lp2_fold<32>(y, scale, run[j]);
                     // done here, not where the sums are next needed (which would keep every column's logits in registers)
                     asm volatile("" : "+v"(run[j].m), "+v"(run[j].l), "+v"(run[j].s));
                     __builtin_amdgcn_sched_barrier(0);
@@ -261,9 +262,9 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
                         for (int v = 0; v < 4; ++v) {
                             const float x = acc[i][j][4 * q + v];
                             const float th = CAP ? lp_tanh(x * a.sh.inv_cap) : 0.f;
-                            const float lp = fmaf((CAP ? a.sh.cap * th : x) - top[j], a.sh.inv_temp, -log_l[j]);
-                            const float p = __builtin_amdgcn_exp2f(lp * kLpLog2e);
-                            d[v] = -p * fmaf(gb[j], fmaxf(lp, -1e30f) + ent[j], ga[j]);
+                            const float lp = fmaf(CAP ? a.sh.cap * th : x, scale, -top[j]) - log_l[j];      // log2 p
+                            const float p = __builtin_amdgcn_exp2f(lp);
+                            d[v] = -p * fmaf(gb[j], fmaf(fmaxf(lp, -1e30f), kLpLn2, ent[j]), ga[j]);
                             if (here && 32 * i + 8 * q + v == t) d[v] += ga[j];
                             d[v] *= CAP ? (1.f - th * th) * a.sh.inv_temp : a.sh.inv_temp;
                             if (target[j] < 0) d[v] = 0.f;
@@ -388,8 +389,7 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
     MA_LDS LpStats* box = (MA_LDS LpStats*)smem;       // [kMWaves][BN]
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        run[j].s *= kLpLn2;
-        const LpStats t = lp_merged(run[j], lp_shuffled(run[j], 32), a.sh.inv_temp);
+        const LpStats t = lp2_merged(run[j], lp_shuffled(run[j], 32));
         if (hh == 0) {
             MA_LDS LpStats* at = box + (BN >= 128 ? (w & 1) : w) * BN + wn + 32 * j + r;
             at->m = t.m;
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
 #pragma unroll
         for (int m = 1; m < kMWaves; ++m) {
             MA_LDS LpStats* o = box + m * BN + n;
-            t = lp_merged(t, {o->m, o->l, o->s}, a.sh.inv_temp);
+            t = lp2_merged(t, {o->m, o->l, o->s});
         }
         a.part[(int64_t)split * a.rows + n0 + n] = t;
     }
@@ -415,16 +415,16 @@ __global__ __launch_bounds__(256) void linear_logprobs_join_kernel(const LinArgs
     const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (n >= a.rows) return;
     LpStats t = {-INFINITY, 0.f, 0.f};
-    for (int s = lane; s < a.splits; s += 64) t = lp_merged(t, a.part[(int64_t)s * a.rows + n], a.sh.inv_temp);
+    for (int s = lane; s < a.splits; s += 64) t = lp2_merged(t, a.part[(int64_t)s * a.rows + n]);
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) t = lp_merged(t, lp_shuffled(t, off), a.sh.inv_temp);
+    for (int off = 32; off > 0; off >>= 1) t = lp2_merged(t, lp_shuffled(t, off));
     if (lane) return;
     const int64_t target = a.targets[n];
     const bool valid = target != a.ignore_index && target >= 0 && target < a.vocab;
-    const float log_l = log2f(t.l) * kLpLn2;
-    logp[n] = valid ? (a.picked[n] - t.m) * a.sh.inv_temp - log_l : 0.f;
-    entropy[n] = valid ? log_l - t.s / t.l : 0.f;
-    if (stats) *(float2*)(stats + 2 * (int64_t)n) = make_float2(t.m, log_l);
+    const float log_l = log2f(t.l);
+    logp[n] = valid ? (fmaf(a.picked[n], a.sh.inv_temp * kLpLog2e, -t.m) - log_l) * kLpLn2 : 0.f;
+    entropy[n] = valid ? (log_l - t.s / t.l) * kLpLn2 : 0.f;
+    if (stats) *(float2*)(stats + 2 * (int64_t)n) = make_float2(t.m, log_l);      // both in units of log2
 }
 
 // Tokens per block and splits of the vocabulary.  A tile of 256 x BN takes (us, of 2560 bytes of K and per 1000 rows' run on

@@ -73,15 +73,25 @@ __device__ __forceinline__ void lp_fold(const float* y, float inv_temp, LpStats&
     t.l += one.l;
     t.s += one.s;
 }
-// The same for logits that are sums of products, with s in units of log2 e and scale = log2 e / T: one multiply-add forms
-// the exponent, (y - m) scale = y scale - m scale.  Logits whose product with the scale overflows come out NaN.
+// The same in units of log2 for logits that are sums of products: scale = log2 e / T, m holds the reference max(y) scale
+// as it was rounded, s is sum x 2^x with x = y scale - m, one multiply-add.  All terms have to refer to the very number
+// m: a reference rounded anew at every use would weigh the parts of a row 2^-24 |m| apart, which showed in the entropy
+// (3e-6 relative, ten times an fp32 softmax's).  Logits whose product with the scale overflows come out NaN.
+__device__ __forceinline__ LpStats lp2_merged(const LpStats& a, const LpStats& b) {
+    const float m = fmaxf(a.m, b.m);
+    const float base = m == -INFINITY ? 0.f : m;
+    const float da = fmaxf(a.m - base, -1e30f), db = fmaxf(b.m - base, -1e30f);
+    const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+    return {m, a.l * fa + b.l * fb, fa * (a.s + da * a.l) + fb * (b.s + db * b.l)};
+}
 template <int N>
-__device__ __forceinline__ void lp_fold2(const float* y, float scale, LpStats& t) {
-    float m = t.m;
+__device__ __forceinline__ void lp2_fold(const float* y, float scale, LpStats& t) {
+    float top = y[0];
 #pragma unroll
-    for (int i = 0; i < N; ++i) m = fmaxf(m, y[i]);
-    const float base = m == -INFINITY ? 0.f : m * scale;
-    const float d = fmaxf(fmaf(t.m, scale, -base), -1e30f);
+    for (int i = 1; i < N; ++i) top = fmaxf(top, y[i]);
+    const float m = fmaxf(t.m, top * scale);
+    const float base = m == -INFINITY ? 0.f : m;
+    const float d = fmaxf(t.m - base, -1e30f);
     const float f = __builtin_amdgcn_exp2f(d);
     float l = 0.f, s = 0.f;
 #pragma unroll
