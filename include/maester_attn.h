@@ -203,9 +203,10 @@ int ma_transpose(const void* src, void* dst, int64_t rows, int64_t cols, int src
  *   workspace: at least ma_token_logprobs_workspace_bytes(...) bytes (0 with many rows: then it may be
  *   NULL), 16-byte aligned, where the parts that few rows are cut into leave their results.
  * Logits of -inf have probability 0 (with a soft cap they are -softcap).  A row with a NaN or +inf (with
- * a soft cap: a NaN), or with nothing but -inf, has NaN outputs.  ma_token_logprobs_bwd: dlogits (rows `dpitch` apart, may alias logits) =
- *   dlogp * d logp + dentropy * d entropy, zeros for a row that does not count; either of dlogp /
- *   dentropy (fp32 [rows]) may be NULL (= 0); stats and entropy as the forward wrote them. */
+ * a soft cap: a NaN), or with nothing but -inf, has NaN outputs.
+ * ma_token_logprobs_bwd: dlogits = dlogp * d logp + dentropy * d entropy (rows `dpitch` apart; may be
+ * logits itself with its pitch), zeros for a row that does not count; either of dlogp / dentropy (fp32
+ * [rows]) may be NULL (= 0); stats and entropy as the forward wrote them. */
 #define MA_LOGPROBS_MAX_TOP 64
 #define MA_LOGPROBS_MAX_VOCAB ((1 << 30) - 1)
 size_t ma_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_k);

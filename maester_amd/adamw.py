@@ -138,8 +138,6 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         raise ValueError("exp_avgs and exp_avg_sqs must all be tensors or all Blocks8")
     shapes, sizes = list(map(_shape, params)), list(map(torch.Tensor.numel, params))
     where = _addresses(params, "a parameter", shapes, _ACTIVATION, dev)
-    if len(set(where)) < n and len({a for a, k in zip(where, sizes) if k}) < sum(map(bool, sizes)):
-        raise ValueError("a parameter is listed twice")
     columns = dict(param=where, grad=_addresses(grads, "a gradient", shapes, _ACTIVATION, dev))
     for name, states in (("exp_avg", exp_avgs), ("exp_avg_sq", exp_avg_sqs)):
         if eight:
@@ -153,6 +151,11 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
             raise ValueError("a master belongs to a bf16 parameter")
         found = iter(_addresses([masters[i] for i in held], "a master", [shapes[i] for i in held], _F32, dev))
         columns["master"] = [0 if w is None else next(found) for w in masters]
+    # a tensor that two entries would write is a race
+    written = [columns[k] for k in ("param", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master") if k in columns]
+    addresses = [a for column in written for a, k in zip(column, sizes) if k and a]
+    if len(set(addresses)) < len(addresses):
+        raise ValueError("a parameter, state or master is listed twice")
     table = _table(n, sizes, params, grads, **columns)
     _scalar(step, "step", torch.int64, dev)
     on_device = isinstance(lr, torch.Tensor)
@@ -242,11 +245,22 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict: dict) -> None:
-        """Restores the states in the types they were saved in (torch's own would cast them to the parameter's)."""
+        """Restores the states in the types they were saved in (torch's own would cast them to the parameter's).  A state of
+        ``torch.optim.AdamW`` is taken over into 32-bit states; its per-parameter counters become the group's, the largest
+        of them."""
         super().load_state_dict(state_dict)
         saved = state_dict["state"]
-        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
-        params = [p for group in self.param_groups for p in group["params"]]
-        for i, p in zip(ids, params):
-            if i in saved:
-                self.state[p] = {k: t.detach().to(p.device, copy=True) for k, t in saved[i].items()}
+        for old, group in zip(state_dict["param_groups"], self.param_groups):
+            foreign = "state_bits" not in old
+            if foreign:
+                group.update(state_bits=32, master_weights=self.defaults["master_weights"], seed=self.defaults["seed"])
+                group["step"] = max((int(saved[i]["step"]) for i in old["params"] if i in saved), default=0)
+            for i, p in zip(old["params"], group["params"]):
+                if i not in saved:
+                    continue
+                if not foreign:
+                    self.state[p] = {k: t.detach().to(p.device, copy=True) for k, t in saved[i].items()}
+                    continue
+                self.state[p] = self._init_state(p, group)
+                for k in ("exp_avg", "exp_avg_sq"):
+                    self.state[p][k].copy_(saved[i][k])

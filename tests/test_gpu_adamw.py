@@ -279,6 +279,47 @@ def test_state_dict_continues_bit_for_bit(gpu, state_bits, master):
             assert t.dtype == u.dtype and torch.equal(t.view(torch.uint8), u.view(torch.uint8)), k
 
 
+def test_takes_over_a_state_of_torchs(gpu):
+    a = _net(gpu)
+    theirs = torch.optim.AdamW(a.parameters(), lr=5e-3, foreach=False)
+
+    def train(net, o, seeds):
+        for s in seeds:
+            x = torch.randn(8, 33, device=gpu, generator=torch.Generator(device=gpu).manual_seed(s))
+            o.zero_grad()
+            net(x).square().mean().backward()
+            o.step()
+
+    train(a, theirs, range(3))
+    b = copy.deepcopy(a)
+    ours = AdamW(b.parameters(), lr=1.0)
+    ours.load_state_dict(theirs.state_dict())
+    assert int(ours.param_groups[0]["step"]) == 3 and ours.param_groups[0]["lr"] == 5e-3
+    train(a, theirs, [3])
+    train(b, ours, [3])
+    assert all(torch.allclose(p, q, rtol=1e-5, atol=1e-6) for p, q in zip(a.parameters(), b.parameters()))
+
+
+def test_beyond_32_bits_of_offset(gpu):
+    # 2^31 + 5 bf16 weights with fp32 states: the last elements as a tensor of their own gets them
+    n, tail = (1 << 31) + 5, 4101
+    p = torch.full((n,), 0.5, dtype=torch.bfloat16, device=gpu)
+    grad = torch.zeros(n, dtype=torch.bfloat16, device=gpu)
+    m, v = torch.zeros(n, device=gpu), torch.zeros(n, device=gpu)
+    g = torch.Generator().manual_seed(1)
+    p[-tail:] = torch.randn(tail, generator=g).to(gpu)
+    grad[-tail:] = torch.randn(tail, generator=g).to(gpu)
+    q, h = p[-tail:].clone(), grad[-tail:].clone()
+    mq, vq = torch.zeros(tail, device=gpu), torch.zeros(tail, device=gpu)
+    for args in ((p, grad, m, v), (q, h, mq, vq)):
+        step = torch.zeros((), dtype=torch.int64, device=gpu)
+        norm = adamw_step(*([t] for t in args), step, **HYPER, max_grad_norm=1.0)
+    assert abs(float(norm) - float(h.double().norm())) <= 1e-5 * float(norm)
+    # (the norms of both calls are the same number up to the order of an fp64 sum)
+    assert torch.allclose(m[-tail:], mq, rtol=1e-6, atol=0) and torch.allclose(p[-tail:].float(), q.float(), rtol=2 ** -8, atol=0)
+    assert float(m[:-tail].abs().max()) == 0 and torch.all(p[:4096] == p[0])
+
+
 def test_optimizer_corners(gpu):
     a = _net(gpu)
     opt = AdamW(a.parameters())
@@ -355,7 +396,9 @@ def test_refusals(gpu):
                     (dict(exp_avgs=[m.bfloat16()]), TypeError), (dict(exp_avgs=[b8]), ValueError),
                     (dict(exp_avgs=[b8], exp_avg_sqs=[Blocks8(b8.codes, b8.scales[:1])]), ValueError),
                     (dict(step=step.int()), ValueError), (dict(step=step.cpu()), ValueError), (dict(masters=[m]), ValueError),
-                    (dict(params=[p, p], grads=[g, g], exp_avgs=[m, m], exp_avg_sqs=[v, v]), ValueError),
+                    (dict(params=[p, p], grads=[g, g], exp_avgs=[m, m.clone()], exp_avg_sqs=[v, v.clone()]), ValueError),
+                    (dict(params=[p, p.clone()], grads=[g, g], exp_avgs=[m, m], exp_avg_sqs=[v, v.clone()]), ValueError),
+                    (dict(exp_avg_sqs=[m]), ValueError),
                     (dict(lr=torch.zeros((), dtype=torch.float64, device=gpu)), ValueError), (dict(seed=-1), ValueError),
                     (dict(max_grad_norm=-1.0), ValueError), (dict(max_grad_norm=1.0, clip=m[0]), ValueError),
                     (dict(params=[p.cpu()]), RuntimeError), (dict(params=[], grads=[], exp_avgs=[], exp_avg_sqs=[]), ValueError)]:

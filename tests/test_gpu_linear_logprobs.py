@@ -82,6 +82,22 @@ def test_full_vocabulary(gpu, n):
     assert float((logp - want.logp).abs().max()) <= 1e-4 and float((entropy - want.entropy).abs().max()) <= 2e-3
 
 
+def test_beyond_32_bits_of_offset(gpu):
+    # a classifier of 4.9 GB: log-probabilities of its last entries against a product taken a slice at a time
+    vocab, k, n = 300_000, 8192, 40
+    c = torch.zeros(vocab, k, dtype=torch.bfloat16, device=gpu)
+    g = torch.Generator(device=gpu).manual_seed(0)
+    for r in range(0, vocab, 50_000):
+        c[r:r + 50_000] = torch.randn(50_000, k, generator=g, device=gpu) * (3 / k ** 0.5)
+    e = torch.randn(n, k, generator=g, device=gpu).bfloat16()
+    t = torch.arange(vocab - n, vocab, device=gpu)
+    logp, entropy = linear_token_logprobs(e, c, t)
+    x = torch.cat([e.float() @ c[r:r + 50_000].float().t() for r in range(0, vocab, 50_000)], 1)
+    want = torch.log_softmax(x.double(), 1)
+    assert float((logp - want[torch.arange(n), t]).abs().max()) <= 1e-4
+    assert float((entropy + (want.exp() * want).sum(1)).abs().max()) <= 1e-3
+
+
 def test_every_target_is_found(gpu):
     # all vocabulary entries as targets once: logp is the log-softmax row by row
     vocab, k = 1111, 64

@@ -272,6 +272,44 @@ def test_refusals(gpu):
         token_logprobs(x.cpu(), t.cpu())
 
 
+def test_beyond_32_bits_of_offset(gpu):
+    # 8300 x 262208 bf16 is 2^31 elements and more: its last rows as a batch of their own
+    rows, vocab = 8300, 262208
+    x = torch.zeros(rows, vocab, dtype=torch.bfloat16, device=gpu)
+    t = torch.randint(0, vocab, (rows,), device=gpu)
+    x[-3:].normal_()
+    x[-3:] *= 3
+    a = torch.ones(rows, device=gpu)
+    whole = x.requires_grad_()
+    out = token_logprobs(whole, t, top_k=4)
+    d, = torch.autograd.grad((out.logp, out.entropy), whole, (a, a))
+    part = x[-3:].detach().clone().requires_grad_()
+    want = token_logprobs(part, t[-3:], top_k=4)
+    e, = torch.autograd.grad((want.logp, want.entropy), part, (a[-3:], a[-3:]))
+    # (few rows are cut into parts: another order of the sums)
+    c = rel_of_sums(vocab)
+    assert float((out.logp[-3:] - want.logp).abs().max()) <= 2 * c and float((out.entropy[-3:] - want.entropy).abs().max()) <= 50 * c
+    assert torch.equal(out.top_ids[-3:], want.top_ids)
+    assert float((d[-3:].float() - e.float()).abs().max()) <= 2 * 2.0 ** -8 * float(e.abs().max())
+    assert abs(float(out.logp[0]) + np.log(vocab)) <= 2 * c * 13
+
+
+def test_gradient_in_place_of_the_logits(gpu):
+    # the C entry point may write the gradient over the logits themselves
+    from maester_amd import _lib
+    from maester_amd.token_logprobs import token_logprobs_backward, token_logprobs_forward
+    for vocab in (1003, 4096):
+        x, t = make(9, vocab, torch.bfloat16, vocab)
+        xg, tg = x.to(gpu), t.to(gpu)
+        a = torch.randn(9, device=gpu)
+        _, entropy, stats, _, _ = token_logprobs_forward(xg, tg)
+        want = token_logprobs_backward(xg, tg, stats, entropy, a, a)
+        rc = _lib.lib().ma_token_logprobs_bwd(xg.data_ptr(), vocab, tg.data_ptr(), 9, vocab, -100, 0.0, 1.0, stats.data_ptr(), entropy.data_ptr(),
+                                              a.data_ptr(), a.data_ptr(), xg.data_ptr(), vocab, _lib.MA_DTYPE_BF16, _lib.current_stream(xg.device))
+        _lib.check(rc)
+        assert torch.equal(xg, want)
+
+
 def test_other_stream_and_graph_replay(gpu):
     x, t = make(33, 30011, torch.bfloat16, 8)
     xg, tg = x.to(gpu), t.to(gpu)
