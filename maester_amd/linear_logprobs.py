@@ -91,16 +91,18 @@ def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentrop
     mixed = {"out_dtype": torch.float32} if e.dtype != torch.float32 else {}
     dc = None
     for r0 in range(0, n, step):
-        rows = slice(r0, min(n, r0 + step))
+        whole, rows = n <= step, slice(r0, min(n, r0 + step))
         buf = block[: rows.stop - r0]
-        _dlogits(e[rows], c, targets[rows], stats[rows], entropy[rows], None if dlogp is None else dlogp[rows],
-                 None if dentropy is None else dentropy[rows], ignore_index, softcap, temperature, buf)
+        e_rows, rest = e, (targets, stats, entropy, dlogp, dentropy)
+        if not whole:
+            e_rows, rest = e[rows], (None if t is None else t[rows] for t in rest)
+        _dlogits(e_rows, c, *rest, ignore_index, softcap, temperature, buf)
         x = buf[:, :vocab]
         if need_de:
-            torch.mm(x, c if c_t is None else c_t.t(), out=de[rows])
+            torch.mm(x, c if c_t is None else c_t.t(), out=de if whole else de[rows])
         if need_dc:
-            hidden = e[rows] if buf.shape[0] < _TRANSPOSE_E_FROM else transpose(e[rows].contiguous()).t()
-            if n <= step:
+            hidden = e_rows if buf.shape[0] < _TRANSPOSE_E_FROM else transpose(e_rows.contiguous()).t()
+            if whole:
                 dc = torch.mm(x.t(), hidden)
             elif dc is None:                     # several blocks: summed in fp32, rounded once at the end
                 dc = torch.mm(x.t(), hidden, **mixed)
@@ -109,8 +111,10 @@ def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentrop
     return de, dc.to(c.dtype) if need_dc else None
 
 
-# rows that a call has to have before ignored ones are dropped: up to here they fill one block of the kernel's anyway
-_FILTER_FROM = 257
+# Ignored rows are dropped from 257 rows on (up to 256 fill one block of the kernel's anyway) and from products of 2^36
+# multiply-adds on: finding and gathering the others costs some 100 us with the wait (300 rows x 888 x 2064, forward and
+# gradients: 283 us with, 140 without), a third of four such products as much.
+_FILTER_FROM, _FILTER_WORK = 257, 1 << 36
 
 
 def _kept_rows(targets, ignore_index, vocab):
@@ -159,8 +163,9 @@ def linear_token_logprobs(e: torch.Tensor, c: torch.Tensor, targets: torch.Tenso
     ``e`` ``[..., K]`` hidden states, ``c`` ``[V, K]`` classifier (Gemma: the tied embedding table), bf16 or fp32 alike,
     ``K`` a multiple of 8 (fp32: 4); the logits are products of the inputs summed in fp32 and never stored.  ``softcap``,
     ``temperature`` and ignored targets as in ``token_logprobs``.  ``chunk_rows``: rows per block of the backward (default:
-    about 4 GiB of gradient of the logits at a time).  ``filter_ignored``: a call of more than 256 rows drops those whose
-    target does not count before any product, which costs its one host synchronisation; not under graph capture."""
+    about 4 GiB of gradient of the logits at a time).  ``filter_ignored``: a large call (more than 256 rows, 2^36
+    multiply-adds a product) drops the rows whose target does not count before any product, which costs its one host
+    synchronisation; not under graph capture."""
     if e.dim() < 1 or targets.shape != e.shape[:-1]:
         raise ValueError(f"targets shape {tuple(targets.shape)} != leading shape of e {tuple(e.shape[:-1])}")
     lead = targets.shape
@@ -168,7 +173,7 @@ def linear_token_logprobs(e: torch.Tensor, c: torch.Tensor, targets: torch.Tenso
         e, targets = e.reshape(targets.numel(), e.shape[-1]), targets.reshape(-1)
     _check(e, c, targets)
     keep = None
-    if filter_ignored and e.shape[0] >= _FILTER_FROM and not torch.cuda.is_current_stream_capturing():
+    if filter_ignored and e.shape[0] >= _FILTER_FROM and e.numel() * c.shape[0] >= _FILTER_WORK and not torch.cuda.is_current_stream_capturing():
         keep = _kept_rows(targets, ignore_index, c.shape[0])
     if torch.is_grad_enabled() and (e.requires_grad or c.requires_grad):
         logp, entropy = _LinearTokenLogprobsFn.apply(e, c, targets, int(ignore_index), softcap, temperature, chunk_rows, keep)
