@@ -112,9 +112,9 @@ def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentrop
 
 
 # Ignored rows are dropped from 257 rows on (up to 256 fill one block of the kernel's anyway) and from products of 2^36
-# multiply-adds on: finding and gathering the others costs some 100 us with the wait (300 rows x 888 x 2064, forward and
+# multiply-adds (fp32: 2^33) on: finding and gathering the others costs some 100 us with the wait (300 rows x 888 x 2064, forward and
 # gradients: 283 us with, 140 without), a third of four such products as much.
-_FILTER_FROM, _FILTER_WORK = 257, 1 << 36
+_FILTER_FROM, _FILTER_WORK = 257, {torch.bfloat16: 1 << 36, torch.float32: 1 << 33}
 
 
 def _kept_rows(targets, ignore_index, vocab):
@@ -173,7 +173,7 @@ def linear_token_logprobs(e: torch.Tensor, c: torch.Tensor, targets: torch.Tenso
         e, targets = e.reshape(targets.numel(), e.shape[-1]), targets.reshape(-1)
     _check(e, c, targets)
     keep = None
-    if filter_ignored and e.shape[0] >= _FILTER_FROM and e.numel() * c.shape[0] >= _FILTER_WORK and not torch.cuda.is_current_stream_capturing():
+    if filter_ignored and e.shape[0] >= _FILTER_FROM and e.numel() * c.shape[0] >= _FILTER_WORK[e.dtype] and not torch.cuda.is_current_stream_capturing():
         keep = _kept_rows(targets, ignore_index, c.shape[0])
     if torch.is_grad_enabled() and (e.requires_grad or c.requires_grad):
         logp, entropy = _LinearTokenLogprobsFn.apply(e, c, targets, int(ignore_index), softcap, temperature, chunk_rows, keep)

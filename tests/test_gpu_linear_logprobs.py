@@ -220,7 +220,7 @@ def test_same_bits_every_time_other_stream_and_graph(gpu):
 @pytest.mark.parametrize("n,ignore", [(256, 0.5), (257, 0.5), (900, 0.9), (400, 1.0), (300, 0.0)])
 def test_dropped_rows_change_nothing(gpu, n, ignore, monkeypatch):
     from maester_amd import linear_logprobs
-    monkeypatch.setattr(linear_logprobs, "_FILTER_WORK", 0)   # also where it would not pay
+    monkeypatch.setitem(linear_logprobs._FILTER_WORK, torch.bfloat16, 0)   # also where it would not pay
     e, c, t = problem(n, 64, 1003, torch.bfloat16, n, ignore=ignore)
     t[0] = -100 if ignore == 1.0 else 5
     if n == 900:
