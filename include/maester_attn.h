@@ -209,6 +209,7 @@ int ma_transpose(const void* src, void* dst, int64_t rows, int64_t cols, int src
  * [rows]) may be NULL (= 0); stats and entropy as the forward wrote them. */
 #define MA_LOGPROBS_MAX_TOP 64
 #define MA_LOGPROBS_MAX_VOCAB ((1 << 30) - 1)
+#define MA_LOGPROBS_MAX_GRAD_VOCAB (1 << 21) /* ma_linear_grads */
 size_t ma_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_k);
 int ma_token_logprobs_fwd(const void* logits, int64_t pitch, const int64_t* targets, int64_t rows, int64_t vocab,
                           int64_t ignore_index, float softcap, float temperature, int top_k, float* logp, float* entropy,
@@ -224,8 +225,12 @@ int ma_token_logprobs_bwd(const void* logits, int64_t pitch, const int64_t* targ
  * fp32.  Outputs as ma_token_logprobs_fwd's, stats in units of log2 (for ma_linear_logprobs_dlogits only).
  * workspace: ma_linear_logprobs_workspace_bytes(rows, vocab) bytes, 16-byte aligned.
  * ma_linear_logprobs_dlogits writes d x for the gradients dlogp / dentropy (either may be NULL) into
- * dlogits, rows `pitch` elements apart (a multiple of 8; up to 3 elements of the padding behind a row are
- * written too), in dtype: the caller multiplies it with c and e (library GEMMs), a block of rows at a time. */
+ * dlogits, rows `pitch` elements apart (a multiple of 8; the padding behind a row up to the next multiple
+ * of 8 is written too, with zeros), in dtype, a block of rows at a time, for
+ * ma_linear_grads: de [rows, dim] = x c and dc [vocab, dim] = x^T e of x = dlogits, contiguous, either may be
+ * NULL (and c or e with it), come in dtype, rounded once; with dc_added dc is fp32 and added to (several
+ * blocks of rows).  x is read up to the next multiple of 8 (fp32: 4) columns: the padding has to hold zeros.  workspace: ma_linear_grads_workspace_bytes(...)
+ * bytes (0: may be NULL), 16-byte aligned.  Sums in a fixed order. */
 size_t ma_linear_logprobs_workspace_bytes(int64_t rows, int64_t vocab);
 int ma_linear_logprobs_fwd(const void* e, int64_t e_stride, const void* c, int64_t c_stride, const int64_t* targets, int64_t rows,
                            int64_t vocab, int64_t dim, int64_t ignore_index, float softcap, float temperature, float* logp,
@@ -234,6 +239,11 @@ int ma_linear_logprobs_dlogits(const void* e, int64_t e_stride, const void* c, i
                                int64_t vocab, int64_t dim, int64_t ignore_index, float softcap, float temperature, const float* stats,
                                const float* entropy, const float* dlogp, const float* dentropy, void* dlogits, int64_t pitch,
                                int dtype, void* stream);
+
+size_t ma_linear_grads_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, int dtype);
+int ma_linear_grads(const void* x, int64_t x_stride, const void* e, int64_t e_stride, const void* c, int64_t c_stride, int64_t rows,
+                    int64_t vocab, int64_t dim, void* de, void* dc, int dc_added, void* workspace, size_t workspace_bytes, int dtype,
+                    void* stream);
 
 /* ---- AdamW over many tensors ---------------------------------------------------------------------------
  * The step that applies a training step's gradients: AdamW with decoupled weight decay over any number

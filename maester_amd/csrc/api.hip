@@ -332,6 +332,37 @@ int ma_linear_logprobs_dlogits(const void* e, int64_t e_stride, const void* c, i
     return launch_linear_logprobs_dlogits(a, dtype, (hipStream_t)stream);
 }
 
+size_t ma_linear_grads_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, int dtype) {
+    if (rows <= 0 || vocab <= 0 || dim <= 0 || (dtype != MA_DTYPE_F32 && dtype != MA_DTYPE_BF16)) return 0;
+    return linear_grads_workspace_bytes(rows, vocab, dim, dtype);
+}
+
+int ma_linear_grads(const void* x, int64_t x_stride, const void* e, int64_t e_stride, const void* c, int64_t c_stride, int64_t rows,
+                    int64_t vocab, int64_t dim, void* de, void* dc, int dc_added, void* workspace, size_t workspace_bytes, int dtype,
+                    void* stream) {
+    const char* who = "ma_linear_grads";
+    MA_TRY(check_dtype(who, dtype));
+    const int64_t al = dtype == MA_DTYPE_BF16 ? 8 : 4;
+    if (!x || (de && !c) || (dc && !e)) return fail(MA_ERR_BAD_ARG, "%s: x / c / e is NULL", who);
+    if (!de && !dc) return fail(MA_ERR_BAD_ARG, "%s: both outputs are NULL", who);
+    if ((((uintptr_t)x | (uintptr_t)e | (uintptr_t)c | (uintptr_t)de | (uintptr_t)dc) & 15) != 0)
+        return fail(MA_ERR_BAD_ARG, "%s: x / e / c / de / dc not 16-byte aligned", who);
+    if (rows <= 0 || rows > ((int64_t)1 << 26)) return fail(MA_ERR_BAD_ARG, "%s: rows=%lld must be in 1 .. 2^26", who, (long long)rows);
+    if (vocab <= 0 || vocab > MA_LOGPROBS_MAX_VOCAB) return fail(MA_ERR_BAD_ARG, "%s: vocab=%lld out of range", who, (long long)vocab);
+    if (dim <= 0 || dim % al != 0 || dim > 65536)
+        return fail(MA_ERR_UNSUPPORTED, "%s: dim=%lld must be a multiple of %lld, at most 65536", who, (long long)dim, (long long)al);
+    if (x_stride < (vocab + al - 1) / al * al || x_stride % al || (de && (c_stride < dim || c_stride % al)) || (dc && (e_stride < dim || e_stride % al)))
+        return fail(MA_ERR_BAD_ARG, "%s: row strides must be multiples of %lld elements, at least the row's length rounded up to one", who, (long long)al);
+    // the rows of a tile (256 of x, 64 of e and c, 256 of the results) are addressed with 31-bit byte offsets
+    if (x_stride > MA_LOGPROBS_MAX_GRAD_VOCAB || (de && c_stride > (1 << 20)) || (dc && e_stride > (1 << 20)))
+        return fail(MA_ERR_UNSUPPORTED, "%s: row strides above 2^21 (x), 2^20 (e, c) elements", who);
+    const size_t need = de ? linear_grads_workspace_bytes(rows, vocab, dim, dtype) : 0;
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0))
+        return fail(MA_ERR_BAD_ARG, "%s: workspace of %zu bytes, need %zu, 16-byte aligned", who, workspace ? workspace_bytes : (size_t)0, need);
+    const LinearGradsArgs a = {x, e, c, x_stride, e_stride, c_stride, rows, vocab, dim, de, dc, dc_added, workspace};
+    return launch_linear_grads(a, dtype, (hipStream_t)stream);
+}
+
 size_t ma_adamw_workspace_bytes(int count) { return count < 0 ? 0 : adamw_workspace_bytes(count); }
 
 static int check_adamw(const char* who, const ma_adamw_tensor* tensors, int count, int state_bits, double max_norm, const void* workspace,

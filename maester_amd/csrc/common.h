@@ -95,6 +95,16 @@ size_t linear_logprobs_workspace_bytes(int64_t rows, int64_t vocab);
 int launch_linear_logprobs_fwd(const LinearLogprobsArgs& a, int dtype, hipStream_t st);
 int launch_linear_logprobs_dlogits(const LinearLogprobsArgs& a, int dtype, hipStream_t st);
 
+struct LinearGradsArgs {
+    const void *x, *e, *c;            // x: gradient of the logits
+    int64_t x_stride, e_stride, c_stride, rows, vocab, dim;
+    void *de, *dc;                    // either may be NULL
+    int dc_added;                     // dc is fp32 and added to; otherwise it has the operands' type
+    void* ws;
+};
+size_t linear_grads_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, int dtype);
+int launch_linear_grads(const LinearGradsArgs& a, int dtype, hipStream_t st);
+
 struct AdamwArgs {
     const ma_adamw_tensor* list;      // host memory
     int count, state_bits, want_norm;

@@ -268,8 +268,10 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
                             if (here && 32 * i + 8 * q + v == t) d[v] += ga[j];
                             d[v] *= CAP ? (1.f - th * th) * a.sh.inv_temp : a.sh.inv_temp;
                             if (target[j] < 0) d[v] = 0.f;
+                            if (PARTIAL && m + v >= a.vocab) d[v] = 0.f;
                         }
-                        if (n < a.rows && m < v1) {     // up to three columns past the vocabulary lie in the row's padding
+                        // (the row's padding up to the next eight columns is written too, zeros: the products that follow read it)
+                        if (n < a.rows && (!PARTIAL || m < (v1 == a.vocab ? (v1 + 7) & ~7 : v1))) {
                             if constexpr (sizeof(T) == 2) {
                                 bf16x4 o;
 #pragma unroll

@@ -3,15 +3,15 @@
 ``token_logprobs`` of ``e @ c.T`` in one matrix-core kernel whose epilogue keeps the softmax statistics of every token: the
 ``[tokens, vocab]`` matrix never exists and its entries stay in fp32 (``linear_cross_entropy`` rounds a block of them to the
 activation dtype between its GEMM and its softmax kernel).  The backward forms the gradient of the logits a block of rows
-at a time, from the statistics that the forward kept, in the activation dtype, and leaves the two products with the
-classifier and the hidden states to the library's GEMMs, as ``linear_cross_entropy`` does.
+at a time, from the statistics that the forward kept, in the activation dtype, and multiplies it with the classifier and
+the hidden states in matrix-core kernels that read both as they lie in memory.
 """
 from __future__ import annotations
 
 import torch
 
 from . import _lib
-from .linear_ce import default_chunk_rows, transpose
+from .linear_ce import default_chunk_rows
 from .token_logprobs import check_softmax_arguments
 
 
@@ -66,11 +66,17 @@ def _dlogits(e, c, targets, stats, entropy, dlogp, dentropy, ignore_index, softc
                 _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.ptr(out), out.shape[1], _lib.dtype_code(e.dtype))
 
 
-# The library's operand orders for the two gradient products, by rows (262208 x 2560 bf16, ms):
-#   de = x c with c as it is 1.5 / 2.9 / 3.5 / 6.0 / 13.3 at 512 / 1433 / 2047 / 4096 / 8192 rows, with c transposed first
-#   2.0 / 3.3 / 3.3 / 4.7 / 8.9;  dc = x^T e with e as it is 0.9 / 2.0 / 2.7 / 4.9 / 9.7, with e transposed 1.0 / 2.1 /
-#   2.8 / 4.2 / 8.2.
-_TRANSPOSE_C_FROM, _TRANSPOSE_E_FROM = 2000, 3000
+MAX_GRAD_VOCAB = 1 << 21                    # ma_linear_grads addresses 256 rows of the logits' gradient with 31 bits
+
+
+def _products(x, e, c, de, dc, add):
+    """``de = x c`` and ``dc = x^T e`` (``add``: added to an fp32 ``dc``), either may be None; the rows of ``x`` are padded."""
+    L, code = _lib.lib(), _lib.dtype_code(e.dtype)
+    ws_bytes = 0 if de is None else L.ma_linear_grads_workspace_bytes(e.shape[0], c.shape[0], e.shape[1], code)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=e.device) if ws_bytes else None
+    _lib.launch(e.device, L.ma_linear_grads, x.data_ptr(), x.shape[1], e.data_ptr(), _pitch(e), c.data_ptr(), _pitch(c), e.shape[0],
+                c.shape[0], e.shape[1], _lib.ptr(de), _lib.ptr(dc), int(add), _lib.ptr(ws), ws_bytes,
+                code)
 
 
 def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentropy, ignore_index=-100, softcap=None,
@@ -87,9 +93,10 @@ def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentrop
     step = int(chunk_rows) if chunk_rows else default_chunk_rows(vocab, e.element_size(), n)
     step = max(1, min(step, n))
     block = torch.empty(step, -(-vocab // 8) * 8, dtype=e.dtype, device=e.device)
-    c_t = transpose(c.contiguous()) if need_de and n >= _TRANSPOSE_C_FROM else None
-    mixed = {"out_dtype": torch.float32} if e.dtype != torch.float32 else {}
+    # several blocks: dc is summed in fp32 and rounded once at the end
     dc = None
+    if need_dc:
+        dc = torch.empty(vocab, k, dtype=c.dtype, device=c.device) if n <= step else torch.zeros(vocab, k, device=c.device)
     for r0 in range(0, n, step):
         whole, rows = n <= step, slice(r0, min(n, r0 + step))
         buf = block[: rows.stop - r0]
@@ -97,17 +104,8 @@ def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentrop
         if not whole:
             e_rows, rest = e[rows], (None if t is None else t[rows] for t in rest)
         _dlogits(e_rows, c, *rest, ignore_index, softcap, temperature, buf)
-        x = buf[:, :vocab]
-        if need_de:
-            torch.mm(x, c if c_t is None else c_t.t(), out=de if whole else de[rows])
-        if need_dc:
-            hidden = e_rows if buf.shape[0] < _TRANSPOSE_E_FROM else transpose(e_rows.contiguous()).t()
-            if whole:
-                dc = torch.mm(x.t(), hidden)
-            elif dc is None:                     # several blocks: summed in fp32, rounded once at the end
-                dc = torch.mm(x.t(), hidden, **mixed)
-            else:
-                torch.addmm(dc, x.t(), hidden, out=dc, **mixed)
+        if need_de or need_dc:
+            _products(buf, e_rows, c, de if whole or de is None else de[rows], dc, not whole)
     return de, dc.to(c.dtype) if need_dc else None
 
 
@@ -163,7 +161,7 @@ def linear_token_logprobs(e: torch.Tensor, c: torch.Tensor, targets: torch.Tenso
     ``e`` ``[..., K]`` hidden states, ``c`` ``[V, K]`` classifier (Gemma: the tied embedding table), bf16 or fp32 alike,
     ``K`` a multiple of 8 (fp32: 4); the logits are products of the inputs summed in fp32 and never stored.  ``softcap``,
     ``temperature`` and ignored targets as in ``token_logprobs``.  ``chunk_rows``: rows per block of the backward (default:
-    about 4 GiB of gradient of the logits at a time).  ``filter_ignored``: a large call (more than 256 rows, 2^36
+    about 4 GiB of gradient of the logits at a time; V is at most 2^21 with gradients).  ``filter_ignored``: a large call (more than 256 rows, 2^36
     multiply-adds a product) drops the rows whose target does not count before any product, which costs its one host
     synchronisation; not under graph capture."""
     if e.dim() < 1 or targets.shape != e.shape[:-1]:
@@ -172,6 +170,8 @@ def linear_token_logprobs(e: torch.Tensor, c: torch.Tensor, targets: torch.Tenso
     if len(lead) != 1:
         e, targets = e.reshape(targets.numel(), e.shape[-1]), targets.reshape(-1)
     _check(e, c, targets)
+    if c.shape[0] > MAX_GRAD_VOCAB and torch.is_grad_enabled() and (e.requires_grad or c.requires_grad):
+        raise ValueError(f"gradients for vocabularies up to {MAX_GRAD_VOCAB}, got V={c.shape[0]}")
     keep = None
     if filter_ignored and e.shape[0] >= _FILTER_FROM and e.numel() * c.shape[0] >= _FILTER_WORK[e.dtype] and not torch.cuda.is_current_stream_capturing():
         keep = _kept_rows(targets, ignore_index, c.shape[0])

@@ -1,0 +1,127 @@
+"""The two gradient products of ``linear_token_logprobs`` on the MI355X: ``de = x c`` and ``dc = x^T e``.
+
+Operands are small whole numbers: every sum stays below 2^24 and is exact in fp32 in any order, so the results have to equal
+the 64-bit products rounded once, bit for bit."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from maester_amd import _lib
+from maester_amd import linear_logprobs as LL
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _whole(*shape, seed, top=6):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(-top, top + 1, shape, generator=g).double()
+
+
+def _on_device(x, dtype, pitch=None):
+    """``x`` in ``dtype`` with rows ``pitch`` apart, 1e4 between them."""
+    pitch = x.shape[1] if pitch is None else pitch
+    out = torch.full((x.shape[0], pitch), 1e4, dtype=dtype, device=DEV)
+    out[:, : x.shape[1]] = x.to(DEV, dtype)
+    return out[:, : x.shape[1]]
+
+
+def _guarded(rows, dim, dtype, value=-7.0):
+    """``[rows, dim]`` inside a buffer of ``value``, and the buffer."""
+    room = torch.full((rows * dim + 2048,), value, dtype=dtype, device=DEV)
+    return room[1024: 1024 + rows * dim].view(rows, dim), room
+
+
+def _products(rows, vocab, dim, dtype, pitch_e=None, pitch_c=None, seed=0):
+    x, e, c = _whole(rows, vocab, seed=seed), _whole(rows, dim, seed=seed + 1), _whole(vocab, dim, seed=seed + 2)
+    assert 36 * max(rows, vocab) < 1 << 24
+    padded = torch.zeros(rows, -(-vocab // 8) * 8, dtype=dtype, device=DEV)
+    padded[:, :vocab] = x.to(DEV, dtype)
+    return x, e, c, padded, _on_device(e, dtype, pitch_e), _on_device(c, dtype, pitch_c)
+
+
+# around the edges of the tiles (256 by 256) and of a step of the contraction (64, fp32: 32), and one of several ranges
+SHAPES = [(1, 1, 8), (1, 300, 8), (3, 64, 40), (31, 63, 264), (32, 65, 256), (33, 257, 248), (64, 256, 512), (65, 255, 520),
+          (255, 1000, 136), (256, 2048, 64), (257, 2051, 72), (300, 40001, 304), (700, 513, 1048), (1025, 7, 8)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("rows,vocab,dim", SHAPES)
+def test_whole_numbers_are_exact(rows, vocab, dim, dtype):
+    x, e, c, xd, ed, cd = _products(rows, vocab, dim, dtype, seed=rows + vocab)
+    de, room_e = _guarded(rows, dim, dtype)
+    dc, room_c = _guarded(vocab, dim, dtype)
+    LL._products(xd, ed, cd, de, dc, False)
+    assert torch.equal(de.cpu(), (x @ c).to(dtype))
+    assert torch.equal(dc.cpu(), (x.t() @ e).to(dtype))
+    for room in (room_e, room_c):
+        assert bool((room[:1024] == -7).all()) and bool((room[-1024:] == -7).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_strided_operands_one_output_and_sums_of_blocks(dtype):
+    rows, vocab, dim = 130, 391, 328
+    x, e, c, xd, ed, cd = _products(rows, vocab, dim, dtype, pitch_e=352, pitch_c=336, seed=5)
+    de, _ = _guarded(rows, dim, dtype)
+    LL._products(xd, ed, cd, de, None, False)
+    assert torch.equal(de.cpu(), (x @ c).to(dtype))
+    dc, room = _guarded(vocab, dim, torch.float32)
+    dc.zero_()
+    for part in (slice(0, 64), slice(64, 129), slice(129, 130)):
+        LL._products(xd[part], ed[part], cd, None, dc, True)
+    assert torch.equal(dc.double().cpu(), x.t() @ e)
+    assert bool((room[:1024] == -7).all()) and bool((room[-1024:] == -7).all())
+
+
+def test_non_finite_values_stay_where_they_belong():
+    rows, vocab, dim = 70, 300, 264
+    x, e, c, xd, ed, cd = _products(rows, vocab, dim, torch.bfloat16, seed=9)
+    ed[3, 5] = float("nan")
+    cd[17, 260] = float("inf")
+    xd[:, 17] = 1.0
+    de, _ = _guarded(rows, dim, torch.bfloat16)
+    dc, _ = _guarded(vocab, dim, torch.bfloat16)
+    LL._products(xd, ed, cd, de, dc, False)
+    bad_e, bad_c = torch.zeros(rows, dim, dtype=torch.bool), torch.zeros(vocab, dim, dtype=torch.bool)
+    bad_e[:, 260] = True
+    bad_c[:, 5] = True
+    assert torch.equal(~torch.isfinite(de.cpu()), bad_e)
+    assert torch.equal(~torch.isfinite(dc.cpu()), bad_c)
+
+
+def test_padding_of_the_vocabulary_takes_no_part():
+    """All logits far below zero: exp(0 - lse) overflows in the padding behind the vocabulary."""
+    rows, vocab, dim = 9, 1003, 64
+    e = torch.ones(rows, dim, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    c = torch.full((vocab, dim), -40.0, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    targets = torch.arange(rows, device=DEV) * 100
+    logp, entropy = LL.linear_token_logprobs(e, c, targets)
+    (logp.sum() + entropy.sum()).backward()
+    assert bool(torch.isfinite(e.grad).all()) and bool(torch.isfinite(c.grad).all())
+    # every alternative is as likely: d logit = (target) - 1 / V, the entropy's gradient is 0
+    want = torch.full((vocab, dim), -rows / vocab, dtype=torch.float64)
+    want[targets.cpu()] += 1.0
+    # each of x's rows and then dc is rounded to bf16, and 1 / V of nine rows is summed: 2^-8 (rows of x) + 2^-8
+    assert float(((c.grad.double().cpu() - want).abs() / want.abs()).max()) <= 2 * 2.0 ** -8 + 1e-4
+
+
+def test_refusals():
+    rows, vocab, dim = 4, 24, 16
+    _, _, _, xd, ed, cd = _products(rows, vocab, dim, torch.float32, seed=1)
+    de = torch.empty(rows, dim, device=DEV)
+    with pytest.raises((RuntimeError, ValueError), match="both outputs"):
+        LL._products(xd, ed, cd, None, None, False)
+    with pytest.raises((RuntimeError, ValueError), match="aligned"):
+        LL._products(xd.view(-1)[1:65].view(4, 16), ed, cd[:16], de, None, False)
+    L = _lib.lib()
+    with pytest.raises((RuntimeError, ValueError), match="workspace"):
+        need = L.ma_linear_grads_workspace_bytes(8, 40000, 64, _lib.dtype_code(torch.float32))
+        assert need > 0
+        x, e, c = torch.zeros(8, 40000, device=DEV), torch.zeros(8, 64, device=DEV), torch.zeros(40000, 64, device=DEV)
+        out = torch.empty(8, 64, device=DEV)
+        _lib.launch(x.device, L.ma_linear_grads, x.data_ptr(), 40000, e.data_ptr(), 64, c.data_ptr(), 64, 8, 40000, 64, out.data_ptr(), None, 0,
+                    None, 0, _lib.dtype_code(torch.float32))
+    meta = torch.empty(LL.MAX_GRAD_VOCAB + 1, 8, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    with pytest.raises(ValueError, match="vocabularies"):
+        LL.linear_token_logprobs(torch.zeros(2, 8, device=DEV, dtype=torch.bfloat16), meta, torch.zeros(2, dtype=torch.int64, device=DEV))
