@@ -229,6 +229,7 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
                 static_for<0, MT / 2>([&](auto half) {
                     constexpr int i0 = decltype(half)::value * 32;
                     __builtin_amdgcn_sched_barrier(0);
+                    asm volatile("" : "+a"(acc[i0 / 16][j]), "+a"(acc[i0 / 16 + 1][j]));
                     float y[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) y[i] = lp_capped<CAP>(acc[(i0 + i) / 16][j][i % 16], a.sh);
@@ -253,7 +254,10 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
                 const int n = n0 + wn + 32 * j + r;
                 T* out = (T*)a.dlogits + (int64_t)n * a.pitch;
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+                for (int i = 0; i < MT; ++i) {
+                    // (an accumulator at a time, in the accumulation registers until then)
+                    __builtin_amdgcn_sched_barrier(0);
+                    asm volatile("" : "+a"(acc[i][j]));
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const int m = m0 + 32 * i + 8 * q + 4 * hh;
@@ -282,6 +286,7 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
                             }
                         }
                     }
+                }
             }
         }
     };
