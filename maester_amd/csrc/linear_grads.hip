@@ -24,7 +24,6 @@ namespace {
 
 constexpr int kSlot = 32 * 1024;         // one operand's step
 constexpr int kSlots = 5;
-using u32x2 = uint32_t __attribute__((ext_vector_type(2)));
 
 struct GradArgs {
     const char *a, *x;                   // a: c or e, rows of K
@@ -295,32 +294,63 @@ __global__ __launch_bounds__(256, 1) void linear_grads_kernel(const GradArgs a) 
         const int64_t start = (int64_t)range * a.range_stride + (int64_t)n0 * a.out_stride + m0;
         const auto out = __builtin_amdgcn_make_buffer_rsrc((char*)a.out + start * kOut, 0,
                                                            (int)(((int64_t)(min(BN, a.n - n0) - 1) * a.out_stride + a.m - m0) * kOut), 0x00020000);
-        const uint32_t row0 = (uint32_t)(wn + r) * (uint32_t)a.out_stride * kOut, left = (uint32_t)(a.m - m0);
-        static_for<0, MT * NT>([&](auto tile) {
-            constexpr int i = decltype(tile)::value % MT, j = decltype(tile)::value / MT;
-            // (an accumulator at a time, in the accumulation registers until then: not all of them copied first)
-            __builtin_amdgcn_sched_barrier(0);
-            asm volatile("" : "+a"(acc[i][j]));
+        const uint32_t pitch = (uint32_t)a.out_stride * kOut, left = (uint32_t)(a.m - m0);
+        if constexpr (kOut == 2) {
+            // Through the slot that is free until the next step's second part, a wave by itself in the runs that only it
+            // loads into, so that whole rows of the tile are stored (as they are, a lane has 8 bytes of a row and an
+            // instruction 32 rows: dc of 2560 x 262208 took 426 us so with 8 rows and 2357 with 2047, now 256 and 2220): 32 rows
+            // at a time, 16-byte chunk c of row r in place c ^ r % kChunks.
+            constexpr int kChunks = BM / 16, kRows = 1024 / BM;
+            const lds_ptr mine = smem + slot_at(slot + 4) + w * 1024;
+            const auto row_at = [&](int row) { return mine + (row / kRows) * 4096 + (row % kRows) * BM; };
+            const lds_ptr put = row_at(r) + 8 * hh;
+            const int chunk = lane % kChunks;
+            static_for<0, NT>([&](auto column) {
+                constexpr int j = decltype(column)::value;
+                static_for<0, MT>([&](auto block) {
+                    constexpr int i = decltype(block)::value;
+                    // (an accumulator at a time, in the accumulation registers until then: not all of them copied first)
+                    __builtin_amdgcn_sched_barrier(0);
+                    asm volatile("" : "+a"(acc[i][j]));
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint32_t m = wm + 32 * i + 8 * q + 4 * hh;
-                const uint32_t at = (row0 + 32 * j * (uint32_t)a.out_stride * kOut + m * kOut) | (m < left ? 0u : 0x80000000u);
-                f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                if constexpr (kOut == 4) {
+                    for (int q = 0; q < 4; ++q) {
+                        bf16x4 o;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] = (__bf16)acc[i][j][4 * q + e];
+                        *(MA_LDS bf16x4*)(put + (((4 * i + q) ^ (r % kChunks)) << 4)) = o;
+                    }
+                });
+                asm volatile("" ::: "memory");
+#pragma unroll
+                for (int k = 0; k < 32 / kRows; ++k) {
+                    const int row = k * kRows + lane / kChunks;
+                    const u32x4 v = *(MA_LDS u32x4*)(row_at(row) + ((chunk ^ (row % kChunks)) << 4));
+                    const uint32_t m = wm + 8 * chunk;
+                    __builtin_amdgcn_raw_buffer_store_b128(v, out, (uint32_t)(wn + 32 * j + row) * pitch + m * kOut + (m < left ? 0u : 0x80000000u), 0, 0);
+                }
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        } else {
+            const uint32_t row0 = (uint32_t)(wn + r) * pitch;
+            static_for<0, MT * NT>([&](auto tile) {
+                constexpr int i = decltype(tile)::value % MT, j = decltype(tile)::value / MT;
+                __builtin_amdgcn_sched_barrier(0);
+                asm volatile("" : "+a"(acc[i][j]));
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t m = wm + 32 * i + 8 * q + 4 * hh;
+                    const uint32_t at = (row0 + 32 * j * pitch + m * kOut) + (m < left ? 0u : 0x80000000u);
+                    f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
                     if constexpr (OUT == kAdded) {
                         const u32x4 before = __builtin_amdgcn_raw_buffer_load_b128(out, at, 0, 0);
                         v += *(const f32x4*)&before;
                     }
                     __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4*)&v, out, at, 0, 0);
-                } else {
-                    bf16x4 o;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = (__bf16)v[e];
-                    __builtin_amdgcn_raw_buffer_store_b64(*(const u32x2*)&o, out, at, 0, 0);
                 }
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        });
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        }
         clear();
     }
     // the last loads (of steps that do not exist) must not land in LDS that another workgroup has been given
@@ -372,7 +402,7 @@ Cut cut(int64_t n, int64_t m, int64_t steps, bool bf16, int most) {
     double least = 1e300;
     for (int t = 0; t < 3; ++t) {
         const int64_t tiles = ((m + kTiles[t][0] - 1) / kTiles[t][0]) * ((n + kTiles[t][1] - 1) / kTiles[t][1]);
-        const double store = kTiles[t][0] * kTiles[t][1] * 1.5e-4;
+        const double store = kTiles[t][0] * kTiles[t][1] * (bf16 ? 0.7e-4 : 1.5e-4);
         for (int r = 1; r <= most && r <= steps; ++r) {
             const double cost = (double)((tiles * r + 255) / 256) * ((double)((steps + r - 1) / r) * step_us[bf16][t] + store) +
                                 (r == 1 ? 0.0 : 4.0 + (double)r * n * m * 8.0 / 4.5e6);
