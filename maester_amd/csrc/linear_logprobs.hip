@@ -8,14 +8,18 @@
 // lane folds its logits of one token without talking to another lane; lanes, waves and workgroups that share a token
 // join their statistics once at the end of a workgroup's whole vocabulary range.
 //
-// A workgroup of four waves owns BN tokens and a range of the vocabulary that it walks in tiles of 256.  Both operands
-// are staged 128 (64) bytes of K at a time, global memory -> LDS without registers; rows past the end of the range or of
-// the tokens lie outside the loads' descriptors and arrive as zeros.  A row of a stage is 8 (4) chunks of 16 bytes, chunk
-// c of row r stored in place c ^ (r / 2 % 8) (c ^ (r / 4 % 4)): the 16 lanes that read together (16 rows, one chunk each)
-// then touch all 64 banks once.  Which chunk a lane of a load fetches is decided on the global side, so the exchange
-// costs nothing.  The loads of step q + STAGES are issued when the last fragment of step q has been read by all waves,
-// before its last products, so one barrier a step is enough and the first fragments of the next step are read while the
-// last products of this one run.
+// A workgroup of four waves owns BN tokens and a range of the vocabulary that it walks in tiles of 256.  Both operands are
+// brought in steps of 128 bytes of K, global memory -> LDS without registers; rows past the end of the range or of the
+// tokens lie outside the loads' descriptors and arrive as zeros.  A row of a step is 8 chunks of 16 bytes, chunk c of row r
+// stored in place c ^ (r / 2 % 8): the 16 lanes that read together (16 rows, one chunk each) then touch all 64 banks once.
+// Which chunk a lane of a load fetches is decided on the global side, so the exchange costs nothing.  With BN = 256 the LDS
+// holds five slots of one operand's step each, with fewer tokens three stages of both; either way one barrier a step is
+// enough, and the reads and loads are issued one or two to a product, in its shadow.
+//
+// What bounds it, in bf16: the matrix units from some 128 tokens on, the classifier's bytes below.  2560 x 262208: 8192
+// tokens 8.85 ms (1.24 PFLOP/s; a library product of these sizes that only stores its result 7.95), 1433 tokens 1.56 ms,
+// 8 tokens 0.24 ms (5.6 TB/s).  fp32, 640 x 32003, 210 tokens: 91 us (94 TFLOP/s; the library's products reach 139 on
+// large squares).
 #include <hip/hip_runtime.h>
 
 #include "common.h"
@@ -73,7 +77,7 @@ struct Tiling {
     static constexpr int kARuns = kBM / kRunRows / 4, kBRuns = BN / kRunRows / 4;       // 1 KB loads per wave and step
     static constexpr int kStage = (kBM + BN) * kStep;
     // place of chunk c of row r of a stage: c ^ key(r)
-    static constexpr __host__ __device__ int key(int r) { return kStep == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
+    static constexpr __host__ __device__ int key(int r) { return (r >> 1) & 7; }
     static constexpr int kLds = kRing ? 5 * kBM * kStep : kStage * kStages;
     static_assert(kLds <= 160 * 1024, "LDS");
 };
@@ -199,7 +203,7 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
     const float scale = a.sh.inv_temp * kLpLog2e;
     int target[NT];
     LpStats run[NT];
-    float ga[NT], gb[NT], top[NT], log_l[NT], ent[NT];
+    float ga[NT], gb[NT], gc[NT], top[NT], log_l[NT];       // d x = p (gb log2 p + gc), at the target + ga
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         const int n = n0 + wn + 32 * j + r;
@@ -208,11 +212,12 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
         target[j] = valid ? (int)t : -1;
         run[j] = {-INFINITY, 0.f, 0.f};
         if (GRAD) {
-            ga[j] = valid && a.dlogp ? a.dlogp[n] : 0.f;
-            gb[j] = valid && a.dentropy ? a.dentropy[n] : 0.f;
+            const float g = valid && a.dlogp ? a.dlogp[n] : 0.f, h = valid && a.dentropy ? a.dentropy[n] : 0.f;
+            ga[j] = g * a.sh.inv_temp;
+            gb[j] = -h * kLpLn2 * a.sh.inv_temp;
+            gc[j] = -fmaf(h, valid ? a.entropy[n] : 0.f, g) * a.sh.inv_temp;
             top[j] = valid ? a.stats[2 * n] : 0.f;
             log_l[j] = valid ? a.stats[2 * n + 1] : 0.f;
-            ent[j] = valid ? a.entropy[n] : 0.f;
         }
     }
 
@@ -253,40 +258,45 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
             } else {
                 const int n = n0 + wn + 32 * j + r;
                 T* out = (T*)a.dlogits + (int64_t)n * a.pitch;
+                // (the row's padding up to the next eight columns is written too, zeros: the products that follow read it)
+                const int m_end = v1 == a.vocab ? (v1 + 7) & ~7 : v1;
+                const auto store = [&](auto is_here) {
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    // (an accumulator at a time, in the accumulation registers until then)
-                    __builtin_amdgcn_sched_barrier(0);
-                    asm volatile("" : "+a"(acc[i][j]));
+                    for (int i = 0; i < MT; ++i) {
+                        // (an accumulator at a time, in the accumulation registers until then)
+                        __builtin_amdgcn_sched_barrier(0);
+                        asm volatile("" : "+a"(acc[i][j]));
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int m = m0 + 32 * i + 8 * q + 4 * hh;
-                        float d[4];
+                        for (int q = 0; q < 4; ++q) {
+                            const int m = m0 + 32 * i + 8 * q + 4 * hh;
+                            float d[4];
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) {
-                            const float x = acc[i][j][4 * q + v];
-                            const float th = CAP ? lp_tanh(x * a.sh.inv_cap) : 0.f;
-                            const float lp = fmaf(CAP ? a.sh.cap * th : x, scale, -top[j]) - log_l[j];      // log2 p
-                            const float p = __builtin_amdgcn_exp2f(lp);
-                            d[v] = -p * fmaf(gb[j], fmaf(fmaxf(lp, -1e30f), kLpLn2, ent[j]), ga[j]);
-                            if (here && 32 * i + 8 * q + v == t) d[v] += ga[j];
-                            d[v] *= CAP ? (1.f - th * th) * a.sh.inv_temp : a.sh.inv_temp;
-                            if (target[j] < 0) d[v] = 0.f;
-                            if (PARTIAL && m + v >= a.vocab) d[v] = 0.f;
-                        }
-                        // (the row's padding up to the next eight columns is written too, zeros: the products that follow read it)
-                        if (n < a.rows && (!PARTIAL || m < (v1 == a.vocab ? (v1 + 7) & ~7 : v1))) {
-                            if constexpr (sizeof(T) == 2) {
-                                bf16x4 o;
+                            for (int v = 0; v < 4; ++v) {
+                                const float x = acc[i][j][4 * q + v];
+                                const float th = CAP ? lp_tanh(x * a.sh.inv_cap) : 0.f;
+                                const float lp = fmaf(CAP ? a.sh.cap * th : x, scale, -top[j]) - log_l[j];      // log2 p
+                                const float p = __builtin_amdgcn_exp2f(lp);
+                                d[v] = p * fmaf(gb[j], fmaxf(lp, -1e30f), gc[j]);
+                                if constexpr (decltype(is_here)::value) d[v] += here && 32 * i + 8 * q + v == t ? ga[j] : 0.f;
+                                if (CAP) d[v] *= 1.f - th * th;
+                                if (target[j] < 0) d[v] = 0.f;
+                                if (PARTIAL && m + v >= a.vocab) d[v] = 0.f;
+                            }
+                            if (n < a.rows && (!PARTIAL || m < m_end)) {
+                                if constexpr (sizeof(T) == 2) {
+                                    bf16x4 o;
 #pragma unroll
-                                for (int v = 0; v < 4; ++v) o[v] = (__bf16)d[v];
-                                *(bf16x4*)(out + m) = o;
-                            } else {
-                                *(float4*)(out + m) = make_float4(d[0], d[1], d[2], d[3]);
+                                    for (int v = 0; v < 4; ++v) o[v] = (__bf16)d[v];
+                                    *(bf16x4*)(out + m) = o;
+                                } else {
+                                    *(float4*)(out + m) = make_float4(d[0], d[1], d[2], d[3]);
+                                }
                             }
                         }
                     }
-                }
+                };
+                if (__any(here)) store(std::true_type{});
+                else store(std::false_type{});
             }
         }
     };
