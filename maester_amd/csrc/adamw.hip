@@ -11,8 +11,8 @@
 // round-to-nearest a moment that changes by less than half a code a step (3 % at best; (1 - b2) of it changes) would
 // never move.  The 16 random bits per rounding come from a hash of (seed, t, tensor, element), so a step is a function of
 // its inputs.  A nonzero r is never rounded to zero: m / (0 + eps) would be a jump of any size.  Scaling by powers of two
-// is exact, and the file is compiled without contraction, reassociation or approximate square roots, so that the codes
-// are those of the formula in IEEE single precision, operation by operation.
+// is exact, and the file is compiled without contraction or reassociation, square roots are rounded correctly (roots8), so
+// that the codes are those of the formula in IEEE single precision, operation by operation.
 #include <hip/hip_runtime.h>
 
 #include "common.h"
