@@ -96,7 +96,7 @@ def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentrop
     # several blocks: dc is summed in fp32 and rounded once at the end
     dc = None
     if need_dc:
-        dc = torch.empty(vocab, k, dtype=c.dtype, device=c.device) if n <= step else torch.zeros(vocab, k, device=c.device)
+        dc = torch.empty(vocab, k, dtype=c.dtype, device=c.device) if n <= step else torch.zeros(vocab, k, dtype=torch.float32, device=c.device)
     for r0 in range(0, n, step):
         whole, rows = n <= step, slice(r0, min(n, r0 + step))
         buf = block[: rows.stop - r0]
@@ -161,9 +161,9 @@ def linear_token_logprobs(e: torch.Tensor, c: torch.Tensor, targets: torch.Tenso
     ``e`` ``[..., K]`` hidden states, ``c`` ``[V, K]`` classifier (Gemma: the tied embedding table), bf16 or fp32 alike,
     ``K`` a multiple of 8 (fp32: 4); the logits are products of the inputs summed in fp32 and never stored.  ``softcap``,
     ``temperature`` and ignored targets as in ``token_logprobs``.  ``chunk_rows``: rows per block of the backward (default:
-    about 4 GiB of gradient of the logits at a time; V is at most 2^21 with gradients).  ``filter_ignored``: a large call (more than 256 rows, 2^36
-    multiply-adds a product) drops the rows whose target does not count before any product, which costs its one host
-    synchronisation; not under graph capture."""
+    about 4 GiB of gradient of the logits at a time; V is at most 2^21 with gradients).  ``filter_ignored``: a large call
+    (more than 256 rows, 2^36 multiply-adds a product; fp32 2^33) drops the rows whose target does not count before any
+    product, which costs its one host synchronisation; not under graph capture."""
     if e.dim() < 1 or targets.shape != e.shape[:-1]:
         raise ValueError(f"targets shape {tuple(targets.shape)} != leading shape of e {tuple(e.shape[:-1])}")
     lead = targets.shape

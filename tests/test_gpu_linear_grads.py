@@ -125,3 +125,22 @@ def test_refusals():
     meta = torch.empty(LL.MAX_GRAD_VOCAB + 1, 8, device=DEV, dtype=torch.bfloat16).requires_grad_()
     with pytest.raises(ValueError, match="vocabularies"):
         LL.linear_token_logprobs(torch.zeros(2, 8, device=DEV, dtype=torch.bfloat16), meta, torch.zeros(2, dtype=torch.int64, device=DEV))
+
+
+def test_blocks_of_rows_under_another_default_dtype():
+    """Several blocks sum the classifier's gradient in fp32 whatever new tensors are by default."""
+    rows, vocab, dim = 37, 515, 64
+    e, c = torch.randn(rows, dim, device=DEV), torch.randn(vocab, dim, device=DEV)
+    targets = torch.randint(0, vocab, (rows,), device=DEV)
+    grads = []
+    for default in (torch.float32, torch.float64, torch.bfloat16):
+        torch.set_default_dtype(default)
+        try:
+            a, b = e.clone().requires_grad_(), c.clone().requires_grad_()
+            logp, entropy = LL.linear_token_logprobs(a, b, targets, chunk_rows=16)
+            (logp.sum() + entropy.sum()).backward()
+        finally:
+            torch.set_default_dtype(torch.float32)
+        grads.append((a.grad, b.grad))
+    for g in grads[1:]:
+        assert torch.equal(g[0], grads[0][0]) and torch.equal(g[1], grads[0][1])
