@@ -259,8 +259,8 @@ int ma_linear_grads(const void* x, int64_t x_stride, const void* e, int64_t e_st
  * magnitude to 448 or less (1 for a block of zeros, NaN for one with a NaN or an infinity); codes are
  * rounded stochastically from a hash of (seed, t, index in the list, element), and a nonzero sqrt(v) is
  * never rounded to 0.
- * tensors: HOST array, copied before the call returns (its pointers are device pointers); tensors of one
- * call must not overlap.  lr_device: fp32 on the device, used in place of lr (NULL: lr).  clip: fp32 on
+ * tensors: HOST array, copied before the call returns (its pointers are device pointers); a buffer that the
+ * step writes and that shares memory with another of the call is refused.  lr_device: fp32 on the device, used in place of lr (NULL: lr).  clip: fp32 on
  * the device, multiplies the gradients (NULL: 1).  max_norm >= 0: the norm of all gradients of the call
  * is formed first (in fp64) and they are multiplied by min(1, max_norm / (norm + 1e-6)) instead; norm_out
  * (fp32, may be NULL) receives it.  step: int64 on the device, incremented.

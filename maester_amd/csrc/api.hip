@@ -2,7 +2,10 @@
 // reachable without a GPU) and dispatch to the kernel launchers.  See include/maester_attn.h.
 #include "common.h"
 
+#include <stdlib.h>
 #include <string.h>
+
+#include <algorithm>
 
 namespace ma {
 
@@ -399,6 +402,50 @@ static int check_adamw(const char* who, const ma_adamw_tensor* tensors, int coun
     return MA_OK;
 }
 
+// What a step writes must not share memory with anything else of the call: elements are read and written in any order.
+namespace {
+struct Extent {
+    uintptr_t begin, end;
+    int tensor;
+    bool written;
+};
+bool before(const Extent& a, const Extent& b) { return a.begin < b.begin; }
+}  // namespace
+static int check_extents(const char* who, const ma_adamw_tensor* tensors, int count, int state_bits) {
+    Extent few[7 * 64];
+    Extent* all = count <= 64 ? few : (Extent*)malloc(sizeof(Extent) * 7 * (size_t)count);
+    if (!all) return fail(MA_ERR_BAD_ARG, "%s: no host memory for a list of %d tensors", who, count);
+    size_t n = 0;
+    for (int i = 0; i < count; ++i) {
+        const ma_adamw_tensor& t = tensors[i];
+        if (t.n == 0) continue;
+        const auto add = [&](const void* p, int64_t bytes, bool written) {
+            if (p) all[n++] = {(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, i, written};
+        };
+        const int64_t state = t.n * (state_bits / 8), scales = state_bits == 8 ? (t.n + MA_ADAMW_BLOCK - 1) / MA_ADAMW_BLOCK * 4 : 0;
+        add(t.param, t.n * (t.param_dtype == MA_DTYPE_BF16 ? 2 : 4), true);
+        add(t.grad, t.n * (t.grad_dtype == MA_DTYPE_BF16 ? 2 : 4), false);
+        add(t.exp_avg, state, true);
+        add(t.exp_avg_sq, state, true);
+        add(t.master, t.n * 4, true);
+        if (scales) {
+            add(t.exp_avg_scale, scales, true);
+            add(t.exp_avg_sq_scale, scales, true);
+        }
+    }
+    std::sort(all, all + n, before);
+    int found = -1;
+    uintptr_t written_to = 0, read_to = 0;
+    for (size_t i = 0; i < n && found < 0; ++i) {
+        if (all[i].begin < written_to || (all[i].written && all[i].begin < read_to)) found = all[i].tensor;
+        uintptr_t& to = all[i].written ? written_to : read_to;
+        if (all[i].end > to) to = all[i].end;
+    }
+    if (all != few) free(all);
+    if (found >= 0) return fail(MA_ERR_BAD_ARG, "%s: a buffer of tensor %d overlaps one that the step writes", who, found);
+    return MA_OK;
+}
+
 int ma_adamw_step(const ma_adamw_tensor* tensors, int count, int state_bits, double lr, const float* lr_device, double beta1,
                   double beta2, double eps, double weight_decay, double max_norm, const float* clip, float* norm_out,
                   int64_t* step, uint32_t seed, void* workspace, size_t workspace_bytes, void* stream) {
@@ -410,6 +457,7 @@ int ma_adamw_step(const ma_adamw_tensor* tensors, int count, int state_bits, dou
     if (!(eps >= 0.0) || !(weight_decay >= 0.0) || (!lr_device && !(lr >= 0.0)))
         return fail(MA_ERR_BAD_ARG, "%s: lr=%g, eps=%g and weight_decay=%g must be >= 0", who, lr, eps, weight_decay);
     if (!step || ((uintptr_t)step & 7) != 0) return fail(MA_ERR_BAD_ARG, "%s: step is NULL or not 8-byte aligned", who);
+    MA_TRY(check_extents(who, tensors, count, state_bits));
     const AdamwArgs a = {tensors, count, state_bits, max_norm >= 0.0 ? 1 : 0, lr, beta1, beta2, eps, weight_decay, max_norm, seed,
                          lr_device, clip, norm_out, nullptr, step, workspace};
     return launch_adamw(a, (hipStream_t)stream);

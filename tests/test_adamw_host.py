@@ -106,3 +106,25 @@ def test_blocks8_values():
     b.scales[2] = 4.0
     b.codes.view(-1).view(torch.uint8)[256:] = 0x38          # 1.0
     assert torch.all(b.float().view(-1)[256:] == 4.0) and torch.all(b.float().view(-1)[:256] == 0)
+
+
+def test_buffers_that_share_memory_are_refused():
+    L = _lib.lib()
+
+    def table(**moved):
+        t = (_lib.MaAdamwTensor * 2)()
+        for i, row in enumerate(t):
+            for j, k in enumerate(("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")):
+                setattr(row, k, P + 0x100000 * (i + 1) + 400 * j)
+            row.n, row.param_dtype, row.grad_dtype = 100, 0, 0
+        for k, v in moved.items():
+            setattr(t[1], k, v)
+        return t
+
+    first = table()[0]
+    for bits, moved in [(32, dict(param=first.param)), (32, dict(param=first.param + 396)), (32, dict(exp_avg=first.exp_avg_sq - 396)),
+                        (32, dict(grad=first.param + 4)), (32, dict(param=first.grad - 200)), (32, dict(exp_avg=first.grad + 399 // 4 * 4)),
+                        (8, dict(exp_avg_scale=first.exp_avg_sq_scale)), (8, dict(exp_avg=first.exp_avg + 99)),
+                        (32, dict(param_dtype=1, master=first.exp_avg))]:
+        assert _step(table=table(**moved), count=2, bits=bits) == -1, moved
+        assert "overlaps" in L.ma_last_error().decode(), moved

@@ -404,6 +404,11 @@ def test_refusals(gpu):
                     (dict(params=[p.cpu()]), RuntimeError), (dict(params=[], grads=[], exp_avgs=[], exp_avg_sqs=[]), ValueError)]:
         with pytest.raises(err):
             adamw_step(**{**ok, **kw})
+    flat = torch.zeros(600, device=gpu)
+    for kw in (dict(params=[flat[:256], flat[255:511]], grads=[g, g], exp_avgs=[m, m.clone()], exp_avg_sqs=[v, v.clone()]),
+               dict(params=[flat[:256]], grads=[flat[200:456]])):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            adamw_step(**{**ok, **kw})
     for kw in (dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(lr=-1.0), dict(weight_decay=float("nan"))):
         with pytest.raises(RuntimeError):
             adamw_step(**ok, **kw)
@@ -413,3 +418,18 @@ def test_refusals(gpu):
             AdamW([torch.nn.Parameter(p)], **kw)
     with pytest.raises(ValueError):
         global_grad_norm([])
+
+
+def test_neighbours_in_one_buffer(gpu):
+    """Everything in one allocation without a gap, one gradient for both parameters: nothing overlaps."""
+    n = 301
+    flat, g = torch.randn(6 * n, device=gpu), torch.randn(n, device=gpu)
+    flat[2 * n:] = 0
+    parts = list(flat.split(n))
+    before = flat.clone()
+    step = torch.zeros((), dtype=torch.int64, device=gpu)
+    adamw_step(parts[:2], [g, g], parts[2:4], parts[4:], step, lr=0.1, weight_decay=0.0)
+    want = before[:2 * n] - 0.1 * torch.sign(g).repeat(2)
+    # |m / sqrt(v)| = 1 in exact arithmetic after one step: eps, some 12 roundings of the update, one each of the two sums
+    limit = 0.1 * (16 * 2.0 ** -24 + 1e-8 / float(g.abs().min())) + 2 * 2.0 ** -24 * (float(before.abs().max()) + 0.1)
+    assert float((flat[:2 * n] - want).abs().max()) <= limit
