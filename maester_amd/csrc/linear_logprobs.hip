@@ -275,8 +275,8 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
                                 const float x = acc[i][j][4 * q + v];
                                 const float th = CAP ? lp_tanh(x * a.sh.inv_cap) : 0.f;
                                 const float lp = fmaf(CAP ? a.sh.cap * th : x, scale, -top[j]) - log_l[j];      // log2 p
-                                const float p = __builtin_amdgcn_exp2f(lp);
-                                d[v] = p * fmaf(gb[j], fmaxf(lp, -1e30f), gc[j]);
+                                const float p = __builtin_amdgcn_exp2f(lp);        // (0 below -150: no product with a larger lp)
+                                d[v] = p * fmaf(gb[j], fmaxf(lp, -200.f), gc[j]);
                                 if constexpr (decltype(is_here)::value) d[v] += here && 32 * i + 8 * q + v == t ? ga[j] : 0.f;
                                 if (CAP) d[v] *= 1.f - th * th;
                                 if (target[j] < 0) d[v] = 0.f;

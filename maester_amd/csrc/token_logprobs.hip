@@ -437,8 +437,8 @@ __global__ __launch_bounds__(kLpBwdThreads) void token_logprobs_bwd_kernel(const
             for (int i = 0; i < 8; ++i) {
                 const float th = CAP ? lp_tanh(v[i] * sh.inv_cap) : 0.f;
                 const float lp = fmaf((CAP ? sh.cap * th : v[i]) - top, sh.inv_temp, -log_l);
-                const float p = __builtin_amdgcn_exp2f(lp * kLpLog2e);
-                d[i] = -p * fmaf(b, fmaxf(lp, -1e30f) + h, a);
+                const float p = __builtin_amdgcn_exp2f(lp * kLpLog2e);        // (0 below -150: no product with a larger lp)
+                d[i] = -p * fmaf(b, fmaxf(lp, -200.f) + h, a);
                 if (j + i == target) d[i] += a;
                 d[i] *= CAP ? (1.f - th * th) * sh.inv_temp : sh.inv_temp;
             }

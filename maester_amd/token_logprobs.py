@@ -111,8 +111,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
     ``softcap * tanh(x / softcap)`` where a cap is given, then divided by ``temperature``.  Rows whose target is
     ``ignore_index`` (or outside the vocabulary) get 0 for both and no gradient; the alternatives come for every row,
     equal logits in the order of their index.  Logits of ``-inf`` have probability 0 (a soft cap makes them
-    ``-softcap`` first: mask after capping); a row with a NaN or ``+inf``, or with nothing but ``-inf``, gives NaN.  ``logp`` and ``entropy`` are differentiable in the logits (once), the
-    alternatives are not."""
+    ``-softcap`` first: mask after capping); a row with a NaN or ``+inf``, or with nothing but ``-inf``, gives NaN.
+    ``logp`` and ``entropy`` are differentiable in the logits (once), the alternatives are not."""
     if logits.dim() < 1 or targets.shape != logits.shape[:-1]:
         raise ValueError(f"targets shape {tuple(targets.shape)} != leading shape of logits {tuple(logits.shape[:-1])}")
     lead, vocab = targets.shape, logits.shape[-1]

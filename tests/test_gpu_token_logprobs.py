@@ -342,3 +342,20 @@ def test_other_stream_and_graph_replay(gpu):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_large_entropy_gradients_on_masked_rows(gpu):
+    """A masked alternative has probability 0 and no gradient, however large the entropy's is."""
+    x = torch.randn(3, 700, dtype=torch.float64)
+    x[:, 300:] = -float("inf")
+    x[1, 5:300] = torch.finfo(torch.float32).min
+    leaf = x.float().to(gpu).requires_grad_()
+    out = token_logprobs(leaf, torch.tensor([3, 1, 299], device=gpu))
+    (out.entropy * 1e12).sum().backward()
+    got = leaf.grad.double().cpu()
+    assert bool(torch.isfinite(got).all()) and bool((got[:, 300:] == 0).all())
+    p = torch.softmax(x.float().double(), 1)
+    lp = torch.where(p > 0, torch.log(p.clamp_min(1e-300)), torch.zeros_like(p))
+    h = -(p * lp).sum(1, keepdim=True)
+    # p, log p + H and their product: errors of 2^-24 relative to |log p| + H + 1, some tens of operations
+    assert bool(((got + 1e12 * p * (lp + h)).abs() <= 1e12 * 64 * 2.0 ** -24 * (p * (lp.abs() + h + 1) ** 2 + 1e-30)).all())
