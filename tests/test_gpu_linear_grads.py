@@ -144,3 +144,33 @@ def test_blocks_of_rows_under_another_default_dtype():
         grads.append((a.grad, b.grad))
     for g in grads[1:]:
         assert torch.equal(g[0], grads[0][0]) and torch.equal(g[1], grads[0][1])
+
+
+def test_beyond_32_bits_of_offset():
+    """The classifier and its gradient take 4.3 GB each; then the logits' gradient does."""
+    rows, vocab, dim = 40, 262144, 8200
+    torch.manual_seed(3)
+    c = torch.randint(-3, 4, (vocab, dim), device=DEV, dtype=torch.int8).to(torch.bfloat16)
+    x = torch.randint(-3, 4, (rows, vocab), device=DEV).to(torch.bfloat16)
+    e = torch.randint(-3, 4, (rows, dim), device=DEV).to(torch.bfloat16)
+    assert c.numel() * 2 > 1 << 32 and 9 * vocab < 1 << 24
+    de, dc = torch.empty(rows, dim, device=DEV, dtype=torch.bfloat16), torch.empty_like(c)
+    LL._products(x, e, c, de, dc, False)
+    want = torch.zeros(rows, dim, device=DEV, dtype=torch.float64)
+    for part in torch.arange(vocab, device=DEV).split(16384):
+        lo, hi = int(part[0]), int(part[-1]) + 1
+        want += x[:, lo:hi].double() @ c[lo:hi].double()
+        assert torch.equal(dc[lo:hi], (x[:, lo:hi].double().t().contiguous() @ e.double()).to(torch.bfloat16)), lo
+    assert torch.equal(de, want.to(torch.bfloat16))
+    del c, dc, x
+
+    rows, dim, last = 8300, 16, 70
+    x = torch.zeros(rows, vocab, device=DEV, dtype=torch.bfloat16)
+    assert (rows - last) * vocab * 2 > 1 << 32
+    x[-last:] = torch.randint(-3, 4, (last, vocab), device=DEV).to(torch.bfloat16)
+    e, c = (torch.randint(-3, 4, (n, dim), device=DEV).to(torch.bfloat16) for n in (rows, vocab))
+    de, dc = torch.empty_like(e), torch.empty_like(c)
+    LL._products(x, e, c, de, dc, False)
+    tail = x[-last:].double()
+    assert bool((de[:-last] == 0).all()) and torch.equal(de[-last:], (tail @ c.double()).to(torch.bfloat16))
+    assert torch.equal(dc, (tail.t().contiguous() @ e[-last:].double()).to(torch.bfloat16))

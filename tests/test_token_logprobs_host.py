@@ -92,3 +92,27 @@ def test_linear_workspace():
     assert L.ma_linear_logprobs_workspace_bytes(0, 100) == 0
     assert L.ma_linear_logprobs_workspace_bytes(5, 600) == 32 + 3 * 5 * 12          # targets' logits, three ranges' statistics
     assert L.ma_linear_logprobs_workspace_bytes(8, 262208) == 32 + 256 * 8 * 12
+
+
+def _grads(x=P, xs=304, e=P, es=64, c=P, cs=64, rows=9, vocab=300, dim=64, de=P, dc=P, add=0, ws=P, ws_bytes=1 << 20, dtype=1):
+    return _lib.lib().ma_linear_grads(x, xs, e, es, c, cs, rows, vocab, dim, de, dc, add, ws, ws_bytes, dtype, None)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(x=None), -1, "NULL"), (dict(c=None), -1, "NULL"), (dict(e=None), -1, "NULL"), (dict(de=None, dc=None), -1, "both outputs"),
+    (dict(x=P + 8), -1, "aligned"), (dict(dc=P + 8), -1, "aligned"), (dict(rows=0), -1, "rows"), (dict(vocab=0), -1, "vocab"),
+    (dict(dim=60, es=64, cs=64), -2, "dim"), (dict(dim=1 << 17, es=1 << 17, cs=1 << 17), -2, "dim"), (dict(xs=300), -1, "strides"),
+    (dict(xs=296), -1, "strides"), (dict(es=56), -1, "strides"), (dict(cs=68), -1, "strides"), (dict(xs=(1 << 21) + 8), -2, "2^21"),
+    (dict(vocab=1 << 22, xs=1 << 22), -2, "2^21"), (dict(es=(1 << 20) + 8), -2, "2^20"), (dict(dtype=7), -1, "dtype"),
+    (dict(vocab=40000, xs=40000, ws=None), -1, "workspace"), (dict(vocab=40000, xs=40000, ws_bytes=16), -1, "workspace"),
+    (dict(vocab=40000, xs=40000, ws=P + 8), -1, "workspace")])
+def test_gradient_products_refuse(kw, code, text):
+    assert _grads(**kw) == code and text in _lib.lib().ma_last_error().decode()
+
+
+def test_workspace_of_the_gradient_products():
+    L = _lib.lib()
+    assert L.ma_linear_grads_workspace_bytes(0, 100, 64, 1) == 0 and L.ma_linear_grads_workspace_bytes(9, 64, 64, 1) == 0
+    for rows, vocab, dim, dtype in ((9, 40000, 64, 1), (2047, 262208, 2560, 1), (210, 32003, 640, 0), (1 << 20, 32003, 640, 1)):
+        need = L.ma_linear_grads_workspace_bytes(rows, vocab, dim, dtype)
+        assert need % (rows * dim * 4) == 0 and need // (rows * dim * 4) <= 128
