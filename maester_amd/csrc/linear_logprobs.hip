@@ -17,7 +17,7 @@
 // enough, and the reads and loads are issued one or two to a product, in its shadow.
 //
 // What bounds it, in bf16: the matrix units from some 128 tokens on, the classifier's bytes below.  2560 x 262208: 8192
-// tokens 8.85 ms (1.24 PFLOP/s; a library product of these sizes that only stores its result 7.95), 1433 tokens 1.56 ms,
+// tokens 8.7 ms (1.26 PFLOP/s; a library product of these sizes that only stores its result 7.95), 1433 tokens 1.56 ms,
 // 8 tokens 0.24 ms (5.6 TB/s).  fp32, 640 x 32003, 210 tokens: 91 us (94 TFLOP/s; the library's products reach 139 on
 // large squares).
 #include <hip/hip_runtime.h>
