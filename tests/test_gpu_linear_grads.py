@@ -43,7 +43,8 @@ def _products(rows, vocab, dim, dtype, pitch_e=None, pitch_c=None, seed=0):
 
 # around the edges of the tiles (256 by 256) and of a step of the contraction (64, fp32: 32), and one of several ranges
 SHAPES = [(1, 1, 8), (1, 300, 8), (3, 64, 40), (31, 63, 264), (32, 65, 256), (33, 257, 248), (64, 256, 512), (65, 255, 520),
-          (255, 1000, 136), (256, 2048, 64), (257, 2051, 72), (300, 40001, 304), (700, 513, 1048), (1025, 7, 8)]
+          (255, 1000, 136), (256, 2048, 64), (257, 2051, 72), (300, 40001, 304), (700, 513, 1048), (1025, 7, 8), (70001, 9, 16),
+          (5, 40, 65536), (2, 300001, 16)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
