@@ -21,6 +21,7 @@
 
 #include "common.h"
 #include "mfma.h"
+#include "split.h"
 
 namespace ma {
 
@@ -39,24 +40,6 @@ struct GradArgs {
 };
 
 enum Output { kInput, kStored, kAdded };      // in the operands' type; fp32, stored; fp32, added to what is there
-
-template <typename T>
-struct Mac;
-template <>
-struct Mac<uint16_t> {
-    static __device__ __forceinline__ f32x16 mac(u32x4 a, u32x4 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(bf16x8*)&a, *(bf16x8*)&b, c, 0, 0, 0);
-    }
-};
-template <>
-struct Mac<float> {
-    static __device__ __forceinline__ f32x16 mac(u32x4 a, u32x4 b, f32x16 c) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
-        return c;
-    }
-};
 
 __device__ __forceinline__ u32x4 uniform_rsrc(uint64_t base, uint32_t bytes) {
     const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)base), hi = __builtin_amdgcn_readfirstlane((uint32_t)(base >> 32));
@@ -219,7 +202,7 @@ __global__ __launch_bounds__(256, 1) void linear_grads_kernel(const GradArgs a) 
     open_x();
 
     const uint32_t lds0 = lds_addr(smem) + w * 1024;
-    u32x4 fa[2][MT], fx[2][NT];
+    Fragments<T, MT, NT> frags;
     f32x16 acc[MT][NT];
     auto clear = [&]() {
 #pragma unroll
@@ -229,8 +212,8 @@ __global__ __launch_bounds__(256, 1) void linear_grads_kernel(const GradArgs a) 
     };
     auto read_one = [&](int buf, lds_ptr slot_a, lds_ptr slot_x, auto sub, auto which) {
         constexpr int SUB = decltype(sub)::value, i = decltype(which)::value;
-        if constexpr (i < MT) fa[buf][i] = ca.template read<i, SUB>(slot_a);
-        else fx[buf][i - MT] = cx.template read<i - MT, SUB>(slot_x);
+        if constexpr (i < MT) frags.a[buf][i] = ca.template read<i, SUB>(slot_a);
+        else frags.b[buf][i - MT] = cx.template read<i - MT, SUB>(slot_x);
     };
     auto load_run = [&](auto run) {                   // 0 .. kA - 1: a, the others x
         constexpr int p = decltype(run)::value;
@@ -245,7 +228,7 @@ __global__ __launch_bounds__(256, 1) void linear_grads_kernel(const GradArgs a) 
             constexpr int i = decltype(step)::value;
             if constexpr (i < H) static_for<i * R / H, (i + 1) * R / H>([&](auto k) { read_one(buf ^ 1, slot_a, slot_x, sub, k); });
             else static_for<W0 + (i - H) * W / (P - H), W0 + (i - H + 1) * W / (P - H)>([&](auto k) { load_run(k); });
-            acc[i % MT][i / MT] = Mac<T>::mac(fa[buf][i % MT], fx[buf][i / MT], acc[i % MT][i / MT]);
+            frags.template product<i>(buf, acc);
             __builtin_amdgcn_sched_barrier(0);
         });
     };
@@ -270,6 +253,7 @@ __global__ __launch_bounds__(256, 1) void linear_grads_kernel(const GradArgs a) 
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kA + kX / 2) : "memory");
     barrier();
     static_for<0, MT + NT>([&](auto k) { read_one(0, smem, smem + kSlot, std::integral_constant<int, 0>{}, k); });
+    frags.begin();
     int slot = 0;
     const auto slot_at = [](int i) { return (i >= kSlots ? i - kSlots : i) * kSlot; };
     for (int t = 0; t < count; ++t) {
@@ -394,14 +378,14 @@ int start(const GradArgs& a, hipStream_t st) {
 // times the steps of a unit and what its results take, and the results of more than one range, written and joined.  The
 // larger tiles do more per byte that they read; the smaller ones leave less of the chip idle and of a tile empty.  Measured
 // with 256 x 256, 128 x 256 and 128 x 128 alone (us, de and dc): bf16, 2560 x 262208, 2047 rows 2157 + 2365, 3077 + 2709,
-// 4103 + 3408; 128 x 2051, 257 rows 21 + 14, 19 + 11, 13 + 7; fp32, 640 x 32003, 210 rows 134 + 126, 110 + 102, 99 + 87, and
-// 1500 rows 557 + 713, 481 + 553, 521 + 485.
+// 4103 + 3408; 128 x 2051, 257 rows 21 + 14, 19 + 11, 13 + 7; fp32, 2048 x 32000, 4096 rows 2456 + 2468, 2767 + 2988,
+// 3388 + 3323, and 640 x 32003, 300 rows 123 + 104, 115 + 93, 107 + 94.
 constexpr int kTiles[3][2] = {{256, 256}, {128, 256}, {128, 128}};          // M, N
 struct Cut {
     int tile, ranges;
 };
 Cut cut(int64_t n, int64_t m, int64_t steps, bool bf16, int most) {
-    static const double step_us[2][3] = {{7.6, 3.9, 2.05}, {1.7, 1.2, 0.8}};
+    static const double step_us[2][3] = {{5.1, 2.9, 1.75}, {1.7, 1.2, 0.8}};
     Cut best = {0, 1};
     double least = 1e300;
     for (int t = 0; t < 3; ++t) {

@@ -18,14 +18,15 @@
 //
 // What bounds it, in bf16: the matrix units from some 128 tokens on, the classifier's bytes below.  2560 x 262208: 8192
 // tokens 8.7 ms (1.26 PFLOP/s; a library product of these sizes that only stores its result 7.95), 1433 tokens 1.56 ms,
-// 8 tokens 0.24 ms (5.6 TB/s).  fp32, 640 x 32003, 210 tokens: 91 us (94 TFLOP/s; the library's products reach 139 on
-// large squares).
+// 8 tokens 0.24 ms (5.6 TB/s).  fp32 (split.h), 2048 x 32000, 4096 tokens 2.38 ms (226 TFLOP/s; the library's fp32
+// products reach 139, and this kernel on the fp32 instructions took 3.82), 640 x 32003, 210 tokens 71 us.
 #include <hip/hip_runtime.h>
 
 #include "common.h"
 #include "logprobs.h"
 #include "mfma.h"
 #include "rowio.h"
+#include "split.h"
 
 namespace ma {
 
@@ -46,25 +47,6 @@ struct LinArgs {
     const float *stats, *entropy, *dlogp, *dentropy;   // gradient
     void* dlogits;
     int64_t pitch;                           // elements between its rows
-};
-
-template <typename T>
-struct Product;
-template <>
-struct Product<uint16_t> {
-    static __device__ __forceinline__ f32x16 mac(u32x4 a, u32x4 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(bf16x8*)&a, *(bf16x8*)&b, c, 0, 0, 0);
-    }
-};
-// fp32: a lane's 16 bytes are four K values, taken one per instruction (both operands in the same order)
-template <>
-struct Product<float> {
-    static __device__ __forceinline__ f32x16 mac(u32x4 a, u32x4 b, f32x16 c) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
-        return c;
-    }
 };
 
 template <int BN>
@@ -171,11 +153,11 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
     uint32_t frag[L::kSubs];
 #pragma unroll
     for (int s = 0; s < L::kSubs; ++s) frag[s] = r * L::kStep + (((2 * s + hh) ^ L::key(r)) << 4);
-    u32x4 fa[2][MT], fb[2][NT];
+    Fragments<T, MT, NT> frags;
     auto read_one = [&](int buf, lds_ptr at_c, lds_ptr at_e, auto which) {
         constexpr int i = decltype(which)::value;
-        if constexpr (i < MT) fa[buf][i] = *(MA_LDS u32x4*)(at_c + (wm + 32 * i) * L::kStep);
-        else fb[buf][i - MT] = *(MA_LDS u32x4*)(at_e + (wn + 32 * (i - MT)) * L::kStep);
+        if constexpr (i < MT) frags.a[buf][i] = *(MA_LDS u32x4*)(at_c + (wm + 32 * i) * L::kStep);
+        else frags.b[buf][i - MT] = *(MA_LDS u32x4*)(at_e + (wn + 32 * (i - MT)) * L::kStep);
     };
     f32x16 acc[MT][NT];
     auto clear = [&]() {
@@ -194,7 +176,7 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
             // the reads in the first half: what the next part begins with has arrived by then
             if constexpr (i < H) static_for<i * R / H, (i + 1) * R / H>([&](auto k) { read_one(buf ^ 1, next_c, next_e, k); });
             else static_for<W0 + (i - H) * W / (P - H), W0 + (i - H + 1) * W / (P - H)>([&](auto k) { load_run(k); });
-            acc[i % MT][i / MT] = Product<T>::mac(fa[buf][i % MT], fb[buf][i / MT], acc[i % MT][i / MT]);
+            frags.template product<i>(buf, acc);
             __builtin_amdgcn_sched_barrier(0);
         });
     };
@@ -332,6 +314,7 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
         asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
         barrier();
         static_for<0, MT + NT>([&](auto k) { read_one(0, smem + frag[0], smem + kSlot + frag[0], k); });
+        frags.begin();
         int slot = 0;                         // of this step's c; e of it and the units after it follow
         const auto slot_at = [](int i) { return (i >= 5 ? i - 5 : i) * kSlot; };
         for (int tile = 0; tile < tiles; ++tile) {
@@ -376,6 +359,7 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
         barrier();
         const auto e_of = [&](lds_ptr c) { return c + kBM * L::kStep; };
         static_for<0, MT + NT>([&](auto k) { read_one(0, smem + frag[0], e_of(smem + frag[0]), k); });
+        frags.begin();
         int stage = 0;
         for (int tile = 0; tile < tiles; ++tile) {
             for (int k = 0; k < ksteps; ++k) {
@@ -450,10 +434,11 @@ __global__ __launch_bounds__(256) void linear_logprobs_join_kernel(const LinArgs
 // with the least of (rounds of 256 workgroups) * (tiles of a range) * (that weight).  Ranges are whole tiles, or for the
 // two narrow blocks, bound by reading c, multiples of 32 so that it is shared out evenly.  Measured at 262208 x 2560 bf16:
 // 48 tokens 248 us in one block of 64 against 309 in two of 32, 384 tokens 549 in three of 128 against 583 in two of 256;
-// at 32003 x 640 fp32, 210 tokens 94 us in two of 128 against 166 in one of 256.
+// at 32003 x 640 fp32, 210 tokens 71 us in two of 128 against 100 in one of 256 and 83 in four of 64, 300 tokens 107 in two of
+// 256 against 118 in five of 64.
 int plan(LinArgs& a, int dtype) {
     constexpr int kWidths[4] = {32, 64, 128, 256};
-    constexpr double kWeight[2][4] = {{0.15, 0.27, 0.51, 1.0}, {0.39, 0.45, 0.58, 1.0}};     // MA_DTYPE_F32, MA_DTYPE_BF16
+    constexpr double kWeight[2][4] = {{0.22, 0.41, 0.60, 1.0}, {0.39, 0.45, 0.58, 1.0}};     // MA_DTYPE_F32, MA_DTYPE_BF16
     constexpr int kUnits = 256;                        // compute units
     const int most = (a.vocab + kBM - 1) / kBM;
     double best = 1e300;

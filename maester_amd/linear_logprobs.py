@@ -159,7 +159,8 @@ def linear_token_logprobs(e: torch.Tensor, c: torch.Tensor, targets: torch.Tenso
     in ``e`` and ``c``.
 
     ``e`` ``[..., K]`` hidden states, ``c`` ``[V, K]`` classifier (Gemma: the tied embedding table), bf16 or fp32 alike,
-    ``K`` a multiple of 8 (fp32: 4); the logits are products of the inputs summed in fp32 and never stored.  ``softcap``,
+    ``K`` a multiple of 8 (fp32: 4); the logits are products of the inputs summed in fp32 and never stored (fp32: an infinity
+    in ``e`` or ``c`` makes them NaN, where bf16 may give an infinity).  ``softcap``,
     ``temperature`` and ignored targets as in ``token_logprobs``.  ``chunk_rows``: rows per block of the backward (default:
     about 4 GiB of gradient of the logits at a time; V is at most 2^21 with gradients).  ``filter_ignored``: a large call
     (more than 256 rows, 2^36 multiply-adds a product; fp32 2^33) drops the rows whose target does not count before any

@@ -175,3 +175,31 @@ def test_beyond_32_bits_of_offset():
     tail = x[-last:].double()
     assert bool((de[:-last] == 0).all()) and torch.equal(de[-last:], (tail @ c.double()).to(torch.bfloat16))
     assert torch.equal(dc, (tail.t().contiguous() @ e[-last:].double()).to(torch.bfloat16))
+
+
+def test_all_bits_of_fp32_operands_count():
+    """Against one-hot rows the products are the other operand's values, 24 bits of them."""
+    rows, vocab, dim = 67, 515, 132
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn(rows, vocab, generator=g) * torch.exp2(torch.randint(-30, 30, (rows, vocab), generator=g).float())
+    pick = torch.randint(0, vocab, (dim,), generator=g)
+    c = torch.zeros(vocab, dim)
+    c[pick, torch.arange(dim)] = 1.0
+    pad = torch.zeros(rows, 520, device=DEV)
+    pad[:, :vocab] = x.to(DEV)
+    e = torch.zeros(rows, dim)
+    e[torch.randint(0, rows, (dim,), generator=g), torch.arange(dim)] = -2.0
+    de, dc = torch.empty(rows, dim, device=DEV), torch.empty(vocab, dim, device=DEV)
+    LL._products(pad, e.to(DEV), c.to(DEV), de, dc, False)
+    assert torch.equal(de.cpu(), x[:, pick])
+    assert torch.equal(dc.cpu(), (x.double().t() @ e.double()).float())
+    # and the other way round: one-hot logits' gradients pick rows of full e and c
+    full_e, full_c = torch.randn(rows, dim, generator=g) * 1e-9, torch.randn(vocab, dim, generator=g) * 1e9
+    x = torch.zeros(rows, vocab)
+    order = torch.randperm(vocab, generator=g)[:rows]
+    x[torch.arange(rows), order] = 1.0
+    pad[:, :vocab] = x.to(DEV)
+    LL._products(pad, full_e.to(DEV), full_c.to(DEV), de, dc, False)
+    want = torch.zeros(vocab, dim)
+    want[order] = full_e
+    assert torch.equal(de.cpu(), full_c[order]) and torch.equal(dc.cpu(), want)

@@ -253,3 +253,34 @@ def test_refusals(gpu):
             linear_token_logprobs(*args, **kw)
     with pytest.raises(RuntimeError):
         linear_token_logprobs(e.cpu(), c.cpu(), t.cpu())
+
+
+def test_infinities_in_fp32(gpu):
+    """An infinity makes NaN of the tokens whose logits it takes part in, and of no others."""
+    e, c = torch.randn(5, 64, device=gpu), torch.randn(300, 64, device=gpu)
+    t = torch.arange(5, device=gpu)
+    want = linear_token_logprobs(e, c, t)
+    for sign in (1.0, -1.0):
+        bad = e.clone()
+        bad[2, 7] = sign * float("inf")
+        for got, ref in zip(linear_token_logprobs(bad, c, t), want):
+            assert bool(torch.isnan(got[2])) and torch.equal(got[[0, 1, 3, 4]], ref[[0, 1, 3, 4]])
+        bad = c.clone()
+        bad[299, 0] = sign * float("inf")
+        assert all(bool(torch.isnan(x).all()) for x in linear_token_logprobs(e, bad, t))
+
+
+def test_fp32_operands_of_any_size(gpu):
+    """24 bits of both operands over 60 binades: against 64 bits of the same values, as the fp32 sum of K products."""
+    torch.manual_seed(5)
+    n, k, v = 70, 132, 515
+    up = torch.exp2(torch.randint(-30, 30, (k,)).float())
+    e, c = (torch.randn(n, k) * up).to(gpu), (torch.randn(v, k) / up).to(gpu)
+    t = torch.randint(0, v, (n,), device=gpu)
+    logp, entropy = linear_token_logprobs(e, c, t)
+    x = e.double() @ c.double().t()
+    size = e.double().abs() @ c.double().abs().t()
+    lse = torch.logsumexp(x, 1)
+    # a logit is off by at most (K + 3) 2^-24 of the sum of its products' sizes, the statistics by some 40 roundings of theirs
+    off = ((k + 3) * 2.0 ** -24 * size).amax(1) * 2 + 40 * 2.0 ** -24 * (x.abs().amax(1) + 10)
+    assert bool(((logp.double() - (x.gather(1, t[:, None])[:, 0] - lse)).abs() <= off).all())
