@@ -205,10 +205,11 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
 
     // this lane's rows of a tile: m0 + row_of(16 i + v) + 4 hh for accumulator i's register v
     auto row_of = [](int i) constexpr { return 32 * (i / 16) + 8 * (i % 16 / 4) + i % 4; };
-    auto finish_tile = [&](int m0, auto is_partial) {
+    auto finish_tile = [&](int m0, auto is_partial) __attribute__((always_inline)) {
         constexpr bool PARTIAL = decltype(is_partial)::value;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
+        // (unrolled by hand where an accumulator is named: past a size the compiler leaves a loop and moves them to memory)
+        static_for<0, NT>([&](auto column) __attribute__((always_inline)) {
+            constexpr int j = decltype(column)::value;
             const int t = target[j] - m0 - 4 * hh;     // the target's row of this tile, if it is one of this lane's
             const bool here = t >= 0 && t < L::kWaveM && (t & 4) == 0 && target[j] >= 0;
             if (!GRAD) {
@@ -242,9 +243,9 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
                 T* out = (T*)a.dlogits + (int64_t)n * a.pitch;
                 // (the row's padding up to the next eight columns is written too, zeros: the products that follow read it)
                 const int m_end = v1 == a.vocab ? (v1 + 7) & ~7 : v1;
-                const auto store = [&](auto is_here) {
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
+                const auto store = [&](auto is_here) __attribute__((always_inline)) {
+                    static_for<0, MT>([&](auto block) __attribute__((always_inline)) {
+                        constexpr int i = decltype(block)::value;
                         // (an accumulator at a time, in the accumulation registers until then)
                         __builtin_amdgcn_sched_barrier(0);
                         asm volatile("" : "+a"(acc[i][j]));
@@ -275,15 +276,15 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
                                 }
                             }
                         }
-                    }
+                    });
                 };
                 if (__any(here)) store(std::true_type{});
                 else store(std::false_type{});
             }
-        }
+        });
     };
 
-    const auto close_tile = [&](int tile) {
+    const auto close_tile = [&](int tile) __attribute__((always_inline)) {
         const int m0 = v0 + tile * kBM + wm;
         if (m0 + L::kWaveM > v1) finish_tile(m0, std::integral_constant<bool, true>{});
         else finish_tile(m0, std::integral_constant<bool, false>{});
