@@ -267,6 +267,7 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
                             }
                             if (n < a.rows && (!PARTIAL || m < m_end)) {
                                 if constexpr (sizeof(T) == 2) {
+                                    // (rounded as the products' instructions take it: the results' own rounding is as large)
                                     bf16x4 o;
 #pragma unroll
                                     for (int v = 0; v < 4; ++v) o[v] = (__bf16)d[v];
