@@ -226,11 +226,13 @@ int ma_token_logprobs_bwd(const void* logits, int64_t pitch, const int64_t* targ
  * workspace: ma_linear_logprobs_workspace_bytes(rows, vocab) bytes, 16-byte aligned.
  * ma_linear_logprobs_dlogits writes d x for the gradients dlogp / dentropy (either may be NULL) into
  * dlogits, rows `pitch` elements apart (a multiple of 8; the padding behind a row up to the next multiple
- * of 8 is written too, with zeros), in dtype, a block of rows at a time, for
- * ma_linear_grads: de [rows, dim] = x c and dc [vocab, dim] = x^T e of x = dlogits, contiguous, either may be
- * NULL (and c or e with it), come in dtype, rounded once; with dc_added dc is fp32 and added to (several
- * blocks of rows).  x is read up to the next multiple of 8 (fp32: 4) columns: the padding has to hold zeros.  workspace: ma_linear_grads_workspace_bytes(...)
- * bytes (0: may be NULL), 16-byte aligned.  Sums in a fixed order. */
+ * of 8 is written too, with zeros), in dtype, a block of rows at a time.  parts 2 (bf16, up to 64 rows):
+ * dlogits has 2 rows rows, n + rows what the rounding of row n left; otherwise 1.
+ * ma_linear_grads: de [rows / parts, dim] = x c, where `parts` rows of x, n, n + rows / parts, ..., make one
+ * of de, and dc [vocab, dim] = x^T e of x = dlogits; contiguous, either may be NULL (and c or e with it),
+ * in dtype, rounded once; with dc_added dc is fp32 and added to (several blocks of rows).  x is read up to
+ * the next multiple of 8 (fp32: 4) columns: the padding has to hold zeros.  workspace:
+ * ma_linear_grads_workspace_bytes(...) bytes (0: may be NULL), 16-byte aligned.  Sums in a fixed order. */
 size_t ma_linear_logprobs_workspace_bytes(int64_t rows, int64_t vocab);
 int ma_linear_logprobs_fwd(const void* e, int64_t e_stride, const void* c, int64_t c_stride, const int64_t* targets, int64_t rows,
                            int64_t vocab, int64_t dim, int64_t ignore_index, float softcap, float temperature, float* logp,
@@ -238,12 +240,12 @@ int ma_linear_logprobs_fwd(const void* e, int64_t e_stride, const void* c, int64
 int ma_linear_logprobs_dlogits(const void* e, int64_t e_stride, const void* c, int64_t c_stride, const int64_t* targets, int64_t rows,
                                int64_t vocab, int64_t dim, int64_t ignore_index, float softcap, float temperature, const float* stats,
                                const float* entropy, const float* dlogp, const float* dentropy, void* dlogits, int64_t pitch,
-                               int dtype, void* stream);
+                               int parts, int dtype, void* stream);
 
-size_t ma_linear_grads_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, int dtype);
+size_t ma_linear_grads_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, int parts, int dtype);
 int ma_linear_grads(const void* x, int64_t x_stride, const void* e, int64_t e_stride, const void* c, int64_t c_stride, int64_t rows,
-                    int64_t vocab, int64_t dim, void* de, void* dc, int dc_added, void* workspace, size_t workspace_bytes, int dtype,
-                    void* stream);
+                    int64_t vocab, int64_t dim, int parts, void* de, void* dc, int dc_added, void* workspace, size_t workspace_bytes,
+                    int dtype, void* stream);
 
 /* ---- AdamW over many tensors ---------------------------------------------------------------------------
  * The step that applies a training step's gradients: AdamW with decoupled weight decay over any number

@@ -118,11 +118,11 @@ def lib() -> ctypes.CDLL:
                                          c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_int, c_void_p]
     L.ma_linear_logprobs_dlogits.restype = c_int
     L.ma_linear_logprobs_dlogits.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64,
-                                             c_float, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]
+                                             c_float, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]
     L.ma_linear_grads_workspace_bytes.restype = c_size_t
-    L.ma_linear_grads_workspace_bytes.argtypes = [c_int64, c_int64, c_int64, c_int]
+    L.ma_linear_grads_workspace_bytes.argtypes = [c_int64, c_int64, c_int64, c_int, c_int]
     L.ma_linear_grads.restype = c_int
-    L.ma_linear_grads.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
+    L.ma_linear_grads.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p,
                                   c_void_p, c_int, c_void_p, c_size_t, c_int, c_void_p]
     L.ma_adamw_workspace_bytes.restype = c_size_t
     L.ma_adamw_workspace_bytes.argtypes = [c_int]

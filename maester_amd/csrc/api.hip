@@ -324,25 +324,27 @@ int ma_linear_logprobs_fwd(const void* e, int64_t e_stride, const void* c, int64
 int ma_linear_logprobs_dlogits(const void* e, int64_t e_stride, const void* c, int64_t c_stride, const int64_t* targets, int64_t rows,
                                int64_t vocab, int64_t dim, int64_t ignore_index, float softcap, float temperature, const float* stats,
                                const float* entropy, const float* dlogp, const float* dentropy, void* dlogits, int64_t pitch,
-                               int dtype, void* stream) {
+                               int parts, int dtype, void* stream) {
     const char* who = "ma_linear_logprobs_dlogits";
     MA_TRY(check_linear_logprobs(who, e, e_stride, c, c_stride, targets, rows, vocab, dim, softcap, temperature, dtype));
     if (!stats || !entropy || !dlogits) return fail(MA_ERR_BAD_ARG, "%s: stats / entropy / dlogits is NULL", who);
     if (((uintptr_t)dlogits & 15) != 0) return fail(MA_ERR_BAD_ARG, "%s: dlogits not 16-byte aligned", who);
     if (pitch % 8 != 0 || pitch < vocab) return fail(MA_ERR_BAD_ARG, "%s: pitch=%lld must be a multiple of 8, at least vocab", who, (long long)pitch);
+    if (parts != 1 && (parts != 2 || dtype != MA_DTYPE_BF16 || rows > kLinearPartsRows))
+        return fail(MA_ERR_BAD_ARG, "%s: parts=%d must be 1, or 2 in bf16 up to %d rows", who, parts, kLinearPartsRows);
     const LinearLogprobsArgs a = {e, c, e_stride, c_stride, targets, rows, vocab, dim, ignore_index, softcap, temperature, nullptr,
-                                  (float*)entropy, (float*)stats, dlogp, dentropy, dlogits, pitch, nullptr};
+                                  (float*)entropy, (float*)stats, dlogp, dentropy, dlogits, pitch, nullptr, parts};
     return launch_linear_logprobs_dlogits(a, dtype, (hipStream_t)stream);
 }
 
-size_t ma_linear_grads_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, int dtype) {
-    if (rows <= 0 || vocab <= 0 || dim <= 0 || (dtype != MA_DTYPE_F32 && dtype != MA_DTYPE_BF16)) return 0;
-    return linear_grads_workspace_bytes(rows, vocab, dim, dtype);
+size_t ma_linear_grads_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, int parts, int dtype) {
+    if (rows <= 0 || vocab <= 0 || dim <= 0 || parts <= 0 || (dtype != MA_DTYPE_F32 && dtype != MA_DTYPE_BF16)) return 0;
+    return linear_grads_workspace_bytes(rows, vocab, dim, parts, dtype);
 }
 
 int ma_linear_grads(const void* x, int64_t x_stride, const void* e, int64_t e_stride, const void* c, int64_t c_stride, int64_t rows,
-                    int64_t vocab, int64_t dim, void* de, void* dc, int dc_added, void* workspace, size_t workspace_bytes, int dtype,
-                    void* stream) {
+                    int64_t vocab, int64_t dim, int parts, void* de, void* dc, int dc_added, void* workspace, size_t workspace_bytes,
+                    int dtype, void* stream) {
     const char* who = "ma_linear_grads";
     MA_TRY(check_dtype(who, dtype));
     const int64_t al = dtype == MA_DTYPE_BF16 ? 8 : 4;
@@ -359,10 +361,12 @@ int ma_linear_grads(const void* x, int64_t x_stride, const void* e, int64_t e_st
     // the rows of a tile (256 of x, 64 of e and c, 256 of the results) are addressed with 31-bit byte offsets
     if (x_stride > MA_LOGPROBS_MAX_GRAD_VOCAB || (de && c_stride > (1 << 20)) || (dc && e_stride > (1 << 20)))
         return fail(MA_ERR_UNSUPPORTED, "%s: row strides above 2^21 (x), 2^20 (e, c) elements", who);
-    const size_t need = de ? linear_grads_workspace_bytes(rows, vocab, dim, dtype) : 0;
+    if (parts < 1 || parts > 8 || rows % parts != 0)
+        return fail(MA_ERR_BAD_ARG, "%s: parts=%d must be in 1 .. 8 and divide rows=%lld", who, parts, (long long)rows);
+    const size_t need = de ? linear_grads_workspace_bytes(rows, vocab, dim, parts, dtype) : 0;
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0))
         return fail(MA_ERR_BAD_ARG, "%s: workspace of %zu bytes, need %zu, 16-byte aligned", who, workspace ? workspace_bytes : (size_t)0, need);
-    const LinearGradsArgs a = {x, e, c, x_stride, e_stride, c_stride, rows, vocab, dim, de, dc, dc_added, workspace};
+    const LinearGradsArgs a = {x, e, c, x_stride, e_stride, c_stride, rows, vocab, dim, de, dc, parts, dc_added, workspace};
     return launch_linear_grads(a, dtype, (hipStream_t)stream);
 }
 

@@ -90,7 +90,9 @@ struct LinearLogprobsArgs {
     void* dlogits;
     int64_t pitch;
     void* ws;
+    int parts;                        // of the gradient in dlogits: 2: row n + rows holds what the rounding of row n left
 };
+constexpr int kLinearPartsRows = 64;          // two parts up to so many rows
 size_t linear_logprobs_workspace_bytes(int64_t rows, int64_t vocab);
 int launch_linear_logprobs_fwd(const LinearLogprobsArgs& a, int dtype, hipStream_t st);
 int launch_linear_logprobs_dlogits(const LinearLogprobsArgs& a, int dtype, hipStream_t st);
@@ -99,10 +101,11 @@ struct LinearGradsArgs {
     const void *x, *e, *c;            // x: gradient of the logits
     int64_t x_stride, e_stride, c_stride, rows, vocab, dim;
     void *de, *dc;                    // either may be NULL
+    int parts;                        // rows of x that make one of de
     int dc_added;                     // dc is fp32 and added to; otherwise it has the operands' type
     void* ws;
 };
-size_t linear_grads_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, int dtype);
+size_t linear_grads_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, int parts, int dtype);
 int launch_linear_grads(const LinearGradsArgs& a, int dtype, hipStream_t st);
 
 struct AdamwArgs {

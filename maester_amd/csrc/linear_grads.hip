@@ -345,13 +345,13 @@ __global__ __launch_bounds__(256, 1) void linear_grads_kernel(const GradArgs a) 
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 }
 
-// de = sum of the ranges' results, rounded once
+// de = sum of the shares of a result (its ranges, its rows' parts), rounded once
 template <typename T>
-__global__ __launch_bounds__(256) void linear_grads_join_kernel(const float* __restrict__ part, int ranges, int64_t n, T* __restrict__ out) {
+__global__ __launch_bounds__(256) void linear_grads_join_kernel(const float* __restrict__ part, int shares, int64_t n, T* __restrict__ out) {
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
     f32x4 v = *(const f32x4*)(part + i);
-    for (int r = 1; r < ranges; ++r) v += *(const f32x4*)(part + (int64_t)r * n + i);
+    for (int r = 1; r < shares; ++r) v += *(const f32x4*)(part + (int64_t)r * n + i);
     if constexpr (sizeof(T) == 4) {
         *(f32x4*)(out + i) = v;
     } else {
@@ -438,12 +438,13 @@ int launch(const LinearGradsArgs& p, hipStream_t st) {
         a.contraction = (int)p.vocab;
         a.range_stride = p.rows * p.dim;
         const Cut how = cut(p.rows, p.dim, steps_of(p.vocab, bf16), bf16, kMostRanges);
-        a.out = how.ranges == 1 ? p.de : p.ws;
-        const int rc = bf16 && how.ranges == 1 ? start_cut<T, false, kInput>(a, how, st) : start_cut<T, false, kStored>(a, how, st);
+        const int shares = how.ranges * p.parts;             // of a result: ranges, and in each the parts' rows
+        a.out = shares == 1 ? p.de : p.ws;
+        const int rc = bf16 && shares == 1 ? start_cut<T, false, kInput>(a, how, st) : start_cut<T, false, kStored>(a, how, st);
         if (rc) return rc;
-        if (how.ranges > 1) {
-            const int64_t n = p.rows * p.dim;
-            linear_grads_join_kernel<T><<<(unsigned)((n / 4 + 255) / 256), 256, 0, st>>>((const float*)p.ws, how.ranges, n, (T*)p.de);
+        if (shares > 1) {
+            const int64_t n = p.rows / p.parts * p.dim;
+            linear_grads_join_kernel<T><<<(unsigned)((n / 4 + 255) / 256), 256, 0, st>>>((const float*)p.ws, shares, n, (T*)p.de);
             const int joined = check_launch("linear_grads_join_kernel");
             if (joined) return joined;
         }
@@ -463,10 +464,10 @@ int launch(const LinearGradsArgs& p, hipStream_t st) {
 
 }  // namespace
 
-size_t linear_grads_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, int dtype) {
+size_t linear_grads_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, int parts, int dtype) {
     const bool bf16 = dtype == MA_DTYPE_BF16;
     const Cut how = cut(rows, dim, steps_of(vocab, bf16), bf16, kMostRanges);
-    return how.ranges == 1 ? 0 : (size_t)how.ranges * rows * dim * sizeof(float);
+    return how.ranges * parts == 1 ? 0 : (size_t)how.ranges * rows * dim * sizeof(float);
 }
 
 int launch_linear_grads(const LinearGradsArgs& p, int dtype, hipStream_t st) {

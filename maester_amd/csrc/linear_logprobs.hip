@@ -47,6 +47,7 @@ struct LinArgs {
     const float *stats, *entropy, *dlogp, *dentropy;   // gradient
     void* dlogits;
     int64_t pitch;                           // elements between its rows
+    int64_t second;                          // elements from a row to what its rounding left (0: not kept)
 };
 
 template <int BN>
@@ -267,11 +268,20 @@ __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a
                             }
                             if (n < a.rows && (!PARTIAL || m < m_end)) {
                                 if constexpr (sizeof(T) == 2) {
-                                    // (rounded as the products' instructions take it: the results' own rounding is as large)
+                                    // Rounded as the products' instructions take it: as large as the results' own rounding, but
+                                    // alike for all results of a row's largest coefficient.  Few rows, among which that does
+                                    // not average out, are kept in two parts (the products are then bound by memory anyway).
                                     bf16x4 o;
 #pragma unroll
                                     for (int v = 0; v < 4; ++v) o[v] = (__bf16)d[v];
                                     *(bf16x4*)(out + m) = o;
+                                    if constexpr (BN <= kLinearPartsRows) {
+                                        if (a.second) {
+#pragma unroll
+                                            for (int v = 0; v < 4; ++v) o[v] = (__bf16)(d[v] - (float)o[v]);
+                                            *(bf16x4*)(out + a.second + m) = o;
+                                        }
+                                    }
                                 } else {
                                     *(float4*)(out + m) = make_float4(d[0], d[1], d[2], d[3]);
                                 }
@@ -534,6 +544,10 @@ int launch_linear_logprobs_dlogits(const LinearLogprobsArgs& p, int dtype, hipSt
     a.dentropy = p.dentropy;
     a.dlogits = p.dlogits;
     a.pitch = p.pitch;
+    if (p.parts == 2) {
+        if (width > kLinearPartsRows) return fail(MA_ERR_UNSUPPORTED, "linear_logprobs: two parts of %d rows", a.rows);
+        a.second = p.rows * p.pitch;
+    }
     return by_type<true>(a, width, dtype, st);
 }
 

@@ -60,22 +60,28 @@ def linear_token_logprobs_forward(e, c, targets, ignore_index=-100, softcap=None
 
 
 def _dlogits(e, c, targets, stats, entropy, dlogp, dentropy, ignore_index, softcap, temperature, out):
-    """Gradient of the logits of a block of rows into ``out`` ``[rows, pitch]``."""
+    """Gradient of the logits of a block of rows into ``out`` ``[rows, pitch]`` (``[2 rows, pitch]``: with what the rounding left)."""
     _lib.launch(e.device, _lib.lib().ma_linear_logprobs_dlogits, _lib.ptr(e), _pitch(e), _lib.ptr(c), _pitch(c), _lib.ptr(targets),
                 e.shape[0], c.shape[0], e.shape[1], int(ignore_index), softcap, temperature, _lib.ptr(stats), _lib.ptr(entropy),
-                _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.ptr(out), out.shape[1], _lib.dtype_code(e.dtype))
+                _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.ptr(out), out.shape[1], out.shape[0] // e.shape[0], _lib.dtype_code(e.dtype))
 
 
+# Up to so many rows a bf16 gradient of the logits is kept in two parts of bf16: its rounding is the same for all results of a
+# row's largest coefficient and does not average out among so few (the gradients' error is up to 2.5 times that of rounding
+# them alone).  The products of so few rows are bound by memory: 2560 x 262208, 8 rows 798 -> 838 us, 64 rows 872 -> 975; 128
+# rows would take 1168 for 983.
+_TWO_PARTS_TO = 64
 MAX_GRAD_VOCAB = 1 << 21                    # ma_linear_grads addresses 256 rows of the logits' gradient with 31 bits
 
 
-def _products(x, e, c, de, dc, add):
-    """``de = x c`` and ``dc = x^T e`` (``add``: added to an fp32 ``dc``), either may be None; the rows of ``x`` are padded."""
+def _products(x, e, c, de, dc, add, parts=1):
+    """``de = x c`` (sums of ``parts`` rows of ``x``) and ``dc = x^T e`` (``add``: added to an fp32 ``dc``), either may be None;
+    the rows of ``x`` are padded."""
     L, code = _lib.lib(), _lib.dtype_code(e.dtype)
-    ws_bytes = 0 if de is None else L.ma_linear_grads_workspace_bytes(e.shape[0], c.shape[0], e.shape[1], code)
+    ws_bytes = 0 if de is None else L.ma_linear_grads_workspace_bytes(x.shape[0], c.shape[0], e.shape[1], parts, code)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=e.device) if ws_bytes else None
-    _lib.launch(e.device, L.ma_linear_grads, x.data_ptr(), x.shape[1], e.data_ptr(), _pitch(e), c.data_ptr(), _pitch(c), e.shape[0],
-                c.shape[0], e.shape[1], _lib.ptr(de), _lib.ptr(dc), int(add), _lib.ptr(ws), ws_bytes,
+    _lib.launch(e.device, L.ma_linear_grads, x.data_ptr(), x.shape[1], e.data_ptr(), _pitch(e), c.data_ptr(), _pitch(c), x.shape[0],
+                c.shape[0], e.shape[1], parts, _lib.ptr(de), _lib.ptr(dc), int(add), _lib.ptr(ws), ws_bytes,
                 code)
 
 
@@ -92,20 +98,23 @@ def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentrop
         return de, torch.zeros(vocab, k, dtype=c.dtype, device=c.device) if need_dc else None
     step = int(chunk_rows) if chunk_rows else default_chunk_rows(vocab, e.element_size(), n)
     step = max(1, min(step, n))
-    block = torch.empty(step, -(-vocab // 8) * 8, dtype=e.dtype, device=e.device)
+    parts = 2 if e.dtype == torch.bfloat16 and step <= _TWO_PARTS_TO else 1
+    block = torch.empty(parts * step, -(-vocab // 8) * 8, dtype=e.dtype, device=e.device)
     # several blocks: dc is summed in fp32 and rounded once at the end
     dc = None
     if need_dc:
         dc = torch.empty(vocab, k, dtype=c.dtype, device=c.device) if n <= step else torch.zeros(vocab, k, dtype=torch.float32, device=c.device)
     for r0 in range(0, n, step):
         whole, rows = n <= step, slice(r0, min(n, r0 + step))
-        buf = block[: rows.stop - r0]
+        buf = block[: parts * (rows.stop - r0)]
         e_rows, rest = e, (targets, stats, entropy, dlogp, dentropy)
         if not whole:
             e_rows, rest = e[rows], (None if t is None else t[rows] for t in rest)
         _dlogits(e_rows, c, *rest, ignore_index, softcap, temperature, buf)
         if need_de or need_dc:
-            _products(buf, e_rows, c, de if whole or de is None else de[rows], dc, not whole)
+            if parts > 1:
+                e_rows = torch.cat((e_rows, e_rows))
+            _products(buf, e_rows, c, de if whole or de is None else de[rows], dc, not whole, parts)
     return de, dc.to(c.dtype) if need_dc else None
 
 

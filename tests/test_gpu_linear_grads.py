@@ -117,11 +117,11 @@ def test_refusals():
         LL._products(xd.view(-1)[1:65].view(4, 16), ed, cd[:16], de, None, False)
     L = _lib.lib()
     with pytest.raises((RuntimeError, ValueError), match="workspace"):
-        need = L.ma_linear_grads_workspace_bytes(8, 40000, 64, _lib.dtype_code(torch.float32))
+        need = L.ma_linear_grads_workspace_bytes(8, 40000, 64, 1, _lib.dtype_code(torch.float32))
         assert need > 0
         x, e, c = torch.zeros(8, 40000, device=DEV), torch.zeros(8, 64, device=DEV), torch.zeros(40000, 64, device=DEV)
         out = torch.empty(8, 64, device=DEV)
-        _lib.launch(x.device, L.ma_linear_grads, x.data_ptr(), 40000, e.data_ptr(), 64, c.data_ptr(), 64, 8, 40000, 64, out.data_ptr(), None, 0,
+        _lib.launch(x.device, L.ma_linear_grads, x.data_ptr(), 40000, e.data_ptr(), 64, c.data_ptr(), 64, 8, 40000, 64, 1, out.data_ptr(), None, 0,
                     None, 0, _lib.dtype_code(torch.float32))
     meta = torch.empty(LL.MAX_GRAD_VOCAB + 1, 8, device=DEV, dtype=torch.bfloat16).requires_grad_()
     with pytest.raises(ValueError, match="vocabularies"):
@@ -203,3 +203,24 @@ def test_all_bits_of_fp32_operands_count():
     want = torch.zeros(vocab, dim)
     want[order] = full_e
     assert torch.equal(de.cpu(), full_c[order]) and torch.equal(dc.cpu(), want)
+
+
+@pytest.mark.parametrize("rows,chunk", [(1, None), (2, None), (5, 3), (33, None), (64, None), (100, 50)])
+def test_gradients_of_few_bf16_rows_are_rounded_once(rows, chunk):
+    """Up to 64 rows at a time the gradient of the logits counts with 16 bits: what is left is the results' own rounding."""
+    vocab, dim, g = 1003, 64, torch.Generator().manual_seed(rows)
+    e = torch.randn(rows, dim, generator=g).to(torch.bfloat16)
+    c = (torch.randn(vocab, dim, generator=g) * 3 / 8).to(torch.bfloat16)
+    targets = torch.randint(0, vocab, (rows,), generator=g)
+    a, b = torch.randn(rows, generator=g), 0.1 * torch.randn(rows, generator=g)
+    ed, cd = e.to(DEV).requires_grad_(), c.to(DEV).requires_grad_()
+    out = LL.linear_token_logprobs(ed, cd, targets.to(DEV), chunk_rows=chunk)
+    de, dc = torch.autograd.grad(out, (ed, cd), (a.to(DEV), b.to(DEV)))
+    lp = torch.log_softmax(e.double() @ c.double().t(), 1)
+    p, h = lp.exp(), -(lp.exp() * lp).sum(1, keepdim=True)
+    x = -p * (b[:, None].double() * (lp + h) + a[:, None].double())
+    x[torch.arange(rows), targets] += a.double()
+    for got, want, size in ((de, x @ c.double(), x.abs() @ c.double().abs()), (dc, x.t() @ e.double(), x.t().abs() @ e.double().abs())):
+        # 2^-8 of the result; of its terms 2^-16 (the second part's rounding) and p's error, that of a logit: (K + 3) 2^-24 of
+        # the sizes of its 64 products (some ten in all), with the factor of the entropy's gradient: 2^-13 together
+        assert bool(((got.double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -13 * size).all())

@@ -77,12 +77,13 @@ def test_linear_forward_refusals(kw, code, text):
     assert _lin(**kw) == code and text in _lib.lib().ma_last_error().decode()
 
 
-def _dlogits(e=P, es=64, c=P, cs=64, targets=P, rows=4, vocab=100, dim=64, cap=0.0, temp=1.0, stats=P, out=P, pitch=104, dtype=1):
-    return _lib.lib().ma_linear_logprobs_dlogits(e, es, c, cs, targets, rows, vocab, dim, -100, cap, temp, stats, P, P, P, out, pitch, dtype, None)
+def _dlogits(e=P, es=64, c=P, cs=64, targets=P, rows=4, vocab=100, dim=64, cap=0.0, temp=1.0, stats=P, out=P, pitch=104, parts=1, dtype=1):
+    return _lib.lib().ma_linear_logprobs_dlogits(e, es, c, cs, targets, rows, vocab, dim, -100, cap, temp, stats, P, P, P, out, pitch, parts, dtype, None)
 
 
 @pytest.mark.parametrize("kw,code,text", LINEAR + [(dict(stats=None), -1, "stats"), (dict(out=P + 8), -1, "aligned"), (dict(pitch=100), -1, "pitch"),
-                                                   (dict(pitch=96), -1, "pitch")])
+                                                   (dict(pitch=96), -1, "pitch"), (dict(parts=0), -1, "parts"), (dict(parts=3), -1, "parts"),
+                                                   (dict(parts=2, rows=65), -1, "parts"), (dict(parts=2, dtype=0), -1, "parts")])
 def test_linear_gradient_refusals(kw, code, text):
     assert _dlogits(**kw) == code and text in _lib.lib().ma_last_error().decode()
 
@@ -94,8 +95,8 @@ def test_linear_workspace():
     assert L.ma_linear_logprobs_workspace_bytes(8, 262208) == 32 + 256 * 8 * 12
 
 
-def _grads(x=P, xs=304, e=P, es=64, c=P, cs=64, rows=9, vocab=300, dim=64, de=P, dc=P, add=0, ws=P, ws_bytes=1 << 20, dtype=1):
-    return _lib.lib().ma_linear_grads(x, xs, e, es, c, cs, rows, vocab, dim, de, dc, add, ws, ws_bytes, dtype, None)
+def _grads(x=P, xs=304, e=P, es=64, c=P, cs=64, rows=9, vocab=300, dim=64, parts=1, de=P, dc=P, add=0, ws=P, ws_bytes=1 << 20, dtype=1):
+    return _lib.lib().ma_linear_grads(x, xs, e, es, c, cs, rows, vocab, dim, parts, de, dc, add, ws, ws_bytes, dtype, None)
 
 
 @pytest.mark.parametrize("kw,code,text", [
@@ -104,7 +105,8 @@ def _grads(x=P, xs=304, e=P, es=64, c=P, cs=64, rows=9, vocab=300, dim=64, de=P,
     (dict(dim=60, es=64, cs=64), -2, "dim"), (dict(dim=1 << 17, es=1 << 17, cs=1 << 17), -2, "dim"), (dict(xs=300), -1, "strides"),
     (dict(xs=296), -1, "strides"), (dict(es=56), -1, "strides"), (dict(cs=68), -1, "strides"), (dict(xs=(1 << 21) + 8), -2, "2^21"),
     (dict(vocab=1 << 22, xs=1 << 22), -2, "2^21"), (dict(es=(1 << 20) + 8), -2, "2^20"), (dict(dtype=7), -1, "dtype"),
-    (dict(vocab=40000, xs=40000, ws=None), -1, "workspace"), (dict(vocab=40000, xs=40000, ws_bytes=16), -1, "workspace"),
+    (dict(parts=0), -1, "parts"), (dict(parts=2), -1, "parts"), (dict(rows=18, parts=9), -1, "parts"),
+    (dict(rows=8, vocab=64, parts=2, ws=None), -1, "workspace"), (dict(vocab=40000, xs=40000, ws=None), -1, "workspace"), (dict(vocab=40000, xs=40000, ws_bytes=16), -1, "workspace"),
     (dict(vocab=40000, xs=40000, ws=P + 8), -1, "workspace")])
 def test_gradient_products_refuse(kw, code, text):
     assert _grads(**kw) == code and text in _lib.lib().ma_last_error().decode()
@@ -112,7 +114,8 @@ def test_gradient_products_refuse(kw, code, text):
 
 def test_workspace_of_the_gradient_products():
     L = _lib.lib()
-    assert L.ma_linear_grads_workspace_bytes(0, 100, 64, 1) == 0 and L.ma_linear_grads_workspace_bytes(9, 64, 64, 1) == 0
+    assert L.ma_linear_grads_workspace_bytes(0, 100, 64, 1, 1) == 0 and L.ma_linear_grads_workspace_bytes(9, 64, 64, 1, 1) == 0
+    assert L.ma_linear_grads_workspace_bytes(10, 64, 64, 2, 1) == 10 * 64 * 4
     for rows, vocab, dim, dtype in ((9, 40000, 64, 1), (2047, 262208, 2560, 1), (210, 32003, 640, 0), (1 << 20, 32003, 640, 1)):
-        need = L.ma_linear_grads_workspace_bytes(rows, vocab, dim, dtype)
+        need = L.ma_linear_grads_workspace_bytes(rows, vocab, dim, 1, dtype)
         assert need % (rows * dim * 4) == 0 and need // (rows * dim * 4) <= 128
