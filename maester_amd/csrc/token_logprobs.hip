@@ -92,11 +92,10 @@ __device__ __forceinline__ LpStats workgroup_stats(LpStats t, float inv_temp, Lp
 
 // ---- order of the alternatives ------------------------------------------------------------------------
 // A candidate is one 64-bit key, unique in its row: the logit's bits made monotone above, the complement
-// of the index below, so that larger is better and equal logits go to the lower index.  -0 equals +0,
-// NaN ranks with -inf.  0 is no key.
+// of the index below, so that larger is better and equal logits go to the lower index.  -0 equals +0 (made
+// so on the bits: the build's math flags drop an addition of 0), NaN ranks with -inf.  0 is no key.
 __device__ __forceinline__ uint32_t ordered(float x) {
-    x = x == x ? x + 0.f : -INFINITY;
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t a = __float_as_uint(x == x ? x : -INFINITY), b = a == 0x80000000u ? 0u : a;
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
