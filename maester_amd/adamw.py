@@ -120,7 +120,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     steps below 2^-9 of the weight.  ``max_grad_norm``: the gradients are scaled by ``min(1, max_grad_norm / (norm + 1e-6))``
     with the global norm of this call's, which is returned as an fp32 scalar on the device; ``clip``: an fp32 factor on the
     device to scale by instead.  A gradient that is not finite makes its element (8-bit states: its block of 128) NaN, or
-    all of them through the norm.  ``seed`` picks the random bits of the 8-bit rounding."""
+    all of them through the norm.  ``seed`` picks the random bits of the 8-bit rounding.  All that is written counts as modified
+in place (a backward through a graph that saved it before the step raises)."""
     n = len(params)
     masters = [None] * n if masters is None else masters
     if not len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(masters) == n:
@@ -169,6 +170,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
                 lr.data_ptr() if on_device else None, float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
                 -1.0 if max_grad_norm is None else float(max_grad_norm), None if clip is None else clip.data_ptr(),
                 None if norm is None else norm.data_ptr(), step.data_ptr(), int(seed), ws.data_ptr(), ws_bytes)
+    # the kernels write behind autograd's back: a graph that saved one of these before the step has to raise
+    states = [t for q in (*exp_avgs, *exp_avg_sqs) for t in q] if eight else [*exp_avgs, *exp_avg_sqs]
+    torch.autograd.graph.increment_version([*params, *states, *(masters[i] for i in held), step])
     return norm
 
 
