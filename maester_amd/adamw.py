@@ -11,6 +11,7 @@ stochastically from a hash of (seed, step, index of the tensor, element): the sa
 """
 from __future__ import annotations
 
+import warnings
 from operator import attrgetter
 from typing import NamedTuple, Sequence
 
@@ -176,6 +177,19 @@ in place (a backward through a graph that saved it before the step raises)."""
     return norm
 
 
+def _check_torchs(group: dict, states: list) -> None:
+    """Refuses what ``torch.optim.AdamW`` has not saved, or what its options make another update."""
+    if not {"betas", "eps", "weight_decay", "amsgrad"} <= set(group) or any(not {"step", "exp_avg", "exp_avg_sq"} <= set(s) or
+                                                                            set(s) - {"step", "exp_avg", "exp_avg_sq", "max_exp_avg_sq"} for s in states):
+        raise ValueError("not a state of torch.optim.AdamW: its groups have betas, eps, weight_decay and amsgrad, its parameters step, "
+                         "exp_avg and exp_avg_sq")
+    for option in ("maximize", "amsgrad"):
+        if group.get(option):
+            raise ValueError(f"a state saved with {option} cannot be continued: AdamW here has no such option")
+    if not group.get("decoupled_weight_decay", True) and group["weight_decay"] != 0:
+        raise ValueError("a state whose weight decay is not decoupled (torch.optim.Adam's) cannot be continued")
+
+
 class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW``'s update (same defaults) through ``adamw_step``.
 
@@ -251,14 +265,22 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict: dict) -> None:
         """Restores the states in the types they were saved in (torch's own would cast them to the parameter's).  A state of
         ``torch.optim.AdamW`` is taken over into 32-bit states; its per-parameter counters become the group's, the largest
-        of them."""
-        super().load_state_dict(state_dict)
+        of them (with a warning where they differ).  One with ``maximize``, ``amsgrad`` or a weight decay that is not decoupled,
+        or of another optimizer, is refused before anything changes."""
         saved = state_dict["state"]
+        for old in state_dict["param_groups"]:
+            if "state_bits" not in old:
+                _check_torchs(old, [saved[i] for i in old["params"] if i in saved])
+        super().load_state_dict(state_dict)
         for old, group in zip(state_dict["param_groups"], self.param_groups):
             foreign = "state_bits" not in old
             if foreign:
-                group.update(state_bits=32, master_weights=self.defaults["master_weights"], seed=self.defaults["seed"])
-                group["step"] = max((int(saved[i]["step"]) for i in old["params"] if i in saved), default=0)
+                steps = {int(saved[i]["step"]) for i in old["params"] if i in saved}
+                if len(steps) > 1:
+                    warnings.warn(f"parameters of one group have taken between {min(steps)} and {max(steps)} steps: all continue with the "
+                                  f"bias correction of step {max(steps)}", stacklevel=2)
+                group.update(state_bits=32, master_weights=self.defaults["master_weights"], seed=self.defaults["seed"],
+                             step=max(steps, default=0))
             for i, p in zip(old["params"], group["params"]):
                 if i not in saved:
                     continue
