@@ -266,7 +266,8 @@ class AdamW(torch.optim.Optimizer):
         """Restores the states in the types they were saved in (torch's own would cast them to the parameter's).  A state of
         ``torch.optim.AdamW`` is taken over into 32-bit states; its per-parameter counters become the group's, the largest
         of them (with a warning where they differ).  One with ``maximize``, ``amsgrad`` or a weight decay that is not decoupled,
-        or of another optimizer, is refused before anything changes."""
+        or of another optimizer, is refused before anything changes.  Counters and rates that are tensors move to the
+        parameters' device.  All tensors are new ones: a graph that captured ``step()`` has to be captured again."""
         saved = state_dict["state"]
         for old in state_dict["param_groups"]:
             if "state_bits" not in old:
@@ -281,6 +282,11 @@ class AdamW(torch.optim.Optimizer):
                                   f"bias correction of step {max(steps)}", stacklevel=2)
                 group.update(state_bits=32, master_weights=self.defaults["master_weights"], seed=self.defaults["seed"],
                              step=max(steps, default=0))
+            dev = group["params"][0].device
+            if "step" in group:
+                group["step"] = torch.as_tensor(group["step"]).to(dev, torch.int64)
+            if isinstance(group["lr"], torch.Tensor):
+                group["lr"] = group["lr"].detach().to(dev, torch.float32)
             for i, p in zip(old["params"], group["params"]):
                 if i not in saved:
                     continue

@@ -7,6 +7,8 @@ import torch
 
 from maester_amd import AdamW
 
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
 
 def _trained(kind=torch.optim.AdamW, steps=(3, 3), device="cpu", **kw):
     """A state of ``kind`` over two parameters after so many steps of each."""
@@ -56,3 +58,23 @@ def test_counters_that_differ_are_said():
     with pytest.warns(UserWarning, match="bias correction"):
         ours.load_state_dict(state)
     assert int(ours.param_groups[0]["step"]) == 5
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_rate_on_the_host_moves_to_the_parameters(device):
+    # torch takes a rate as a tensor on the host; map_location="cpu" brings one of ours there too
+    for state in (_trained(device=device, lr=torch.tensor(0.25), foreach=False)[1], None):
+        params, ours = _ours(device, lr=torch.tensor(0.25, device=device))
+        if state is None:
+            state = copy.deepcopy(ours.state_dict())
+            state["param_groups"][0]["lr"] = torch.tensor(0.25, dtype=torch.float64)
+            state["param_groups"][0]["step"] = torch.tensor(3)
+        ours.load_state_dict(state)
+        group = ours.param_groups[0]
+        assert group["lr"].device == params[0].device and group["lr"].dtype == torch.float32 and float(group["lr"]) == 0.25
+        assert group["step"].device == params[0].device and group["step"].dtype == torch.int64 and int(group["step"]) == 3
+        if device == "cuda":
+            for p in params:
+                p.grad = torch.ones_like(p)
+            ours.step()
+            assert int(group["step"]) == 4 and bool((params[0] < 1).all())
