@@ -177,6 +177,19 @@ in place (a backward through a graph that saved it before the step raises)."""
     return norm
 
 
+def _check_options(o: dict) -> None:
+    """The options of a group, by name: a wrong one would show first in a step, after the states have been made."""
+    lr, betas, eps, decay, seed = o["lr"], o["betas"], o["eps"], o["weight_decay"], o["seed"]
+    if o["state_bits"] not in (32, 8):
+        raise ValueError(f"state_bits must be 32 or 8, got {o['state_bits']}")
+    if not isinstance(lr, torch.Tensor) and not float(lr) >= 0:
+        raise ValueError(f"lr must be >= 0, got {lr}")
+    if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0 and decay >= 0):
+        raise ValueError(f"betas {betas}, eps {eps} or weight_decay {decay} out of range")
+    if not 0 <= int(seed) < 1 << 32:
+        raise ValueError(f"seed must be in [0, 2^32), got {seed}")
+
+
 def _check_torchs(group: dict, states: list) -> None:
     """Refuses what ``torch.optim.AdamW`` has not saved, or what its options make another update."""
     if not {"betas", "eps", "weight_decay", "amsgrad"} <= set(group) or any(not {"step", "exp_avg", "exp_avg_sq"} <= set(s) or
@@ -202,18 +215,18 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, master_weights: bool = False,
                  max_grad_norm: float | None = None, seed: int = 0):
-        if state_bits not in (32, 8):
-            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
-        if not isinstance(lr, torch.Tensor) and not float(lr) >= 0:
-            raise ValueError(f"lr must be >= 0, got {lr}")
-        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0 and weight_decay >= 0):
-            raise ValueError(f"betas {betas}, eps {eps} or weight_decay {weight_decay} out of range")
         if max_grad_norm is not None and not float(max_grad_norm) >= 0:
             raise ValueError(f"max_grad_norm must be >= 0, got {max_grad_norm}")
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
-                                      master_weights=master_weights, seed=seed))
+        options = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                       master_weights=master_weights, seed=seed)
+        _check_options(options)
+        super().__init__(params, options)
         self.max_grad_norm = max_grad_norm
         self.grad_norm = None
+
+    def add_param_group(self, param_group: dict) -> None:
+        _check_options({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     def _init_state(self, p: torch.Tensor, group: dict) -> dict:
         state = {}
@@ -270,7 +283,9 @@ class AdamW(torch.optim.Optimizer):
         parameters' device.  All tensors are new ones: a graph that captured ``step()`` has to be captured again."""
         saved = state_dict["state"]
         for old in state_dict["param_groups"]:
-            if "state_bits" not in old:
+            if "state_bits" in old:
+                _check_options(old)
+            else:
                 _check_torchs(old, [saved[i] for i in old["params"] if i in saved])
         super().load_state_dict(state_dict)
         for old, group in zip(state_dict["param_groups"], self.param_groups):

@@ -78,3 +78,12 @@ def test_a_rate_on_the_host_moves_to_the_parameters(device):
                 p.grad = torch.ones_like(p)
             ours.step()
             assert int(group["step"]) == 4 and bool((params[0] < 1).all())
+
+
+@pytest.mark.parametrize("bits", [16, 0, None])
+def test_a_state_of_ours_with_unknown_bits(bits):
+    _, ours = _ours()
+    state = copy.deepcopy(ours.state_dict())
+    state["param_groups"][0]["state_bits"] = bits
+    with pytest.raises(ValueError, match="state_bits"):
+        ours.load_state_dict(state)
