@@ -10,6 +10,7 @@ import os
 from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p)
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmaester_attn.so")
 
@@ -198,6 +199,12 @@ def launch(dev: torch.device, fn, *args) -> None:
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc != MA_OK:
         check(rc)
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor) -> None:
+    """Kernels called outside of autograd would drop a tangent; inside of it ``Function.apply`` refuses it the same way."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def require_gpu(t: torch.Tensor, what: str) -> None:

@@ -94,6 +94,7 @@ def global_grad_norm(grads: Sequence[torch.Tensor], max_norm: float | None = Non
     grads = list(grads)
     if not grads:
         raise ValueError("no gradients")
+    _lib.refuse_tangents("global_grad_norm", *grads)
     if max_norm is not None and not float(max_norm) >= 0:
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
     dev = _device(grads, "global_grad_norm")
@@ -133,6 +134,7 @@ in place (a backward through a graph that saved it before the step raises)."""
         raise ValueError("max_grad_norm must be >= 0 and cannot be given together with clip")
     if not 0 <= int(seed) < 1 << 32:
         raise ValueError("seed must be in [0, 2^32)")
+    _lib.refuse_tangents("adamw_step", *params, *grads)
     dev = _device(params, "adamw_step")
     kinds = set(map(type, exp_avgs)) | set(map(type, exp_avg_sqs))
     eight = Blocks8 in kinds
