@@ -201,10 +201,20 @@ def launch(dev: torch.device, fn, *args) -> None:
         check(rc)
 
 
+_PLAIN = {torch.Tensor, torch.nn.Parameter}
+
+
 def refuse_tangents(what: str, *tensors: torch.Tensor) -> None:
     """Kernels called outside of autograd would drop a tangent; inside of it ``Function.apply`` refuses it the same way."""
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
+def require_plain(what: str, *tensors) -> None:
+    """Refuses tensors that wrap others (``DTensor`` and the like): they have no memory of their own to hand to a kernel."""
+    for kind in set(map(type, tensors)) - _PLAIN:
+        if hasattr(kind, "__tensor_flatten__"):
+            raise TypeError(f"{what} takes plain tensors, got {kind.__name__} (of a sharded tensor: its local part)")
 
 
 def require_gpu(t: torch.Tensor, what: str) -> None:

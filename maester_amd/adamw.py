@@ -94,6 +94,7 @@ def global_grad_norm(grads: Sequence[torch.Tensor], max_norm: float | None = Non
     grads = list(grads)
     if not grads:
         raise ValueError("no gradients")
+    _lib.require_plain("global_grad_norm", *grads)
     _lib.refuse_tangents("global_grad_norm", *grads)
     if max_norm is not None and not float(max_norm) >= 0:
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
@@ -134,6 +135,7 @@ in place (a backward through a graph that saved it before the step raises)."""
         raise ValueError("max_grad_norm must be >= 0 and cannot be given together with clip")
     if not 0 <= int(seed) < 1 << 32:
         raise ValueError("seed must be in [0, 2^32)")
+    _lib.require_plain("adamw_step", *params, *grads, *exp_avgs, *exp_avg_sqs, *masters)
     _lib.refuse_tangents("adamw_step", *params, *grads)
     dev = _device(params, "adamw_step")
     kinds = set(map(type, exp_avgs)) | set(map(type, exp_avg_sqs))
@@ -192,6 +194,17 @@ def _check_options(o: dict) -> None:
         raise ValueError(f"seed must be in [0, 2^32), got {seed}")
 
 
+def _check_params(params: list) -> None:
+    """What a step would refuse, before their states take memory."""
+    _lib.require_plain("AdamW", *params)
+    for p in params:
+        if p.dtype not in _ACTIVATION:
+            raise TypeError(f"a parameter must be {' or '.join(sorted(map(str, _ACTIVATION)))}, got {p.dtype}")
+        if not p.is_contiguous():
+            raise ValueError(f"a parameter must be contiguous, got {tuple(p.shape)} with strides {p.stride()}")
+    _device(params, "AdamW")
+
+
 def _check_torchs(group: dict, states: list) -> None:
     """Refuses what ``torch.optim.AdamW`` has not saved, or what its options make another update."""
     if not {"betas", "eps", "weight_decay", "amsgrad"} <= set(group) or any(not {"step", "exp_avg", "exp_avg_sq"} <= set(s) or
@@ -229,6 +242,11 @@ class AdamW(torch.optim.Optimizer):
     def add_param_group(self, param_group: dict) -> None:
         _check_options({**self.defaults, **param_group})
         super().add_param_group(param_group)
+        try:
+            _lib.require_plain("AdamW", *self.param_groups[-1]["params"])
+        except TypeError:
+            self.param_groups.pop()
+            raise
 
     def _init_state(self, p: torch.Tensor, group: dict) -> dict:
         state = {}
@@ -252,9 +270,11 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             params = [p for p in group["params"] if p.grad is not None]
             if params:
-                for p in params:
-                    if not self.state[p]:
-                        self.state[p].update(self._init_state(p, group))
+                fresh = [p for p in params if not self.state.get(p)]
+                if fresh:
+                    _check_params(fresh)
+                    for p in fresh:
+                        self.state[p] = self._init_state(p, group)
                 if not isinstance(group.get("step"), torch.Tensor) or group["step"].device != params[0].device:
                     group["step"] = torch.as_tensor(group.get("step", 0), dtype=torch.int64).to(params[0].device)
                 work.append((group, params, [p.grad.contiguous() for p in params]))

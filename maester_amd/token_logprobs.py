@@ -115,6 +115,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
     ``logp`` and ``entropy`` are differentiable in the logits (once), the alternatives are not."""
     if logits.dim() < 1 or targets.shape != logits.shape[:-1]:
         raise ValueError(f"targets shape {tuple(targets.shape)} != leading shape of logits {tuple(logits.shape[:-1])}")
+    _lib.require_plain("token_logprobs", logits, targets)
     _lib.refuse_tangents("token_logprobs", logits)
     lead, vocab = targets.shape, logits.shape[-1]
     if vocab < 1:
