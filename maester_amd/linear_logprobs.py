@@ -47,7 +47,7 @@ def linear_token_logprobs_forward(e, c, targets, ignore_index=-100, softcap=None
     softcap, temperature = check_softmax_arguments(softcap, temperature)
     e, c, targets = _rows_in_place(e), _rows_in_place(c), targets.contiguous()
     n, vocab = e.shape[0], c.shape[0]
-    logp, entropy = torch.empty(2, n, dtype=torch.float32, device=e.device).unbind()
+    logp, entropy = (torch.empty(n, dtype=torch.float32, device=e.device) for _ in range(2))
     stats = torch.empty(n, 2, dtype=torch.float32, device=e.device)
     if n:
         L = _lib.lib()
@@ -138,7 +138,8 @@ class _LinearTokenLogprobsFn(torch.autograd.Function):
         if keep is not None:
             e, targets = e.index_select(0, keep), targets.index_select(0, keep)
         logp, entropy, stats = linear_token_logprobs_forward(e, c, targets, ignore_index, softcap, temperature)
-        ctx.save_for_backward(e, c, targets, stats, entropy, keep)
+        # (the caller may edit the outputs: spread ones are copies, others share no memory with what is saved)
+        ctx.save_for_backward(e, c, targets, stats, entropy.clone() if keep is None else entropy, keep)
         ctx.args = (ignore_index, softcap, temperature, chunk_rows)
         ctx.set_materialize_grads(False)
         return _spread(logp, keep, ctx.rows), _spread(entropy, keep, ctx.rows)

@@ -49,7 +49,7 @@ def token_logprobs_forward(logits, targets, top_k=0, ignore_index=-100, softcap=
     softcap, temperature = check_softmax_arguments(softcap, temperature)
     code = _lib.dtype_code(logits.dtype)
     targets = targets.contiguous()
-    logp, entropy = torch.empty(2, rows, dtype=torch.float32, device=dev).unbind()
+    logp, entropy = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2))
     stats = torch.empty(rows, 2, dtype=torch.float32, device=dev) if need_stats else None
     top_ids = torch.empty(rows, top_k, dtype=torch.int64, device=dev) if top_k else None
     top_logp = torch.empty(rows, top_k, dtype=torch.float32, device=dev) if top_k else None
@@ -87,7 +87,7 @@ class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top_k, ignore_index, softcap, temperature):
         logp, entropy, stats, top_ids, top_logp = token_logprobs_forward(logits, targets, top_k, ignore_index, softcap, temperature)
-        ctx.save_for_backward(logits, targets, stats, entropy)
+        ctx.save_for_backward(logits, targets, stats, entropy.clone())       # (the caller may edit the output)
         ctx.args = (ignore_index, softcap, temperature)
         ctx.set_materialize_grads(False)
         if top_k:
