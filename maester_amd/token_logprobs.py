@@ -129,5 +129,5 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
     if len(lead) != 1:
         logp, entropy = logp.view(lead), entropy.view(lead)
         if top_ids is not None:
-            top_ids, top_logp = top_ids.view(*lead, -1), top_logp.view(*lead, -1)
+            top_ids, top_logp = (x.view(*lead, x.shape[1]) for x in (top_ids, top_logp))
     return TokenLogprobs(logp, entropy, top_ids, top_logp)
