@@ -232,7 +232,10 @@ int ma_token_logprobs_bwd(const void* logits, int64_t pitch, const int64_t* targ
  * of de, and dc [vocab, dim] = x^T e of x = dlogits; contiguous, either may be NULL (and c or e with it),
  * in dtype, rounded once; with dc_added dc is fp32 and added to (several blocks of rows).  x is read up to
  * the next multiple of 8 (fp32: 4) columns: the padding has to hold zeros.  workspace:
- * ma_linear_grads_workspace_bytes(...) bytes (0: may be NULL), 16-byte aligned.  Sums in a fixed order. */
+ * ma_linear_grads_workspace_bytes(...) bytes (0: may be NULL), 16-byte aligned.  Sums in a fixed order.
+ * ma_linear_counted_rows copies e for dc: out [copies rows, dim], contiguous, row n (and n + rows, ...) that of e, or
+ * zeros where target n does not count: its row of x is 0, but 0 times a NaN or an infinity would be NaN.  copies
+ * is ma_linear_grads' parts. */
 size_t ma_linear_logprobs_workspace_bytes(int64_t rows, int64_t vocab);
 int ma_linear_logprobs_fwd(const void* e, int64_t e_stride, const void* c, int64_t c_stride, const int64_t* targets, int64_t rows,
                            int64_t vocab, int64_t dim, int64_t ignore_index, float softcap, float temperature, float* logp,
@@ -246,6 +249,9 @@ size_t ma_linear_grads_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim,
 int ma_linear_grads(const void* x, int64_t x_stride, const void* e, int64_t e_stride, const void* c, int64_t c_stride, int64_t rows,
                     int64_t vocab, int64_t dim, int parts, void* de, void* dc, int dc_added, void* workspace, size_t workspace_bytes,
                     int dtype, void* stream);
+
+int ma_linear_counted_rows(const void* e, int64_t e_stride, const int64_t* targets, int64_t rows, int64_t vocab, int64_t dim,
+                           int64_t ignore_index, int copies, void* out, int dtype, void* stream);
 
 /* ---- AdamW over many tensors ---------------------------------------------------------------------------
  * The step that applies a training step's gradients: AdamW with decoupled weight decay over any number

@@ -30,7 +30,7 @@ MA_ADAMW_BLOCK = 128
 MA_BWD_DELTA, MA_BWD_DKV, MA_BWD_DQ, MA_BWD_ALL = 1, 2, 4, 7
 
 EXPORTS = (
-    "ma_version", "ma_last_error", "ma_probe_mfma", "ma_tile_map_workspace_bytes", "ma_tile_map_build", "ma_tile_map_build_static", "ma_packed_ids_build", "ma_rmsnorm_bwd_workspace_bytes", "ma_rmsnorm_fwd", "ma_rmsnorm_bwd", "ma_ce_valid_count", "ma_ce_rows", "ma_ce_loss_reduce", "ma_transpose", "ma_token_logprobs_workspace_bytes", "ma_token_logprobs_fwd", "ma_token_logprobs_bwd", "ma_linear_logprobs_workspace_bytes", "ma_linear_logprobs_fwd", "ma_linear_logprobs_dlogits", "ma_linear_grads_workspace_bytes", "ma_linear_grads", "ma_adamw_workspace_bytes", "ma_adamw_step", "ma_grad_norm", "ma_prologue_fwd",
+    "ma_version", "ma_last_error", "ma_probe_mfma", "ma_tile_map_workspace_bytes", "ma_tile_map_build", "ma_tile_map_build_static", "ma_packed_ids_build", "ma_rmsnorm_bwd_workspace_bytes", "ma_rmsnorm_fwd", "ma_rmsnorm_bwd", "ma_ce_valid_count", "ma_ce_rows", "ma_ce_loss_reduce", "ma_transpose", "ma_token_logprobs_workspace_bytes", "ma_token_logprobs_fwd", "ma_token_logprobs_bwd", "ma_linear_logprobs_workspace_bytes", "ma_linear_logprobs_fwd", "ma_linear_logprobs_dlogits", "ma_linear_grads_workspace_bytes", "ma_linear_grads", "ma_linear_counted_rows", "ma_adamw_workspace_bytes", "ma_adamw_step", "ma_grad_norm", "ma_prologue_fwd",
     "ma_prologue_bwd_workspace_bytes", "ma_prologue_bwd", "ma_attn_fwd", "ma_attn_bwd_workspace_bytes", "ma_attn_bwd_ds_workspace_bytes",
     "ma_attn_bwd", "ma_attn_bwd_stages",
 )
@@ -125,6 +125,8 @@ def lib() -> ctypes.CDLL:
     L.ma_linear_grads.restype = c_int
     L.ma_linear_grads.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p,
                                   c_void_p, c_int, c_void_p, c_size_t, c_int, c_void_p]
+    L.ma_linear_counted_rows.restype = c_int
+    L.ma_linear_counted_rows.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_void_p]
     L.ma_adamw_workspace_bytes.restype = c_size_t
     L.ma_adamw_workspace_bytes.argtypes = [c_int]
     L.ma_adamw_step.restype = c_int

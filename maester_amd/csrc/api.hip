@@ -370,6 +370,23 @@ int ma_linear_grads(const void* x, int64_t x_stride, const void* e, int64_t e_st
     return launch_linear_grads(a, dtype, (hipStream_t)stream);
 }
 
+int ma_linear_counted_rows(const void* e, int64_t e_stride, const int64_t* targets, int64_t rows, int64_t vocab, int64_t dim,
+                           int64_t ignore_index, int copies, void* out, int dtype, void* stream) {
+    const char* who = "ma_linear_counted_rows";
+    MA_TRY(check_dtype(who, dtype));
+    const int64_t al = dtype == MA_DTYPE_BF16 ? 8 : 4;
+    if (!e || !targets || !out) return fail(MA_ERR_BAD_ARG, "%s: e / targets / out is NULL", who);
+    if ((((uintptr_t)e | (uintptr_t)out) & 15) != 0) return fail(MA_ERR_BAD_ARG, "%s: e / out not 16-byte aligned", who);
+    // a wave a row: a launch has fewer than 2^32 threads
+    if (rows <= 0 || rows >= ((int64_t)1 << 26)) return fail(MA_ERR_BAD_ARG, "%s: rows=%lld must be in 1 .. 2^26 - 1", who, (long long)rows);
+    if (vocab <= 0 || vocab > MA_LOGPROBS_MAX_VOCAB) return fail(MA_ERR_BAD_ARG, "%s: vocab=%lld out of range", who, (long long)vocab);
+    if (dim <= 0 || dim % al != 0 || dim > 65536)
+        return fail(MA_ERR_UNSUPPORTED, "%s: dim=%lld must be a multiple of %lld, at most 65536", who, (long long)dim, (long long)al);
+    if (e_stride < dim || e_stride % al) return fail(MA_ERR_BAD_ARG, "%s: e_stride=%lld must be a multiple of %lld elements, at least dim", who, (long long)e_stride, (long long)al);
+    if (copies < 1 || copies > 8) return fail(MA_ERR_BAD_ARG, "%s: copies=%d must be in 1 .. 8", who, copies);
+    return launch_linear_counted_rows(e, e_stride, targets, rows, vocab, dim, ignore_index, copies, out, dtype, (hipStream_t)stream);
+}
+
 size_t ma_adamw_workspace_bytes(int count) { return count < 0 ? 0 : adamw_workspace_bytes(count); }
 
 static int check_adamw(const char* who, const ma_adamw_tensor* tensors, int count, int state_bits, double max_norm, const void* workspace,

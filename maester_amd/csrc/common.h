@@ -107,6 +107,8 @@ struct LinearGradsArgs {
 };
 size_t linear_grads_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, int parts, int dtype);
 int launch_linear_grads(const LinearGradsArgs& a, int dtype, hipStream_t st);
+int launch_linear_counted_rows(const void* e, int64_t e_stride, const int64_t* targets, int64_t rows, int64_t vocab, int64_t dim,
+                               int64_t ignore_index, int copies, void* out, int dtype, hipStream_t st);
 
 struct AdamwArgs {
     const ma_adamw_tensor* list;      // host memory

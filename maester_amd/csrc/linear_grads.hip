@@ -362,6 +362,21 @@ __global__ __launch_bounds__(256) void linear_grads_join_kernel(const float* __r
     }
 }
 
+// e's rows as the contraction over them takes them: zeros for a token that does not count, since its x is 0 but its hidden
+// state may be anything, and 0 * NaN is NaN; `copies` times, one for each part of x.  A wave a row, 16 bytes a lane.
+__global__ __launch_bounds__(256) void linear_counted_rows_kernel(const char* __restrict__ e, int64_t stride, const int64_t* __restrict__ targets,
+                                                                  int64_t rows, int64_t vocab, int64_t ignore_index, int bytes, int copies,
+                                                                  char* __restrict__ out) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int64_t target = targets[row];
+    const bool valid = target != ignore_index && target >= 0 && target < vocab;
+    for (int at = (threadIdx.x & 63) * 16; at < bytes; at += 64 * 16) {
+        const u32x4 v = valid ? *(const u32x4*)(e + row * stride + at) : u32x4{0, 0, 0, 0};
+        for (int c = 0; c < copies; ++c) *(u32x4*)(out + (c * rows + row) * bytes + at) = v;
+    }
+}
+
 template <typename T, bool X_ROWS, Output OUT, int BM, int BN>
 int start(const GradArgs& a, hipStream_t st) {
     auto kernel = linear_grads_kernel<T, X_ROWS, OUT == kInput && sizeof(T) == 4 ? kStored : OUT, BM, BN>;
@@ -468,6 +483,14 @@ size_t linear_grads_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, in
     const bool bf16 = dtype == MA_DTYPE_BF16;
     const Cut how = cut(rows, dim, steps_of(vocab, bf16), bf16, kMostRanges);
     return how.ranges * parts == 1 ? 0 : (size_t)how.ranges * rows * dim * sizeof(float);
+}
+
+int launch_linear_counted_rows(const void* e, int64_t e_stride, const int64_t* targets, int64_t rows, int64_t vocab, int64_t dim,
+                               int64_t ignore_index, int copies, void* out, int dtype, hipStream_t st) {
+    const int elt = dtype == MA_DTYPE_BF16 ? 2 : 4;
+    linear_counted_rows_kernel<<<(unsigned)((rows + 3) / 4), 256, 0, st>>>((const char*)e, e_stride * elt, targets, rows, vocab, ignore_index,
+                                                                           (int)dim * elt, copies, (char*)out);
+    return check_launch("linear_counted_rows_kernel");
 }
 
 int launch_linear_grads(const LinearGradsArgs& p, int dtype, hipStream_t st) {

@@ -85,9 +85,18 @@ def _products(x, e, c, de, dc, add, parts=1):
                 code)
 
 
+def _counted_rows(e, targets, vocab, ignore_index, copies):
+    """``copies`` copies of ``e``, one after the other, with zeros for the rows that do not count."""
+    out = torch.empty(copies * e.shape[0], e.shape[1], dtype=e.dtype, device=e.device)
+    _lib.launch(e.device, _lib.lib().ma_linear_counted_rows, _lib.ptr(e), _pitch(e), _lib.ptr(targets), e.shape[0], vocab, e.shape[1],
+                int(ignore_index), copies, _lib.ptr(out), _lib.dtype_code(e.dtype))
+    return out
+
+
 def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentropy, ignore_index=-100, softcap=None,
-                                   temperature=1.0, chunk_rows=None, need_de=True, need_dc=True):
-    """``(de, dc)`` (None where not needed) from the gradients of ``logp`` and ``entropy`` (either may be None)."""
+                                   temperature=1.0, chunk_rows=None, need_de=True, need_dc=True, all_count=False):
+    """``(de, dc)`` (None where not needed) from the gradients of ``logp`` and ``entropy`` (either may be None).
+    ``all_count``: every target is known to count, so that ``dc`` may take the rows of ``e`` as they are."""
     softcap, temperature = check_softmax_arguments(softcap, temperature)
     e, c, targets = _rows_in_place(e), _rows_in_place(c), targets.contiguous()
     dlogp, dentropy = (None if t is None else t.float().contiguous() for t in (dlogp, dentropy))
@@ -109,11 +118,11 @@ def linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentrop
         buf = block[: parts * (rows.stop - r0)]
         e_rows, rest = e, (targets, stats, entropy, dlogp, dentropy)
         if not whole:
-            e_rows, rest = e[rows], (None if t is None else t[rows] for t in rest)
+            e_rows, rest = e[rows], tuple(None if t is None else t[rows] for t in rest)
         _dlogits(e_rows, c, *rest, ignore_index, softcap, temperature, buf)
         if need_de or need_dc:
-            if parts > 1:
-                e_rows = torch.cat((e_rows, e_rows))
+            if need_dc and (parts > 1 or not all_count):
+                e_rows = _counted_rows(e_rows, rest[0], vocab, ignore_index, parts)
             _products(buf, e_rows, c, de if whole or de is None else de[rows], dc, not whole, parts)
     return de, dc.to(c.dtype) if need_dc else None
 
@@ -133,8 +142,8 @@ def _kept_rows(targets, ignore_index, vocab):
 
 class _LinearTokenLogprobsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, e, c, targets, ignore_index, softcap, temperature, chunk_rows, keep):
-        ctx.rows = e.shape[0]
+    def forward(ctx, e, c, targets, ignore_index, softcap, temperature, chunk_rows, keep, all_count):
+        ctx.rows, ctx.all_count = e.shape[0], all_count
         if keep is not None:
             e, targets = e.index_select(0, keep), targets.index_select(0, keep)
         logp, entropy, stats = linear_token_logprobs_forward(e, c, targets, ignore_index, softcap, temperature)
@@ -148,13 +157,13 @@ class _LinearTokenLogprobsFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dlogp, dentropy):
         if dlogp is None and dentropy is None:
-            return (None,) * 8
+            return (None,) * 9
         e, c, targets, stats, entropy, keep = ctx.saved_tensors
         if keep is not None:
             dlogp, dentropy = (None if t is None else t.index_select(0, keep) for t in (dlogp, dentropy))
         de, dc = linear_token_logprobs_backward(e, c, targets, stats, entropy, dlogp, dentropy, *ctx.args,
-                                                ctx.needs_input_grad[0], ctx.needs_input_grad[1])
-        return None if de is None else _spread(de, keep, ctx.rows), dc, None, None, None, None, None, None
+                                                ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.all_count)
+        return None if de is None else _spread(de, keep, ctx.rows), dc, None, None, None, None, None, None, None
 
 
 def _spread(x, keep, rows):
@@ -185,11 +194,11 @@ def linear_token_logprobs(e: torch.Tensor, c: torch.Tensor, targets: torch.Tenso
     _check(e, c, targets)
     if c.shape[0] > MAX_GRAD_VOCAB and torch.is_grad_enabled() and (e.requires_grad or c.requires_grad):
         raise ValueError(f"gradients for vocabularies up to {MAX_GRAD_VOCAB}, got V={c.shape[0]}")
-    keep = None
+    keep, all_count = None, False
     if filter_ignored and e.shape[0] >= _FILTER_FROM and e.numel() * c.shape[0] >= _FILTER_WORK[e.dtype] and not torch.cuda.is_current_stream_capturing():
-        keep = _kept_rows(targets, ignore_index, c.shape[0])
+        keep, all_count = _kept_rows(targets, ignore_index, c.shape[0]), True
     if torch.is_grad_enabled() and (e.requires_grad or c.requires_grad):
-        logp, entropy = _LinearTokenLogprobsFn.apply(e, c, targets, int(ignore_index), softcap, temperature, chunk_rows, keep)
+        logp, entropy = _LinearTokenLogprobsFn.apply(e, c, targets, int(ignore_index), softcap, temperature, chunk_rows, keep, all_count)
     else:
         if keep is not None:
             e, targets = e.index_select(0, keep), targets.index_select(0, keep)
