@@ -47,7 +47,7 @@ extern "C" {
 /* Version of this header (major*10000 + minor*100 + patch).  It changes whenever a struct or a
  * signature below changes; ma_version() returns the value the library was built with, and a caller
  * built against another header must not go on (its ma_tile_map has another layout). */
-#define MA_ABI_VERSION 10200
+#define MA_ABI_VERSION 10300
 int ma_version(void);
 
 /* Message describing the last error returned to the calling thread ("" if none). */

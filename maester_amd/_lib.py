@@ -14,7 +14,7 @@ from torch.autograd import forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmaester_attn.so")
 
-MA_ABI_VERSION = 10200   # include/maester_attn.h: the struct layouts and signatures bound below
+MA_ABI_VERSION = 10300   # include/maester_attn.h: the struct layouts and signatures bound below
 MA_OK = 0
 MA_ERR_BAD_ARG = -1
 MA_ERR_UNSUPPORTED = -2
