@@ -1,7 +1,9 @@
-// fp32 products on the bf16 matrix instructions.  An fp32 value is the exact sum of three bf16 values, x = h + m + l: its
-// first 8 mantissa bits, the next 8 and the last 8 (cut off, not rounded, so all three have the sign of x).  Of the nine
-// products of two such sums six are formed, h h + m m, h m + m h and h l + l h; what is left out is below 2^-23 of the
-// product and 2^-25 on average, a rounding of fp32.  Products are exact and summed in fp32, as with the fp32 instructions.
+// fp32 products on the bf16 matrix instructions.  An fp32 value is the exact sum of three bf16 values, x = h + m + l, the first
+// two rounded to the nearest: |m| <= 2^-8 |x|, |l| <= 2^-16 |x|, of either sign.  Of the nine products of two such sums six are
+// formed, h h + m m, h m + m h and h l + l h; what is left out, m l + l m + l l, is at most 2^-23 of the product (a last place
+// of fp32) and 0 on average.  (Cut off instead of rounded, the parts are as cheap, but all have the sign of x and are twice as
+// large: up to 2^-21 were left out and 2^-24.6 on average, always towards zero.)  Products are exact and summed in fp32, as with
+// the fp32 instructions.
 //
 // v_mfma_f32_32x32x16_bf16 takes 8 values a lane: the four values of an fp32 fragment fill it with two of the six products,
 // so a fragment pair is three instructions (96 cycles) where v_mfma_f32_32x32x2_f32 needs four of 64 (256), and the sums
@@ -9,7 +11,9 @@
 // unit works on earlier ones.  Measured (us, before and after): 2048 x 32000, 4096 rows, statistics 3821 -> 2379 (226 TFLOP/s);
 // 640 x 32003, 300 rows, statistics and gradients 520 -> 407, their error against 64 bits 9.2e-7 -> 7.3e-7 of their size.
 //
-// An infinity has no parts: it makes NaN of the sums that it takes part in.  Parts below 2^-126 may count as zero.
+// An infinity has no parts: it makes NaN of the sums that it takes part in, and so does a magnitude that rounds to one in bf16,
+// above 2^128 (1 - 2^-9) = 3.396e38.  Parts below 2^-126 may count as zero: values below 2^-103 may lose their last bits, below
+// 2^-110 their third part, below 2^-118 the second.
 #pragma once
 
 #include "mfma.h"
@@ -23,14 +27,19 @@ struct SplitB {
     u32x4 hm, mh, lh;
 };
 
+__device__ __forceinline__ uint32_t nearest_pair(float x0, float x1) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 p = __builtin_convertvector(f32x2{x0, x1}, bf16x2);
+    return *(const uint32_t*)&p;
+}
 __device__ __forceinline__ void split_pair(uint32_t x0, uint32_t x1, uint32_t& h, uint32_t& m, uint32_t& l) {
-    constexpr uint32_t kHigh = 0xffff0000u, kHalves = 0x07060302u;       // the upper halves of two words
-    const float r0 = __uint_as_float(x0) - __uint_as_float(x0 & kHigh), r1 = __uint_as_float(x1) - __uint_as_float(x1 & kHigh);
-    const uint32_t u0 = __float_as_uint(r0), u1 = __float_as_uint(r1);
-    const float s0 = r0 - __uint_as_float(u0 & kHigh), s1 = r1 - __uint_as_float(u1 & kHigh);
-    h = __builtin_amdgcn_perm(x1, x0, kHalves);
-    m = __builtin_amdgcn_perm(u1, u0, kHalves);
-    l = __builtin_amdgcn_perm(__float_as_uint(s1), __float_as_uint(s0), kHalves);
+    h = nearest_pair(__uint_as_float(x0), __uint_as_float(x1));
+    const float r0 = __uint_as_float(x0) - __uint_as_float(h << 16), r1 = __uint_as_float(x1) - __uint_as_float(h & 0xffff0000u);
+    m = nearest_pair(r0, r1);
+    // (what is left has 8 bits: its upper half is all of it)
+    const float s0 = r0 - __uint_as_float(m << 16), s1 = r1 - __uint_as_float(m & 0xffff0000u);
+    l = __builtin_amdgcn_perm(__float_as_uint(s1), __float_as_uint(s0), 0x07060302u);
 }
 __device__ __forceinline__ SplitA split_a(u32x4 x) {
     uint32_t h[2], m[2], l[2];
