@@ -1,9 +1,9 @@
-// fp32 products on the bf16 matrix instructions.  An fp32 value is the exact sum of three bf16 values, x = h + m + l, the first
-// two rounded to the nearest: |m| <= 2^-8 |x|, |l| <= 2^-16 |x|, of either sign.  Of the nine products of two such sums six are
-// formed, h h + m m, h m + m h and h l + l h; what is left out, m l + l m + l l, is at most 2^-23 of the product (a last place
-// of fp32) and 0 on average.  (Cut off instead of rounded, the parts are as cheap, but all have the sign of x and are twice as
-// large: up to 2^-21 were left out and 2^-24.6 on average, always towards zero.)  Products are exact and summed in fp32, as with
-// the fp32 instructions.
+// fp32 products on the bf16 matrix instructions.  An fp32 value is the exact sum of three bf16 values, x = h + m + l: its first
+// 8 mantissa bits, cut off; the next 8, rounded to the nearest; what is left.  |m| <= 2^-7 |x| and |l| <= 2^-16 |x|, l of either
+// sign.  Of the nine products of two such sums six are formed, h h + m m, h m + m h and h l + l h; what is left out, m l + l m +
+// l l, is at most 2^-22 of the product and 0 on average.  Products are exact and summed in fp32, as with the fp32 instructions.
+// (With m cut off too, l has the sign of x and is twice as large: up to 2^-21 were left out, 2^-24.6 on average and always towards
+// zero.  With h rounded as well 2^-23 are left out, but fp32's largest magnitudes have no h, unless it is clamped: 3 % of the time.)
 //
 // v_mfma_f32_32x32x16_bf16 takes 8 values a lane: the four values of an fp32 fragment fill it with two of the six products,
 // so a fragment pair is three instructions (96 cycles) where v_mfma_f32_32x32x2_f32 needs four of 64 (256), and the sums
@@ -11,9 +11,9 @@
 // unit works on earlier ones.  Measured (us, before and after): 2048 x 32000, 4096 rows, statistics 3821 -> 2379 (226 TFLOP/s);
 // 640 x 32003, 300 rows, statistics and gradients 520 -> 407, their error against 64 bits 9.2e-7 -> 7.3e-7 of their size.
 //
-// An infinity has no parts: it makes NaN of the sums that it takes part in, and so does a magnitude that rounds to one in bf16,
-// above 2^128 (1 - 2^-9) = 3.396e38.  Parts below 2^-126 may count as zero: values below 2^-103 may lose their last bits, below
-// 2^-110 their third part, below 2^-118 the second.
+// Magnitudes up to fp32's largest have parts (a product above 2^128 (1 - 2^-17) may overflow, as h + m may round up to 2^128).
+// An infinity has none: it makes NaN of the sums that it takes part in.  Parts below 2^-126 may count as zero: values below
+// 2^-103 may lose their last bits, below 2^-110 their third part, below 2^-118 the second.
 #pragma once
 
 #include "mfma.h"
@@ -34,12 +34,13 @@ __device__ __forceinline__ uint32_t nearest_pair(float x0, float x1) {
     return *(const uint32_t*)&p;
 }
 __device__ __forceinline__ void split_pair(uint32_t x0, uint32_t x1, uint32_t& h, uint32_t& m, uint32_t& l) {
-    h = nearest_pair(__uint_as_float(x0), __uint_as_float(x1));
-    const float r0 = __uint_as_float(x0) - __uint_as_float(h << 16), r1 = __uint_as_float(x1) - __uint_as_float(h & 0xffff0000u);
+    constexpr uint32_t kHigh = 0xffff0000u, kHalves = 0x07060302u;       // the upper halves of two words
+    const float r0 = __uint_as_float(x0) - __uint_as_float(x0 & kHigh), r1 = __uint_as_float(x1) - __uint_as_float(x1 & kHigh);
+    h = __builtin_amdgcn_perm(x1, x0, kHalves);
     m = nearest_pair(r0, r1);
-    // (what is left has 8 bits: its upper half is all of it)
-    const float s0 = r0 - __uint_as_float(m << 16), s1 = r1 - __uint_as_float(m & 0xffff0000u);
-    l = __builtin_amdgcn_perm(__float_as_uint(s1), __float_as_uint(s0), 0x07060302u);
+    // (8 bits: the upper halves are all there is)
+    const float s0 = r0 - __uint_as_float(m << 16), s1 = r1 - __uint_as_float(m & kHigh);
+    l = __builtin_amdgcn_perm(__float_as_uint(s1), __float_as_uint(s0), kHalves);
 }
 __device__ __forceinline__ SplitA split_a(u32x4 x) {
     uint32_t h[2], m[2], l[2];
