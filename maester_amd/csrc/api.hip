@@ -234,7 +234,9 @@ static int check_logprobs(const char* who, const void* logits, int64_t pitch, co
     if (rows >= ((int64_t)1 << 23)) return fail(MA_ERR_UNSUPPORTED, "%s: rows=%lld is 2^23 or more", who, (long long)rows);
     if (vocab <= 0 || vocab > MA_LOGPROBS_MAX_VOCAB) return fail(MA_ERR_BAD_ARG, "%s: vocab=%lld out of range", who, (long long)vocab);
     if (pitch < vocab) return fail(MA_ERR_BAD_ARG, "%s: pitch=%lld is below vocab=%lld", who, (long long)pitch, (long long)vocab);
-    if (!(softcap >= 0.f) || softcap > 1e30f) return fail(MA_ERR_BAD_ARG, "%s: softcap must be >= 0 (0 = none) and finite", who);
+    // (its reciprocal is taken in fp32)
+    if (softcap != 0.f && !(softcap >= 1e-30f && softcap <= 1e30f))
+        return fail(MA_ERR_BAD_ARG, "%s: softcap must be 0 (none) or in [1e-30, 1e30]", who);
     if (!(temperature > 1e-6f) || temperature > 1e6f) return fail(MA_ERR_BAD_ARG, "%s: temperature must be in (1e-6, 1e6]", who);
     if (((uintptr_t)logits & (dtype == MA_DTYPE_BF16 ? 1 : 3)) != 0)
         return fail(MA_ERR_BAD_ARG, "%s: logits not aligned to its element size", who);
@@ -297,7 +299,9 @@ static int check_linear_logprobs(const char* who, const void* e, int64_t e_strid
                     (long long)c_stride, (long long)al);
     // the rows of a 256-row tile are addressed with 31-bit byte offsets
     if (e_stride > (1 << 20) || c_stride > (1 << 20)) return fail(MA_ERR_UNSUPPORTED, "%s: row strides above 2^20 elements", who);
-    if (!(softcap >= 0.f) || softcap > 1e30f) return fail(MA_ERR_BAD_ARG, "%s: softcap must be >= 0 (0 = none) and finite", who);
+    // (its reciprocal is taken in fp32)
+    if (softcap != 0.f && !(softcap >= 1e-30f && softcap <= 1e30f))
+        return fail(MA_ERR_BAD_ARG, "%s: softcap must be 0 (none) or in [1e-30, 1e30]", who);
     if (!(temperature > 1e-6f) || temperature > 1e6f) return fail(MA_ERR_BAD_ARG, "%s: temperature must be in (1e-6, 1e6]", who);
     return MA_OK;
 }

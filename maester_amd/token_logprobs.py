@@ -26,8 +26,8 @@ class TokenLogprobs(NamedTuple):
 def check_softmax_arguments(softcap, temperature) -> tuple[float, float]:
     """(softcap, 0.0 for none; temperature) as the library takes them."""
     softcap = 0.0 if softcap is None else float(softcap)
-    if not 0.0 <= softcap <= 1e30:
-        raise ValueError(f"softcap must be positive and finite, or None, got {softcap}")
+    if softcap != 0.0 and not 1e-30 <= softcap <= 1e30:      # (the kernels take its reciprocal in fp32)
+        raise ValueError(f"softcap must be in [1e-30, 1e30], or None, got {softcap}")
     if not 1e-6 < float(temperature) <= 1e6:
         raise ValueError(f"temperature must be in (1e-6, 1e6], got {temperature}")
     return softcap, float(temperature)

@@ -1,0 +1,25 @@
+"""Arguments of the log-probabilities at the ends of their ranges, before any launch (no GPU)."""
+import pytest
+import torch
+
+from maester_amd import _lib, gemma_layers, linear_token_logprobs
+from maester_amd.gemma_layers import GemmaLayerConfig, GemmaTextModel
+from maester_amd.token_logprobs import check_softmax_arguments
+
+P = 0x1000
+
+
+@pytest.mark.parametrize("cap", [1e-50, 1e-45, 1e-39, 9e-31, 2e30, float("inf"), float("nan"), -1e-3])
+def test_caps_whose_reciprocal_fp32_cannot_hold(cap):
+    with pytest.raises(ValueError, match="softcap"):
+        check_softmax_arguments(cap, 1.0)
+    if abs(cap) > 1e-46 or cap != cap:                      # (a float argument of 1e-50 is 0, no cap)
+        L = _lib.lib()
+        assert L.ma_token_logprobs_fwd(P, 10, P, 1, 10, -100, cap, 1.0, 0, P, P, None, None, None, P, 1 << 20, 0, None) == -1
+        assert "softcap" in L.ma_last_error().decode()
+        assert L.ma_linear_logprobs_fwd(P, 64, P, 64, P, 1, 10, 64, -100, cap, 1.0, P, P, P, P, 1 << 20, 0, None) == -1
+        assert "softcap" in L.ma_last_error().decode()
+
+
+def test_caps_in_range():
+    assert [check_softmax_arguments(c, 1.0)[0] for c in (None, 0, 0.0, 1e-30, 30, 1e30)] == [0.0, 0.0, 0.0, 1e-30, 30.0, 1e30]
