@@ -186,6 +186,8 @@ def linear_token_logprobs(e: torch.Tensor, c: torch.Tensor, targets: torch.Tenso
     product, which costs its one host synchronisation; not under graph capture."""
     if e.dim() < 1 or targets.shape != e.shape[:-1]:
         raise ValueError(f"targets shape {tuple(targets.shape)} != leading shape of e {tuple(e.shape[:-1])}")
+    if chunk_rows is not None and int(chunk_rows) < 0:
+        raise ValueError(f"chunk_rows must be positive, or None, got {chunk_rows}")
     _lib.require_plain("linear_token_logprobs", e, c, targets)
     _lib.refuse_tangents("linear_token_logprobs", e, c)
     lead = targets.shape

@@ -23,3 +23,9 @@ def test_caps_whose_reciprocal_fp32_cannot_hold(cap):
 
 def test_caps_in_range():
     assert [check_softmax_arguments(c, 1.0)[0] for c in (None, 0, 0.0, 1e-30, 30, 1e30)] == [0.0, 0.0, 0.0, 1e-30, 30.0, 1e30]
+
+
+@pytest.mark.parametrize("chunk", [-1, -300])
+def test_negative_blocks(chunk):
+    with pytest.raises(ValueError, match="chunk_rows"):
+        linear_token_logprobs(torch.zeros(4, 16), torch.zeros(8, 16), torch.zeros(4, dtype=torch.long), chunk_rows=chunk)
