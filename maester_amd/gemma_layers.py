@@ -148,9 +148,12 @@ class GemmaTextModel(nn.Module):
         return torch.matmul(hidden_states, weight.t())
 
     def token_logprobs(self, tokens: torch.Tensor, labels: torch.Tensor, position_ids=None, document_ids=None,
-                       temperature: float = 1.0):
+                       temperature: float = 1.0, *, ignore_index: int = -100, softcap: float | None = None,
+                       chunk_rows: int | None = None, filter_ignored: bool = True):
         """``(logp, entropy)``, fp32 ``[B, S]``: the log-probability of every label (aligned as ``forward`` takes them, -100
         ignored: 0 there) and the entropy of its position, differentiable, without the logits: what a policy, preference
-        or distillation objective and the scoring of a packed batch start from."""
+        or distillation objective and the scoring of a packed batch start from.  The arguments are
+        ``linear_token_logprobs``'s; ``filter_ignored=False`` leaves out its host synchronisation."""
         hidden_states = self._hidden_states(tokens, position_ids, document_ids)
-        return linear_token_logprobs(hidden_states, self.tok_embeddings.weight, labels, temperature=temperature)
+        return linear_token_logprobs(hidden_states, self.tok_embeddings.weight, labels, ignore_index=ignore_index, softcap=softcap,
+                                     temperature=temperature, chunk_rows=chunk_rows, filter_ignored=filter_ignored)

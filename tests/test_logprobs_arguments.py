@@ -29,3 +29,21 @@ def test_caps_in_range():
 def test_negative_blocks(chunk):
     with pytest.raises(ValueError, match="chunk_rows"):
         linear_token_logprobs(torch.zeros(4, 16), torch.zeros(8, 16), torch.zeros(4, dtype=torch.long), chunk_rows=chunk)
+
+
+def test_the_model_hands_its_arguments_on(monkeypatch):
+    config = GemmaLayerConfig(dim=256, n_heads=4, num_key_value_heads=2, head_dim=128, max_seq_len=64, sliding_window_size=64,
+                              intermediate_size=64, n_layers=1, attn_types=("global",), vocab_size=40)
+    with torch.device("meta"):
+        model = GemmaTextModel(config)
+    seen = []
+    monkeypatch.setattr(gemma_layers, "linear_token_logprobs", lambda *a, **kw: seen.append((a, kw)))
+    monkeypatch.setattr(model, "_hidden_states", lambda tokens, pos, doc: (tokens, pos, doc))
+    model.token_logprobs(1, 2, 3, 4)
+    model.token_logprobs(1, 2, 3, 4, temperature=0.5, softcap=30.0, ignore_index=0, chunk_rows=64, filter_ignored=False)
+    model.token_logprobs(1, 2, 3, 4, 0.7)
+    weight = model.tok_embeddings.weight
+    defaults = dict(ignore_index=-100, softcap=None, temperature=1.0, chunk_rows=None, filter_ignored=True)
+    assert [(a[0], a[1] is weight, a[2]) for a, _ in seen] == [((1, 3, 4), True, 2)] * 3
+    assert [kw for _, kw in seen] == [defaults, dict(ignore_index=0, softcap=30.0, temperature=0.5, chunk_rows=64, filter_ignored=False),
+                                      {**defaults, "temperature": 0.7}]
