@@ -55,21 +55,6 @@ __device__ __forceinline__ int tensor_of(const Batch& b, int chunk) {
     return lo;
 }
 
-template <typename T>
-__device__ __forceinline__ float ld1(const T* p);
-template <>
-__device__ __forceinline__ float ld1<float>(const float* p) { return *p; }
-template <>
-__device__ __forceinline__ float ld1<uint16_t>(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
-template <typename T>
-__device__ __forceinline__ void st1(T* p, float v);
-template <>
-__device__ __forceinline__ void st1<float>(float* p, float v) { *p = v; }
-template <>
-__device__ __forceinline__ void st1<uint16_t>(uint16_t* p, float v) {
-    const __bf16 b = (__bf16)v;
-    *p = *(const uint16_t*)&b;
-}
 // 8 elements from i, n of them inside the tensor (whole: all 8, and 16-byte aligned)
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, int64_t i, int n, bool whole, float* v) {

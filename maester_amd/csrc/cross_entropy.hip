@@ -35,22 +35,6 @@ __device__ __forceinline__ float wave_max(float x) {
     return x;
 }
 
-template <typename T>
-__device__ __forceinline__ float ld1(const T* p);
-template <>
-__device__ __forceinline__ float ld1<float>(const float* p) { return *p; }
-template <>
-__device__ __forceinline__ float ld1<uint16_t>(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
-template <typename T>
-__device__ __forceinline__ void st1(T* p, float v);
-template <>
-__device__ __forceinline__ void st1<float>(float* p, float v) { *p = v; }
-template <>
-__device__ __forceinline__ void st1<uint16_t>(uint16_t* p, float v) {
-    const __bf16 b = (__bf16)v;
-    *p = *(const uint16_t*)&b;
-}
-
 // ---- arithmetic on 8 logits ------------------------------------------------------------------------
 // Everything is kept in log2 units so that an exponential is one fused multiply-add and one exp2:
 // exp(x - lse) * scale = exp2(x * log2e - (lse2 - log2 scale)).

@@ -41,11 +41,6 @@ struct GradArgs {
 
 enum Output { kInput, kStored, kAdded };      // in the operands' type; fp32, stored; fp32, added to what is there
 
-__device__ __forceinline__ u32x4 uniform_rsrc(uint64_t base, uint32_t bytes) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)base), hi = __builtin_amdgcn_readfirstlane((uint32_t)(base >> 32));
-    return tile_rsrc((uint64_t)hi << 32 | lo, __builtin_amdgcn_readfirstlane(bytes));
-}
-
 // One operand: how its step lies in a slot, which bytes a lane loads, where a lane reads its fragments.
 // ROWS: the contraction runs along its rows; otherwise its rows are those of the tile, 128 bytes of contraction a step.
 template <typename T, bool ROWS, int EDGE>

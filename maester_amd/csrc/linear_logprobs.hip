@@ -80,12 +80,6 @@ __device__ __forceinline__ bool place(const LinArgs& a, int& rb, int& split) {
     return true;
 }
 
-// descriptor of wave-uniform values, in scalar registers whatever the compiler has made of them
-__device__ __forceinline__ u32x4 uniform_rsrc(uint64_t base, uint32_t bytes) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)base), hi = __builtin_amdgcn_readfirstlane((uint32_t)(base >> 32));
-    return tile_rsrc((uint64_t)hi << 32 | lo, __builtin_amdgcn_readfirstlane(bytes));
-}
-
 template <typename T, int BN, bool CAP, bool GRAD>
 __global__ __launch_bounds__(256, 1) void linear_logprobs_kernel(const LinArgs a) {
     using L = Tiling<BN>;

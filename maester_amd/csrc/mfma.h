@@ -518,6 +518,11 @@ __device__ __forceinline__ u32x4 tile_rsrc(uint64_t base, uint32_t bytes_in_rang
     asm volatile("" : "+s"(r));
     return r;
 }
+// descriptor of wave-uniform values, in scalar registers whatever the compiler has made of them
+__device__ __forceinline__ u32x4 uniform_rsrc(uint64_t base, uint32_t bytes) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)base), hi = __builtin_amdgcn_readfirstlane((uint32_t)(base >> 32));
+    return tile_rsrc((uint64_t)hi << 32 | lo, __builtin_amdgcn_readfirstlane(bytes));
+}
 // (the same two with the LDS address given as a wave-uniform base plus a compile-time constant: the sum goes
 // straight into m0, one instruction less than adding first and moving then)
 template <int IMM>

@@ -1,5 +1,5 @@
 // Row-wise I/O helpers shared by the HBM-bound kernels (norms, cross entropy): 8 consecutive
-// elements per lane as one 16-byte (bf16) or two 16-byte (fp32) accesses, converted to and from fp32.
+// elements per lane as one 16-byte (bf16) or two 16-byte (fp32) accesses, converted to and from fp32; single elements for edges.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -39,6 +39,22 @@ __device__ __forceinline__ void st8<uint16_t>(uint16_t* p, const float* v) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = (__bf16)v[i];  // round to nearest even, like torch's cast
     *(bf16x8_v*)p = o;
+}
+// one element
+template <typename T>
+__device__ __forceinline__ float ld1(const T* p);
+template <>
+__device__ __forceinline__ float ld1<float>(const float* p) { return *p; }
+template <>
+__device__ __forceinline__ float ld1<uint16_t>(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
+template <typename T>
+__device__ __forceinline__ void st1(T* p, float v);
+template <>
+__device__ __forceinline__ void st1<float>(float* p, float v) { *p = v; }
+template <>
+__device__ __forceinline__ void st1<uint16_t>(uint16_t* p, float v) {
+    const __bf16 b = (__bf16)v;
+    *p = *(const uint16_t*)&b;
 }
 // what a value becomes when it is stored in T and read back
 template <typename T>

@@ -29,22 +29,6 @@ constexpr int kLpThreads = 512;       // >= 8 * MA_LOGPROBS_MAX_TOP: the waves' 
 constexpr int kLpWaves = kLpThreads / 64;
 constexpr int kLpMaxParts = 64;       // of a row: a lane each in the join
 
-template <typename T>
-__device__ __forceinline__ float ld1(const T* p);
-template <>
-__device__ __forceinline__ float ld1<float>(const float* p) { return *p; }
-template <>
-__device__ __forceinline__ float ld1<uint16_t>(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
-template <typename T>
-__device__ __forceinline__ void st1(T* p, float v);
-template <>
-__device__ __forceinline__ void st1<float>(float* p, float v) { *p = v; }
-template <>
-__device__ __forceinline__ void st1<uint16_t>(uint16_t* p, float v) {
-    const __bf16 b = (__bf16)v;
-    *p = *(const uint16_t*)&b;
-}
-
 // A row in groups of 8 elements whose full groups start on a 16-byte boundary wherever the row itself
 // starts: group g holds elements [8 g - shift, 8 g - shift + 8) cut to [0, vocab).
 template <typename T>
