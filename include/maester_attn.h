@@ -260,7 +260,8 @@ int ma_linear_counted_rows(const void* e, int64_t e_stride, const int64_t* targe
  * clipping in train.py).  With c the clip factor and t the step counter after its increment:
  *   g = c g;  m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2
  *   p = p (1 - lr wd) - lr / (1-b1^t) * m / (sqrt(v) / sqrt(1-b2^t) + eps)
- * evaluated in fp32 in this order, from `master` where one is given (then param is its rounding).
+ * in fp32, from `master` where one is given (then param is its rounding): m and v operation by operation
+ * as written, p with the quotient as a product with a reciprocal that is a last place off at most.
  * state_bits 32: exp_avg = m, exp_avg_sq = v, fp32 [n].  state_bits 8: exp_avg = m and exp_avg_sq =
  * sqrt(v) as e4m3 codes [n], with scales fp32 [ceil(n / MA_ADAMW_BLOCK)]: element i is code i *
  * scale[i / MA_ADAMW_BLOCK].  The scale is the smallest power of two that brings the block's largest

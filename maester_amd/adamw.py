@@ -5,7 +5,7 @@ The step that applies what ``loss.backward()`` left: the reference builds torch'
 both in a few launches, without a host synchronisation: ``adamw_step`` on lists of tensors, ``AdamW`` as a
 ``torch.optim.Optimizer``, ``global_grad_norm`` for the norm alone.
 
-8-bit states (a quarter of the memory, 4.06 instead of 16 bytes moved per element and step): exp_avg and the square root
+8-bit states (a quarter of the memory, 4.13 instead of 16 bytes moved per element and step): exp_avg and the square root
 of exp_avg_sq as ``torch.float8_e4m3fn`` values with one power-of-two scale per 128 consecutive elements, rounded
 stochastically from a hash of (seed, step, index of the tensor, element): the same call twice gives the same bits.
 """

@@ -27,7 +27,7 @@ HIPCC_FLAGS = [
     "-Wall", "-Wno-unused-function",
 ]
 
-# sources whose results are those of their formulas in IEEE single precision, operation by operation
+# sources whose results are those of their formulas in IEEE single precision, operation by operation (but for what they say)
 EXACT_SOURCES = {"adamw.hip"}
 EXACT_FLAGS = ["-fno-fast-math", "-ffp-contract=off"]
 

@@ -12,7 +12,8 @@
 // never move.  The 16 random bits per rounding come from a hash of (seed, t, tensor, element), so a step is a function of
 // its inputs.  A nonzero r is never rounded to zero: m / (0 + eps) would be a jump of any size.  Scaling by powers of two
 // is exact, and the file is compiled without contraction or reassociation, square roots are rounded correctly (roots8), so
-// that the codes are those of the formula in IEEE single precision, operation by operation.
+// that the states, in 32 and in 8 bits, are those of the formula in IEEE single precision, operation by operation.  A
+// parameter's quotient alone is a product with the hardware's reciprocal, a last place off at most (step8).
 #include <hip/hip_runtime.h>
 
 #include "common.h"

@@ -107,7 +107,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
                    softcap: float | None = None, temperature: float = 1.0) -> TokenLogprobs:
     """Log-probability of every target, entropy and the ``top_k`` (at most 64) best alternatives of rows of logits.
 
-    ``logits`` ``[..., V]`` bf16 or fp32, ``targets`` int64 of the leading shape.  Logits are capped as
+    ``logits`` ``[..., V]`` bf16 or fp32, ``targets`` int64 of the leading shape.  Entries of a row are neighbours in memory (a
+    transposed matrix is refused); rows may lie apart, anywhere, in a matrix, while more dimensions whose rows are not
+    evenly spaced, such as ``logits[:, :-1]`` of a batch, are copied first.  Logits are capped as
     ``softcap * tanh(x / softcap)`` where a cap is given, then divided by ``temperature``.  Rows whose target is
     ``ignore_index`` (or outside the vocabulary) get 0 for both and no gradient; the alternatives come for every row,
     equal logits in the order of their index.  Logits of ``-inf`` have probability 0 (a soft cap makes them
