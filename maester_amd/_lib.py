@@ -214,7 +214,11 @@ def refuse_tangents(what: str, *tensors: torch.Tensor) -> None:
 
 def require_plain(what: str, *tensors) -> None:
     """Refuses tensors that wrap others (``DTensor`` and the like): they have no memory of their own to hand to a kernel."""
-    for kind in set(map(type, tensors)) - _PLAIN:
+    require_plain_types(what, set(map(type, tensors)))
+
+
+def require_plain_types(what: str, kinds: set) -> None:
+    for kind in kinds - _PLAIN:
         if hasattr(kind, "__tensor_flatten__"):
             raise TypeError(f"{what} takes plain tensors, got {kind.__name__} (of a sharded tensor: its local part)")
 

@@ -56,15 +56,15 @@ def _device(tensors, who: str) -> torch.device:
     return tensors[0].device
 
 
-def _addresses(tensors, what: str, shapes: list, dtypes: frozenset, dev: torch.device) -> list:
-    """Data pointers of ``tensors`` after checking them against the parameters' shapes and device (whole lists at a time:
-    a step over hundreds of small tensors is as fast as its host code)."""
+def _addresses(tensors, what: str, shapes: list, dtypes: frozenset, dev: torch.device | None) -> list:
+    """Data pointers of ``tensors`` after checking them against the parameters' shapes and device (None: checked already;
+    whole lists at a time: a step over hundreds of small tensors is as fast as its host code)."""
     found = set(map(_dtype, tensors))
     if not found <= dtypes:
         raise TypeError(f"{what} must be {' or '.join(sorted(map(str, dtypes)))}, got {', '.join(sorted(map(str, found - dtypes)))}")
     if list(map(_shape, tensors)) != shapes or not all(map(torch.Tensor.is_contiguous, tensors)):
         raise ValueError(f"{what} must be contiguous and of its parameter's shape")
-    if set(map(torch.Tensor.get_device, tensors)) != {dev.index}:
+    if dev is not None and set(map(torch.Tensor.get_device, tensors)) != {dev.index}:
         raise ValueError(f"{what} must be on its parameter's device {dev}")
     return list(map(torch.Tensor.data_ptr, tensors))
 
@@ -135,15 +135,15 @@ in place (a backward through a graph that saved it before the step raises)."""
         raise ValueError("max_grad_norm must be >= 0 and cannot be given together with clip")
     if not 0 <= int(seed) < 1 << 32:
         raise ValueError("seed must be in [0, 2^32)")
-    _lib.require_plain("adamw_step", *params, *grads, *exp_avgs, *exp_avg_sqs, *masters)
+    kinds = set(map(type, exp_avgs)) | set(map(type, exp_avg_sqs))
+    _lib.require_plain_types("adamw_step", kinds.union(map(type, params), map(type, grads), map(type, masters)))
     _lib.refuse_tangents("adamw_step", *params, *grads)
     dev = _device(params, "adamw_step")
-    kinds = set(map(type, exp_avgs)) | set(map(type, exp_avg_sqs))
     eight = Blocks8 in kinds
     if eight and len(kinds) > 1:
         raise ValueError("exp_avgs and exp_avg_sqs must all be tensors or all Blocks8")
     shapes, sizes = list(map(_shape, params)), list(map(torch.Tensor.numel, params))
-    where = _addresses(params, "a parameter", shapes, _ACTIVATION, dev)
+    where = _addresses(params, "a parameter", shapes, _ACTIVATION, None)
     columns = dict(param=where, grad=_addresses(grads, "a gradient", shapes, _ACTIVATION, dev))
     for name, states in (("exp_avg", exp_avgs), ("exp_avg_sq", exp_avg_sqs)):
         if eight:
