@@ -48,7 +48,7 @@ def token_logprobs_forward(logits, targets, top_k=0, ignore_index=-100, softcap=
         raise ValueError(f"top_k must be in 0 .. {_lib.MA_LOGPROBS_MAX_TOP} and at most the vocabulary of {vocab}, got {top_k}")
     softcap, temperature = check_softmax_arguments(softcap, temperature)
     code = _lib.dtype_code(logits.dtype)
-    targets = targets.contiguous()
+    logits, targets = _apart(logits), targets.contiguous()
     logp, entropy = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2))
     stats = torch.empty(rows, 2, dtype=torch.float32, device=dev) if need_stats else None
     top_ids = torch.empty(rows, top_k, dtype=torch.int64, device=dev) if top_k else None
@@ -64,6 +64,11 @@ def token_logprobs_forward(logits, targets, top_k=0, ignore_index=-100, softcap=
     return logp, entropy, stats, top_ids, top_logp
 
 
+def _apart(x: torch.Tensor) -> torch.Tensor:
+    """``x`` itself, or a copy where its rows share memory (a broadcast row)."""
+    return x.contiguous() if x.shape[0] > 1 and x.stride(0) < x.shape[1] else x
+
+
 def _row_pitch(x: torch.Tensor) -> int:
     """Elements between rows (a single row has no meaningful stride)."""
     return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
@@ -72,7 +77,7 @@ def _row_pitch(x: torch.Tensor) -> int:
 def token_logprobs_backward(logits, targets, stats, entropy, dlogp, dentropy, ignore_index=-100, softcap=None, temperature=1.0):
     """Gradient of the logits, contiguous, from those of ``logp`` and ``entropy`` (either may be None)."""
     softcap, temperature = check_softmax_arguments(softcap, temperature)
-    targets = targets.contiguous()
+    logits, targets = _apart(logits), targets.contiguous()
     dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     rows, vocab = logits.shape
     dlogp, dentropy = (None if t is None else t.float().contiguous() for t in (dlogp, dentropy))
@@ -109,7 +114,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
 
     ``logits`` ``[..., V]`` bf16 or fp32, ``targets`` int64 of the leading shape.  Entries of a row are neighbours in memory (a
     transposed matrix is refused); rows may lie apart, anywhere, in a matrix, while more dimensions whose rows are not
-    evenly spaced, such as ``logits[:, :-1]`` of a batch, are copied first.  Logits are capped as
+    evenly spaced, such as ``logits[:, :-1]`` of a batch, and rows that share memory are copied first.  Logits are capped as
     ``softcap * tanh(x / softcap)`` where a cap is given, then divided by ``temperature``.  Rows whose target is
     ``ignore_index`` (or outside the vocabulary) get 0 for both and no gradient; the alternatives come for every row,
     equal logits in the order of their index.  Logits of ``-inf`` have probability 0 (a soft cap makes them
