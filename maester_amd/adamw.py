@@ -124,7 +124,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     with the global norm of this call's, which is returned as an fp32 scalar on the device; ``clip``: an fp32 factor on the
     device to scale by instead.  A gradient that is not finite makes its element (8-bit states: its block of 128) NaN, or
     all of them through the norm.  ``seed`` picks the random bits of the 8-bit rounding.  All that is written counts as modified
-in place (a backward through a graph that saved it before the step raises)."""
+    in place (a backward through a graph that saved it before the step raises)."""
     n = len(params)
     masters = [None] * n if masters is None else masters
     if not len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(masters) == n:
@@ -319,11 +319,11 @@ class AdamW(torch.optim.Optimizer):
                                   f"bias correction of step {max(steps)}", stacklevel=2)
                 group.update(state_bits=32, master_weights=self.defaults["master_weights"], seed=self.defaults["seed"],
                              step=max(steps, default=0))
-            dev = group["params"][0].device
-            if "step" in group:
-                group["step"] = torch.as_tensor(group["step"]).to(dev, torch.int64)
-            if isinstance(group["lr"], torch.Tensor):
-                group["lr"] = group["lr"].detach().to(dev, torch.float32)
+            for dev in {p.device for p in group["params"]}:          # (one, or none in an empty group)
+                if "step" in group:
+                    group["step"] = torch.as_tensor(group["step"]).to(dev, torch.int64)
+                if isinstance(group["lr"], torch.Tensor):
+                    group["lr"] = group["lr"].detach().to(dev, torch.float32)
             for i, p in zip(old["params"], group["params"]):
                 if i not in saved:
                     continue

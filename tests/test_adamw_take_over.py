@@ -87,3 +87,12 @@ def test_a_state_of_ours_with_unknown_bits(bits):
     state["param_groups"][0]["state_bits"] = bits
     with pytest.raises(ValueError, match="state_bits"):
         ours.load_state_dict(state)
+
+
+def test_a_group_without_parameters():
+    p = torch.nn.Parameter(torch.ones(4))
+    make = lambda: AdamW([{"params": [p]}, {"params": [], "lr": torch.tensor(0.5)}])  # noqa: E731
+    state = copy.deepcopy(make().state_dict())
+    ours = make()
+    ours.load_state_dict(state)
+    assert ours.param_groups[1]["params"] == [] and float(ours.param_groups[1]["lr"]) == 0.5
